@@ -263,6 +263,111 @@ typedef struct tde_device_info_out {
 } tde_device_info_out;
 int tde_device_info(tde_device_info_out *out);
 
+/* ---- operators of the attention block behind the norm ------------------------------------------
+   What a rank runs between two of its reduce-and-normalize stages: the product that takes the int8 codes and scales
+   of TDE_QUANT_INT8_TOKEN, norms and rotation of query and key heads, appending keys and values to a paged cache, and
+   the attention over it.  No counterpart in the reference, which ends at the normed rows.
+   As above: nothing synchronizes, nothing allocates, every launch goes to `hip_stream` of the current device, and a
+   call may be captured into a graph.  Structures must be zero-initialized before their fields are set; `reserved` is checked. */
+
+/* y[t][n] = T( float(sum_k codes[t][k] * weight[n][k]) * (scales[t] * weight_scales[n]) + bias[n] ), T = out_dtype.
+   codes [tokens, k] and weight [n, k] int8, scales [tokens], weight_scales [n] and bias [n] fp32 (bias may be null), out
+   [tokens, n]; all contiguous, no alignment beyond the element's.  The sum is exact, hence k <= TDE_INT8_MAX_K (TDE_EHIDDEN). */
+#define TDE_INT8_MAX_K 131071
+typedef struct tde_int8_product {
+    int64_t tokens, k, n; /* tokens, n >= 0, k >= 1 */
+    int32_t out_dtype;    /* TDE_BF16, TDE_F16, TDE_F32 */
+    int32_t reserved;     /* must be 0 */
+    const int8_t *codes, *weight;
+    const float *scales, *weight_scales, *bias;
+    void *out;            /* must not overlap an input */
+} tde_int8_product;
+int tde_int8_linear(const tde_int8_product *product, void *hip_stream);
+
+/* Rows of heads: element (row r, head h, channel d) at data[r * row_stride + h * head_stride + d]; strides in elements. */
+typedef struct tde_heads {
+    void *data;
+    int64_t row_stride, head_stride;
+} tde_heads;
+
+/* A paged cache of keys or of values: channel d of head h in slot s of page p at
+   data[p * page_stride + s * slot_stride + h * head_stride + d]; strides in elements. */
+typedef struct tde_cache {
+    void *data;
+    int64_t page_stride, slot_stride, head_stride;
+} tde_cache;
+
+/* A ragged batch over a paged cache (device arrays).  Sequence b has the call's rows q_starts[b] .. q_starts[b+1] and kv_lens[b]
+   keys in the cache, those of its new rows included: row q_starts[b] + i has position kv_lens[b] - new_b + i, and key j of
+   the sequence lies in slot j % page_size of page page_table[b][j / page_size].
+   The contents are not checked on the host and cannot lead a kernel out of bounds:
+   - rows from q_starts[seqs] on belong to no sequence; rows of a sequence with fewer keys than rows may have a negative position;
+   - a page number outside [0, cache_pages), or a key beyond the table's row, names no page;
+   - q_starts is expected to ascend within [0, tokens]; where it does not, what the rows concerned get is unspecified. */
+typedef struct tde_paged_batch {
+    const int32_t *page_table; /* [seqs, table_pages] */
+    const int32_t *q_starts;   /* [seqs + 1] */
+    const int32_t *kv_lens;    /* [seqs] */
+    int64_t table_stride;      /* elements from one row of page_table to the next */
+    int32_t seqs, table_pages, cache_pages, page_size;
+} tde_paged_batch;
+
+/* Norm and rotation of heads.  With u = x / sqrt(mean(x^2) + eps) * gamma (u = x without a gamma), rotated pairs (a, b) of u become
+   (a cos - b sin, b cos + a sin): pairs of channels (d, d + rot_dim/2), or (2d, 2d + 1) if interleaved, d < rot_dim/2; channels
+   from rot_dim on are not rotated.  All in fp32, rounded to `dtype` once.  cos_sin row p holds the cosines and then the sines of
+   position p; a position outside the table makes the rotated channels NaN. */
+typedef struct tde_head_rows {
+    int32_t dtype;              /* TDE_BF16, TDE_F16, TDE_F32 */
+    int32_t dim;                /* channels of a head, 1 .. TDE_MAX_HEAD_DIM */
+    int32_t rot_dim;            /* even, 0 .. dim; 0: no rotation (cos_sin may be null) */
+    int32_t interleaved;        /* 0/1 */
+    int32_t q_heads, kv_heads;
+    int64_t tokens;
+    float eps;
+    int32_t positions_bytes;    /* 4 or 8: the integers in `positions` */
+    const void *positions;      /* [tokens]; tde_append_kv: may be null, the rows' positions in the cache then */
+    const float *cos_sin;       /* [cos_sin_rows, rot_dim] */
+    int64_t cos_sin_rows, cos_sin_stride;
+    const void *q_gamma, *k_gamma; /* [dim] of `dtype`, or null */
+    tde_heads q, k, v;             /* inputs: tde_qk_norm_rope q, k; tde_append_kv k, v and, if q_heads > 0, q */
+    tde_heads q_out, k_out;        /* outputs, not overlapping the inputs: q_out; k_out of tde_qk_norm_rope */
+    tde_cache k_cache, v_cache;    /* tde_append_kv: kv_heads heads */
+    tde_paged_batch batch;         /* tde_append_kv */
+    int64_t reserved;              /* must be 0 */
+} tde_head_rows;
+#define TDE_MAX_HEAD_DIM 1024
+int tde_qk_norm_rope(const tde_head_rows *rows, void *hip_stream);
+
+/* k, normed and rotated, and v as it is, into their slots of the caches; with q_heads > 0 the queries, normed and rotated, to q_out
+   in the same launch.  Rows without a position, and rows whose page does not exist, change nothing in the caches; q_out's rows
+   without a position become zeros.  Two rows of one call with one slot (a page named twice) leave either's channels in it. */
+int tde_append_kv(const tde_head_rows *rows, void *hip_stream);
+
+/* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] over the keys j of the row's sequence up to its own position, for every query head;
+   key head h serves query heads h * q_heads / kv_heads and the following.  Scores, softmax and sums in fp32, the weights rounded to
+   `dtype` for the product with the values.  What the caches hold in slots that a row does not see -- behind a
+   sequence's last key, or later rows of the call -- does not reach it, whatever it is.  A key without a page makes the rows that see
+   it NaN.  Rows without a position (see tde_paged_batch) become zeros; rows behind the last sequence become zeros if zero_tail, else
+   they are left as they are. */
+typedef struct tde_attention {
+    int32_t dtype;            /* TDE_BF16, TDE_F16 */
+    int32_t dim;              /* a multiple of 8, 8 .. 256 (TDE_ESHAPE, TDE_EHIDDEN) */
+    int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads */
+    int64_t tokens;
+    float scale;              /* > 0, finite */
+    int32_t zero_tail;        /* 0/1 */
+    tde_heads q, out;         /* out must not overlap q */
+    tde_cache k_cache, v_cache; /* data and strides multiples of 16 bytes (TDE_EALIGN); page and slot strides
+                                   below 2^32 bytes (TDE_ESHAPE) */
+    tde_paged_batch batch;
+    void *workspace;          /* tde_paged_attention_workspace bytes, 16-byte aligned; of this call alone until it has run */
+    int64_t workspace_bytes;
+    int64_t reserved;         /* must be 0 */
+} tde_attention;
+/* Pure host: bytes of workspace that the problem needs on the current device (often 0); depends on sizes alone. */
+int tde_paged_attention_workspace(const tde_attention *attention, int64_t *bytes);
+int tde_paged_attention(const tde_attention *attention, void *hip_stream);
+
 /* ---- emulated peer workspace ----------------------------------------------------------------
    One allocation per emulated rank plays the role of that rank's IPC-mapped comm buffer
    (CommWorkspace, src/ops/all_reduce_fusion.cpp:63-96).  Each slot is 2*slot_bytes large: the

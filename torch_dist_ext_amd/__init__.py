@@ -136,3 +136,25 @@ def reduce_rms(partials, residual_in, rms_gamma, eps, quant_mode=QUANT_NONE, wri
 
 
 allreduce_rms = torch.ops.torch_dist_ext.allreduce_rms
+
+# The attention block behind the norm, registered by the C++ library (CUDA and Meta kernels; the outputs are plain tensors).
+#
+#   int8_linear(codes, scales, weight, weight_scales, bias=None, out_dtype=bf16) -> [..., n]
+#     codes [..., k] int8 and their scales as allreduce_rms_quant(QUANT_INT8_TOKEN) returns them, weight [n, k] int8 with a scale a
+#     channel, bias [n] fp32; out_dtype bf16, fp16 or fp32.
+#   qk_norm_rope(q, k, q_gamma, k_gamma, eps, positions, cos_sin, interleaved=False) -> (q_out, k_out)
+#     q [tokens, heads, dim], k [tokens, kv_heads, dim]: RMSNorm of every head, then the rotation by cos_sin [positions, rot_dim] fp32
+#     (cosines, then sines) at the token's position.  Views into one projection's output are fine.
+#   append_kv(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos_sin=None, positions=None, q=None, q_gamma=None,
+#             k_gamma=None, eps=1e-6, interleaved=False) -> q_out or None
+#     keys, normed (with k_gamma) and rotated (with cos_sin), and values into caches [pages, page_size, kv_heads, dim]; the queries
+#     likewise in the same launch.  Sequence b has the rows q_starts[b]:q_starts[b + 1] and kv_lens[b] keys with these; page_table
+#     [sequences, pages] int32 names its pages.
+#   paged_attention(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale=None) -> [tokens, heads, dim]
+#     causal attention of the new rows over their sequences' keys, bf16 or fp16; scale defaults to dim ** -0.5.  Rows behind the last
+#     sequence become zeros; paged_attention_out(..., out, scale=None) writes to `out` and leaves them as they are.
+int8_linear = torch.ops.torch_dist_ext.int8_linear.default
+qk_norm_rope = torch.ops.torch_dist_ext.qk_norm_rope.default
+append_kv = torch.ops.torch_dist_ext.append_kv.default
+paged_attention = torch.ops.torch_dist_ext.paged_attention.default
+paged_attention_out = torch.ops.torch_dist_ext.paged_attention_out.default

@@ -24,7 +24,8 @@ TORCH_LIB = os.path.join(ROOT, "libtorch_dist_ext.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIP_SOURCES = ["tde_abi.hip", "tde_rows_bf16.hip", "tde_rows_f16.hip", "tde_rows_f32.hip", "tde_rows_f64.hip", "tde_shifted_rows_bf16.hip", "tde_shifted_rows_f16.hip",
-               "tde_shifted_rows_f32.hip", "tde_converted_rows_f16.hip", "tde_short_rows.hip", "tde_probe.hip"]
+               "tde_shifted_rows_f32.hip", "tde_converted_rows_f16.hip", "tde_short_rows.hip", "tde_probe.hip", "tde_block_abi.hip", "tde_int8_linear.hip",
+               "tde_head_rows.hip", "tde_paged_attention.hip"]
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
     # keep fp32 arithmetic scalar: packed fp32 forms are not used on this hardware pool
@@ -84,7 +85,7 @@ def build_torch(verbose=False):
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi,
         "-I", INCLUDE, "-isystem", os.path.join(ROCM, "include"),
     ] + inc + [
-        os.path.join(CSRC, "tde_torch.cpp"), "-o", TORCH_LIB,
+        os.path.join(CSRC, "tde_torch.cpp"), os.path.join(CSRC, "tde_block_torch.cpp"), "-o", TORCH_LIB,
         "-L", PKG_DIR, "-ltde_hip", "-L", torch_lib_dir, "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_hip",
         "-Wl,-rpath,$ORIGIN/torch_dist_ext_amd", "-Wl,-rpath," + torch_lib_dir, "-Wl,--no-as-needed",
     ]

@@ -25,6 +25,7 @@ EXPORTS = (
     "tde_probe_copy", "tde_probe_launch", "tde_probe_stream", "tde_probe_rows", "tde_probe_rows_parts", "tde_device_info",
     "tde_workspace_create", "tde_workspace_destroy", "tde_workspace_slot", "tde_workspace_stage",
     "tde_workspace_slot_bytes", "tde_workspace_nranks", "tde_workspace_fill_table",
+    "tde_int8_linear", "tde_qk_norm_rope", "tde_append_kv", "tde_paged_attention", "tde_paged_attention_workspace",
 )
 
 
@@ -67,6 +68,52 @@ class DeviceInfo(ctypes.Structure):
     _fields_ = [
         ("compute_units", ctypes.c_int32), ("memory_clock_khz", ctypes.c_int32), ("memory_bus_bits", ctypes.c_int32),
         ("reserved", ctypes.c_int32), ("total_memory_bytes", ctypes.c_int64),
+    ]
+
+
+INT8_MAX_K, MAX_HEAD_DIM = 131071, 1024
+
+
+class Int8Product(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("k", ctypes.c_int64), ("n", ctypes.c_int64), ("out_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("codes", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("weight_scales", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
+    ]
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("seqs", ctypes.c_int32), ("table_pages", ctypes.c_int32), ("cache_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+    ]
+
+
+class HeadRows(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("tokens", ctypes.c_int64), ("eps", ctypes.c_float),
+        ("positions_bytes", ctypes.c_int32), ("positions", ctypes.c_void_p), ("cos_sin", ctypes.c_void_p),
+        ("cos_sin_rows", ctypes.c_int64), ("cos_sin_stride", ctypes.c_int64), ("q_gamma", ctypes.c_void_p), ("k_gamma", ctypes.c_void_p),
+        ("q", Heads), ("k", Heads), ("v", Heads), ("q_out", Heads), ("k_out", Heads), ("k_cache", Cache), ("v_cache", Cache),
+        ("batch", PagedBatch), ("reserved", ctypes.c_int64),
+    ]
+
+
+class Attention(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("dim", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("tokens", ctypes.c_int64), ("scale", ctypes.c_float), ("zero_tail", ctypes.c_int32), ("q", Heads), ("out", Heads),
+        ("k_cache", Cache), ("v_cache", Cache), ("batch", PagedBatch), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64), ("reserved", ctypes.c_int64),
     ]
 
 
@@ -127,6 +174,12 @@ def load():
     lib.tde_workspace_nranks.argtypes = [ctypes.c_void_p]
     lib.tde_workspace_fill_table.restype = ctypes.c_int
     lib.tde_workspace_fill_table.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p), ctypes.c_int32]
+    for fn, struct in ((lib.tde_int8_linear, Int8Product), (lib.tde_qk_norm_rope, HeadRows), (lib.tde_append_kv, HeadRows),
+                       (lib.tde_paged_attention, Attention)):
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+    lib.tde_paged_attention_workspace.restype = ctypes.c_int
+    lib.tde_paged_attention_workspace.argtypes = [ctypes.POINTER(Attention), ctypes.POINTER(ctypes.c_int64)]
     _lib = lib
     return lib
 

@@ -10,6 +10,7 @@
 #include <new>
 
 #include "tde_abi.h"
+#include "tde_block.h"
 #include "tde_rows.h"
 
 // Stage buffer of tde_reduce_rms_static_stage: part of the library's device image, one copy per GPU, held
@@ -657,6 +658,11 @@ __global__ void __launch_bounds__(256) stream_kernel(const void *src, void *dst,
 
 } // namespace
 
+namespace tde {
+int hip_failed(hipError_t e) { return hip_fail(e); }
+int device_compute_units() { return compute_units(); }
+} // namespace tde
+
 struct tde_workspace {
     int32_t nranks;
     int32_t nblocks;
@@ -676,9 +682,9 @@ const char *tde_status_string(int status) {
     case TDE_EINVAL: return "invalid argument (null pointer or malformed struct)";
     case TDE_ENRANKS: return "nranks must be 2, 4 or 8";
     case TDE_EDTYPE: return "unsupported dtype (bf16, f16, f32, f64)";
-    case TDE_ESHAPE: return "bad shape: hidden*elem_size must be a positive multiple of 16 bytes, tokens >= 0";
-    case TDE_EHIDDEN: return "hidden too large for the one-pass row kernel (max 1024 16-byte vectors per row: 8192 bf16/f16, 4096 f32, 2048 f64)";
-    case TDE_EALIGN: return "buffer not 16-byte aligned";
+    case TDE_ESHAPE: return "bad shape: hidden*elem_size must be a positive multiple of 16 bytes, tokens >= 0; sizes, head counts or strides out of range";
+    case TDE_EHIDDEN: return "hidden too large for the one-pass row kernel (max 1024 16-byte vectors per row: 8192 bf16/f16, 4096 f32, 2048 f64), the int8 product (k) or a head";
+    case TDE_EALIGN: return "buffer (or a cache's strides) not 16-byte aligned";
     case TDE_EQUANT: return "bad quant mode, per-group quant with hidden not a multiple of 128, or static scale not > 0";
     case TDE_EALGO: return "bad algorithm, or staged algorithm without a stage buffer";
     case TDE_EHIP: return "HIP runtime error (see tde_last_hip_error)";

@@ -1,0 +1,306 @@
+// Rows of one head each: RMSNorm over the head's channels, the position rotation, and where the row goes -- a dense output or a slot
+// of a paged cache.  One kernel family serves tde_qk_norm_rope and tde_append_kv.
+//
+//   u = x * 1/sqrt(mean(x^2) + eps) * gamma       in fp32 (left out without a gamma)
+//   (a, b) -> (a cos - b sin, b cos + a sin)      for the rotated channels' pairs: (d, d + rot/2), or (2d, 2d + 1) if interleaved
+//   T(.)                                          one rounding, at the end; the sum of squares is held in fp32
+//
+// Bound by memory: every row is read and written once.  A row's chunks of 16 bytes (8 where the head's length or the rotation's
+// halves need it) lie in neighbouring lanes, so several rows share a wavefront and the partner of a chunk in the other half
+// of the rotation is a lane of the same wavefront.  All rows of a wavefront belong to one token: its position, its row of the
+// rotation's table and its page are looked up once, with scalar or shared loads, while the rows are on their way.
+#include "tde_block.h"
+#include "tde_head_rows.h"
+
+namespace tde {
+namespace block {
+
+// The token's place: its sequence's cache position and the slot's page.  position < 0: the row belongs to no sequence's range (it
+// lies behind the last one, or its sequence is shorter than its new tokens).
+struct Place {
+    int64_t position;
+    int32_t page, slot; // page < 0: not in the cache
+};
+
+__device__ __forceinline__ Place place_of(const PagedBatch &b, int64_t token, int lane) {
+    Place p{-1, -1, 0};
+    const int seq = __builtin_amdgcn_readfirstlane(sequence_of(b, token, lane));
+    if (seq >= b.seqs) return p;
+    const int64_t begin = b.starts[seq], end = b.starts[seq + 1], len = b.lens[seq];
+    if (token < begin) return p;
+    p.position = len - (end - begin) + (token - begin);
+    if (p.position < 0) return p;
+    if (p.position > 0x7fffffff) return p; // only where starts do not ascend
+    const uint32_t at = b.page.quotient((uint32_t)p.position);
+    p.slot = (int32_t)((uint32_t)p.position - at * b.page.d);
+    p.page = page_number(b, b.table + seq * b.table_stride, at);
+    return p;
+}
+
+__device__ __forceinline__ int64_t explicit_position(const HeadRowsArgs &a, int64_t token) {
+    return a.positions_wide ? ((const int64_t *)a.positions)[token] : (int64_t)((const int32_t *)a.positions)[token];
+}
+
+// Address of head `h` of class `cls` (0 query, 1 key, 2 value) in the outputs; null where the row is not stored.
+template <bool PAGED>
+__device__ __forceinline__ char *destination(const HeadRowsArgs &a, const Place &place, int64_t token, int cls, int h) {
+    if (!PAGED || cls == 0) return a.out[cls] + token * a.out_token[cls] + h * a.out_head[cls];
+    if (place.page < 0) return nullptr;
+    return a.out[cls] + place.page * a.out_page[cls] + place.slot * a.out_token[cls] + h * a.out_head[cls];
+}
+
+template <class T, int VE, int R, bool INTERLEAVED, bool PAGED>
+__global__ void __launch_bounds__(256) head_rows_kernel(const HeadRowsArgs a) {
+    constexpr int BYTES = VE * T::kBytes;
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t row = a.waves_per_token.quotient(wave);
+    const int64_t token = row;
+    if (token >= a.tokens) return;
+    const int part = (int)(wave - row * a.waves_per_token.d);
+    const int rows_at_once = 64 >> a.lanes_log2;
+    const int chunk = lane & ((1 << a.lanes_log2) - 1);
+    const int d0 = chunk * VE;
+    const bool active = d0 < a.dim;
+    const int heads = a.heads[0] + a.heads[1] + a.heads[2];
+
+    Words<BYTES> raw[R];
+    int cls[R], head[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        int h = (part * R + r) * rows_at_once + (lane >> a.lanes_log2);
+        const bool there = active && h < heads;
+        cls[r] = h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2);
+        h -= cls[r] == 0 ? 0 : (cls[r] == 1 ? a.heads[0] : a.heads[0] + a.heads[1]);
+        head[r] = there ? h : -1;
+        const char *src = cls[r] == 0 ? a.in[0] : (cls[r] == 1 ? a.in[1] : a.in[2]);
+        const int64_t per_token = cls[r] == 0 ? a.in_token[0] : (cls[r] == 1 ? a.in_token[1] : a.in_token[2]);
+        const int64_t per_head = cls[r] == 0 ? a.in_head[0] : (cls[r] == 1 ? a.in_head[1] : a.in_head[2]);
+        if (there) raw[r] = load_words<BYTES>(src + token * per_token + h * per_head + d0 * T::kBytes);
+        else raw[r] = Words<BYTES>{};
+    }
+
+    Place place{0, -1, 0};
+    if (PAGED) place = place_of(a.batch, token, lane);
+    const bool placed = !PAGED || place.position >= 0;
+    const int64_t position = a.positions != nullptr ? explicit_position(a, token) : place.position;
+
+    // cosines and sines of this lane's chunk; outside the table they are NaN, and so become the rotated channels
+    const int rot = 2 * a.half;
+    const bool turned = active && d0 < rot;
+    float cs[VE], sn[VE];
+    {
+        const bool known = position >= 0 && position < a.table_rows;
+        const float *row_of = a.cos_sin + (known ? position : 0) * a.table_stride;
+        constexpr int N = INTERLEAVED ? VE / 2 : VE;
+        const int j = INTERLEAVED ? d0 / 2 : (d0 < a.half ? d0 : d0 - a.half);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            cs[i] = 1.0f;
+            sn[i] = 0.0f;
+        }
+        if (turned) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                cs[i] = known ? row_of[j + i] : __builtin_nanf("");
+                sn[i] = known ? row_of[a.half + j + i] : __builtin_nanf("");
+            }
+        }
+    }
+    float gamma_q[VE], gamma_k[VE];
+    {
+        Words<BYTES> g{};
+        if (active && a.gamma[0] != nullptr) g = load_words<BYTES>(a.gamma[0] + d0 * T::kBytes);
+        widen_all<T, VE>(g, gamma_q);
+        if (active && a.gamma[1] != nullptr) g = load_words<BYTES>(a.gamma[1] + d0 * T::kBytes);
+        widen_all<T, VE>(g, gamma_k);
+    }
+
+    // the lane of the partner chunk
+    const int partner = INTERLEAVED || !turned ? lane : (d0 < a.half ? lane + a.half / VE : lane - a.half / VE);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float x[VE];
+        widen_all<T, VE>(raw[r], x);
+        const bool normed = cls[r] == 0 ? a.gamma[0] != nullptr : (cls[r] == 1 && a.gamma[1] != nullptr);
+        if (a.gamma[0] != nullptr || a.gamma[1] != nullptr) {
+            float sq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) sq = __builtin_fmaf(x[i], x[i], sq);
+            sq = sum_over_lanes(sq, a.lanes_log2);
+            const float scale = 1.0f / __builtin_sqrtf(sq / (float)a.dim + a.eps);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) x[i] = normed ? x[i] * scale * (cls[r] == 0 ? gamma_q[i] : gamma_k[i]) : x[i];
+        }
+        if (rot != 0) {
+            float y[VE];
+            if constexpr (INTERLEAVED) {
+#pragma unroll
+                for (int i = 0; i < VE / 2; ++i) {
+                    y[2 * i] = __builtin_fmaf(x[2 * i], cs[i], -(x[2 * i + 1] * sn[i]));
+                    y[2 * i + 1] = __builtin_fmaf(x[2 * i + 1], cs[i], x[2 * i] * sn[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    const float other = __shfl(x[i], partner);
+                    const float s = other * sn[i];
+                    y[i] = __builtin_fmaf(x[i], cs[i], d0 < a.half ? -s : s);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) x[i] = turned ? y[i] : x[i];
+        }
+        if (head[r] < 0) continue;
+        Words<BYTES> out = narrow_all<T, VE>(x);
+        if (cls[r] == 2) out = raw[r]; // values go as they are
+        if (!placed) {
+            if (cls[r] != 0) continue;
+            out = Words<BYTES>{};
+        }
+        char *to = destination<PAGED>(a, place, token, cls[r], head[r]);
+        if (to != nullptr) store_words<BYTES>(to + d0 * T::kBytes, out);
+    }
+}
+
+// Any head length and rotation: a wavefront for each row, one element a lane at a time; the partner is read again (from the cache
+// nearest to the unit).  Taken where no chunk of 8 bytes divides the head and the rotation's halves.
+template <class T, bool INTERLEAVED, bool PAGED>
+__global__ void __launch_bounds__(256) head_elements_kernel(const HeadRowsArgs a) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t row = a.waves_per_token.quotient(wave); // one wavefront a head here
+    const int64_t token = row;
+    if (token >= a.tokens) return;
+    int h = (int)(wave - row * a.waves_per_token.d);
+    const int cls = h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2);
+    h -= cls == 0 ? 0 : (cls == 1 ? a.heads[0] : a.heads[0] + a.heads[1]);
+    const char *src = a.in[cls] + token * a.in_token[cls] + h * a.in_head[cls];
+
+    Place place{0, -1, 0};
+    if (PAGED) place = place_of(a.batch, token, lane);
+    const bool placed = !PAGED || place.position >= 0;
+    const int64_t position = a.positions != nullptr ? explicit_position(a, token) : place.position;
+    const bool known = position >= 0 && position < a.table_rows;
+    const float *row_of = a.cos_sin + (known ? position : 0) * a.table_stride;
+    if (!placed && cls != 0) return;
+    char *to = destination<PAGED>(a, place, token, cls, h);
+    if (to == nullptr) return;
+
+    const char *gamma = cls == 2 ? nullptr : a.gamma[cls];
+    float scale = 1.0f;
+    if (gamma != nullptr) {
+        float sq = 0.0f;
+        for (int d = lane; d < a.dim; d += 64) {
+            const float x = load_element<T>(src + d * T::kBytes);
+            sq = __builtin_fmaf(x, x, sq);
+        }
+        scale = 1.0f / __builtin_sqrtf(sum_over_lanes(sq, 6) / (float)a.dim + a.eps);
+    }
+    const auto normed = [&](int d) {
+        const float x = load_element<T>(src + d * T::kBytes);
+        return gamma != nullptr ? x * scale * load_element<T>(gamma + d * T::kBytes) : x;
+    };
+    for (int d = lane; d < a.dim; d += 64) {
+        float y = normed(d);
+        if (cls != 2 && d < 2 * a.half) {
+            const bool first = INTERLEAVED ? (d & 1) == 0 : d < a.half;
+            const int j = INTERLEAVED ? d >> 1 : (first ? d : d - a.half);
+            const int other = INTERLEAVED ? d ^ 1 : (first ? d + a.half : d - a.half);
+            const float c = known ? row_of[j] : __builtin_nanf(""), s = known ? row_of[a.half + j] : __builtin_nanf("");
+            const float t = normed(other) * s;
+            y = __builtin_fmaf(y, c, first ? -t : t);
+        }
+        if (!placed) y = 0.0f;
+        store_element<T>(to + d * T::kBytes, y);
+    }
+}
+
+namespace {
+
+template <class T, int VE, int R>
+void launch_rows(const HeadRowsArgs &a, uint32_t blocks, hipStream_t s) {
+    if (a.paged) {
+        if (a.interleaved) head_rows_kernel<T, VE, R, true, true><<<blocks, 256, 0, s>>>(a);
+        else head_rows_kernel<T, VE, R, false, true><<<blocks, 256, 0, s>>>(a);
+    } else {
+        if (a.interleaved) head_rows_kernel<T, VE, R, true, false><<<blocks, 256, 0, s>>>(a);
+        else head_rows_kernel<T, VE, R, false, false><<<blocks, 256, 0, s>>>(a);
+    }
+}
+
+template <class T>
+void launch_elements(const HeadRowsArgs &a, uint32_t blocks, hipStream_t s) {
+    if (a.paged) {
+        if (a.interleaved) head_elements_kernel<T, true, true><<<blocks, 256, 0, s>>>(a);
+        else head_elements_kernel<T, false, true><<<blocks, 256, 0, s>>>(a);
+    } else {
+        if (a.interleaved) head_elements_kernel<T, true, false><<<blocks, 256, 0, s>>>(a);
+        else head_elements_kernel<T, false, false><<<blocks, 256, 0, s>>>(a);
+    }
+}
+
+template <class T>
+int launch_typed(HeadRowsArgs &a, const HeadRowsPlan &plan, hipStream_t s) {
+    constexpr int V = 16 / T::kBytes;
+    if (plan.chunk_bytes == 16) {
+        if (plan.rows == 4) launch_rows<T, V, 4>(a, plan.blocks, s);
+        else launch_rows<T, V, 1>(a, plan.blocks, s);
+    } else if (plan.chunk_bytes == 8) {
+        if (plan.rows == 4) launch_rows<T, V / 2, 4>(a, plan.blocks, s);
+        else launch_rows<T, V / 2, 1>(a, plan.blocks, s);
+    } else {
+        launch_elements<T>(a, plan.blocks, s);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? TDE_OK : hip_failed(e);
+}
+
+} // namespace
+
+// Which kernel, and its launch.  heads_all: rows a token has.
+int plan_head_rows(int elem, int dim, int half, bool interleaved, int64_t tokens, int64_t heads_all, HeadRowsPlan *p) {
+    p->chunk_bytes = 0;
+    for (int bytes = 16; bytes >= 8; bytes /= 2) {
+        const int ve = bytes / elem;
+        if (dim % ve == 0 && (interleaved ? 2 * half : half) % ve == 0 && dim / ve <= 64) {
+            p->chunk_bytes = bytes;
+            break;
+        }
+    }
+    int64_t waves = heads_all; // a token
+    p->lanes_log2 = 6;
+    p->rows = 1;
+    if (p->chunk_bytes != 0) {
+        const int lanes = dim * elem / p->chunk_bytes;
+        p->lanes_log2 = 0;
+        while ((1 << p->lanes_log2) < lanes) ++p->lanes_log2;
+        const int at_once = 64 >> p->lanes_log2;
+        const int64_t waves4 = (heads_all + 4 * at_once - 1) / (4 * at_once);
+        p->rows = tokens * waves4 >= 4096 ? 4 : 1;
+        waves = p->rows == 4 ? waves4 : (heads_all + at_once - 1) / at_once;
+    }
+    p->waves_per_token = (uint32_t)waves;
+    if (waves != 0 && tokens > (int64_t)0x7ffffff0 / waves) return TDE_ETOOBIG;
+    p->blocks = (uint32_t)((tokens * waves + 3) / 4);
+    return TDE_OK;
+}
+
+int launch_head_rows(HeadRowsArgs &a, int dtype, hipStream_t s) {
+    const int64_t heads_all = (int64_t)a.heads[0] + a.heads[1] + a.heads[2];
+    if (a.tokens == 0 || heads_all == 0) return TDE_OK;
+    HeadRowsPlan plan;
+    const int st = plan_head_rows(dtype == TDE_F32 ? 4 : 2, a.dim, a.half, a.interleaved, a.tokens, heads_all, &plan);
+    if (st != TDE_OK) return st;
+    a.lanes_log2 = plan.lanes_log2;
+    a.waves_per_token = Divisor32(plan.waves_per_token);
+    switch (dtype) {
+    case TDE_BF16: return launch_typed<Bf16>(a, plan, s);
+    case TDE_F16: return launch_typed<F16>(a, plan, s);
+    case TDE_F32: return launch_typed<F32>(a, plan, s);
+    }
+    return TDE_EDTYPE;
+}
+
+} // namespace block
+} // namespace tde

@@ -1,0 +1,669 @@
+// Attention of new tokens over a paged cache: o_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys j <= the token's position.
+//
+// One pass over the keys with a running maximum m and sum l for each row, in fp32.  A tile's rows are (new token, query head of one
+// key head's group), so every key and value is loaded once for the whole group.  Both products run on the matrix units, transposed:
+//
+//   S' = K Q'   16 keys x 16 rows an instruction, 32 channels deep
+//   O' = V' P'  16 channels x 16 rows, 32 keys deep
+//
+// An instruction's result has its 16 columns -- the rows -- along the lanes, so a row's maximum, sum and rescaling factor are one value
+// a lane, and a lane's scores of two key blocks are, converted to T, its operand of the second product without any exchange: the
+// product's keys only need the same order on both sides, and V' is read from LDS with transposing loads in just that order.
+// The weights p <= 1 are rounded to T for the second product (its operands are T); l sums them before the rounding.
+//
+// Where the rows of a call fill few workgroups the keys are split as well (see locate) and a second launch joins the parts.
+#include "tde_paged_attention.h"
+
+#include <algorithm>
+
+namespace tde {
+namespace block {
+
+#define TDE_LDS __attribute__((address_space(3)))
+
+namespace {
+
+template <class T>
+struct Mfma;
+template <>
+struct Mfma<Bf16> {
+    typedef bf16x8 operand;
+    static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t kExponent = 0x7f80u, kMantissa = 0x007fu;
+};
+template <>
+struct Mfma<F16> {
+    static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static constexpr uint32_t kExponent = 0x7c00u, kMantissa = 0x03ffu;
+};
+
+// Maximum over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48).
+__device__ __forceinline__ float max_of_row(float x) {
+    x = __builtin_fmaxf(x, __shfl_xor(x, 16));
+    return __builtin_fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_of_row(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// What a workgroup works on.  The items of a call: for every sequence its tiles of rows, for every tile its chunks of keys, in that
+// order; the rows behind the last sequence are one more "sequence" without keys.
+struct Item {
+    int32_t seq;      // seqs: rows behind the last sequence; -1: none
+    int32_t tile;     // of the sequence
+    int32_t chunk, chunks;
+    int32_t first;    // the sequence's first item
+    int32_t begin, count; // its rows of the call
+    int32_t len;      // its keys
+    int32_t keys;     // of a chunk
+};
+
+__device__ __forceinline__ int64_t clamped(int64_t x, int64_t low, int64_t high) { return x < low ? low : (x > high ? high : x); }
+
+// The rows and keys of sequence i, whatever the arrays hold: rows inside the call's, lengths not negative.
+__device__ __forceinline__ void extent(const AttentionArgs &a, int i, int32_t &begin, int32_t &count, int32_t &len) {
+    begin = count = len = 0;
+    if (i > a.batch.seqs) return;
+    const int64_t s = clamped(a.batch.starts[i], 0, a.tokens);
+    const int64_t e = i == a.batch.seqs ? a.tokens : clamped(a.batch.starts[i + 1], 0, a.tokens);
+    begin = (int32_t)s;
+    count = (int32_t)(e > s ? e - s : 0);
+    if (i < a.batch.seqs) len = a.batch.lens[i] > 0 ? a.batch.lens[i] : 0;
+}
+
+template <int ROWS>
+__device__ __forceinline__ int32_t tiles_of(const AttentionArgs &a, int32_t count) {
+    return (int32_t)(((int64_t)count * a.group.d + ROWS - 1) / ROWS);
+}
+
+// Keys that are walked through: a length beyond the page table's row needs one key of it to make the rows that see it NaN.
+__device__ __forceinline__ int32_t walked(const AttentionArgs &a, int32_t len) { return len > a.capacity ? a.capacity + 1 : len; }
+
+// Keys of a chunk: all keys that the tiles have between them, over the number of items aimed at, in whole blocks of 64; sequences
+// of any lengths then give chunks of one size, and the number of items is at most target + tiles.
+template <int ROWS>
+__device__ __forceinline__ int32_t keys_of_chunk(const AttentionArgs &a, int lane) {
+    int64_t total = 0;
+    for (int i = lane; i < a.batch.seqs; i += 64) {
+        int32_t begin, count, len;
+        extent(a, i, begin, count, len);
+        total += (int64_t)tiles_of<ROWS>(a, count) * walked(a, len);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) total += __shfl_xor((long long)total, m);
+    int64_t keys = (total + a.target - 1) / a.target;
+    keys = (keys + 63) & ~(int64_t)63;
+    return (int32_t)clamped(keys, a.min_chunk, 0x7fffffc0);
+}
+
+// The item with number `want` (BY_ITEM), or the first item of sequence `want`; one wavefront, 64 sequences at a time.
+template <int ROWS, bool SPLIT, bool BY_ITEM>
+__device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int lane) {
+    Item it{-1, 0, 0, 1, 0, 0, 0, 0, 0x7fffffc0};
+    if (SPLIT) it.keys = keys_of_chunk<ROWS>(a, lane);
+    int32_t passed = 0;
+    for (int base = 0; base <= a.batch.seqs; base += 64) {
+        int32_t begin, count, len;
+        extent(a, base + lane, begin, count, len);
+        const int32_t tiles = tiles_of<ROWS>(a, count);
+        const int32_t chunks = SPLIT && walked(a, len) > it.keys ? (walked(a, len) - 1) / it.keys + 1 : 1;
+        const int32_t items = tiles * chunks;
+        int32_t upto = items; // inclusive sum over the lanes
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int32_t below = __shfl_up(upto, m);
+            if (lane >= m) upto += below;
+        }
+        const int32_t all = __builtin_amdgcn_readlane(upto, 63);
+        int at;
+        if (BY_ITEM) at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(passed + upto <= want));
+        else at = want - base;
+        if (BY_ITEM ? at < 64 : at < 64) {
+            it.seq = base + at;
+            it.begin = __builtin_amdgcn_readlane(begin, at);
+            it.count = __builtin_amdgcn_readlane(count, at);
+            it.len = __builtin_amdgcn_readlane(len, at);
+            it.chunks = __builtin_amdgcn_readlane(chunks, at);
+            it.first = passed + __builtin_amdgcn_readlane(upto - items, at);
+            const int32_t local = BY_ITEM ? want - it.first : 0;
+            const int32_t all_tiles = __builtin_amdgcn_readlane(tiles, at);
+            it.tile = local / it.chunks;
+            it.chunk = local - it.tile * it.chunks;
+            // unsplit, a sequence's last tiles, which see most keys, go first
+            if (!SPLIT) it.tile = all_tiles - 1 - it.tile;
+            return it;
+        }
+        passed += all;
+    }
+    return it;
+}
+
+} // namespace
+
+// NB blocks of 16 rows a wavefront.  SHARED: the wavefronts have rows of their own and share the keys of a tile (double-buffered
+// in LDS); otherwise all have the same rows and take the tiles of keys in turn, each through LDS of its own, and are joined at the end.
+template <class T, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
+__global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionArgs a) {
+    constexpr int KT = SHARED && D <= 128 ? 64 : 32; // keys a tile
+    constexpr int CH = D / 8;                        // chunks of 16 bytes a row
+    constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
+    constexpr int LOADERS = 64 * (SHARED ? WAVES : 1);
+    constexpr int LOADS = KT * CH / LOADERS; // a thread, of keys and of values
+    constexpr int TILE = KT * D * 2;
+    constexpr int BUFFERS = SHARED ? 2 : WAVES;
+    constexpr int JOIN = SHARED ? 0 : WAVES * 16 * NB * (D + 4) * 4;
+    constexpr int LDS = 2 * TILE * BUFFERS > JOIN ? 2 * TILE * BUFFERS : JOIN;
+    __shared__ __align__(16) char lds[LDS];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t item_index = a.kv_heads.quotient(blockIdx.x);
+    const int kv_head = (int)(blockIdx.x - item_index * a.kv_heads.d);
+    const Item it = locate<ROWS, SPLIT, true>(a, (int32_t)item_index, lane);
+    if (it.seq < 0) return;
+    const int group = (int)a.group.d;
+    const int col = lane & 15, quad = lane >> 4;
+
+    // this lane's row in each of its blocks: the token, the head, the last key that it sees
+    int32_t token[NB], last[NB];
+    int head[NB];
+    const int64_t rows_all = (int64_t)it.count * group;
+    const int row0 = SHARED ? wave * 16 * NB : 0;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int64_t r = (int64_t)it.tile * ROWS + row0 + n * 16 + col;
+        const bool there = r < rows_all;
+        const uint32_t t = a.group.quotient((uint32_t)(there ? r : 0));
+        head[n] = kv_head * group + (int)((uint32_t)(there ? r : 0) - t * a.group.d);
+        token[n] = there ? it.begin + (int32_t)t : -1;
+        last[n] = there ? it.len - it.count + (int32_t)t : -1;
+    }
+    if (it.seq == a.batch.seqs) { // rows behind the last sequence
+        if (!a.zero_tail || (!SHARED && wave != 0)) return;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+            if (token[n] >= 0)
+                for (int d = quad * 8; d < a.dim; d += 32)
+                    store_words<16>(a.out + token[n] * a.out_token + head[n] * a.out_head + d * 2, Words<16>{});
+        return;
+    }
+
+    // keys that the tile's rows see, of this item's chunk
+    const int64_t top_row = std::min<int64_t>((int64_t)(it.tile + 1) * ROWS, rows_all) - 1;
+    const int32_t top = it.len - it.count + (int32_t)a.group.quotient((uint32_t)top_row) + 1; // keys that the tile's last row sees
+    const int32_t lowest = it.len - it.count + (int32_t)a.group.quotient((uint32_t)((int64_t)it.tile * ROWS)) + 1;
+    const int64_t from64 = SPLIT ? (int64_t)it.chunk * it.keys : 0;
+    const int32_t from = (int32_t)std::min<int64_t>(from64, 0x7fffffc0);
+    const int32_t until = (int32_t)std::min<int64_t>(SPLIT ? from64 + it.keys : 0x7fffffc0, std::min(top, walked(a, it.len)));
+
+    u32x4 q[NB][D / 32];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            const int d = s * 32 + quad * 8;
+            q[n][s] = u32x4{0, 0, 0, 0};
+            if (token[n] >= 0 && d < a.dim) {
+                const Words<16> w = load_words<16>(a.q + token[n] * a.q_token + head[n] * a.q_head + d * 2);
+                q[n][s] = u32x4{w.w[0], w.w[1], w.w[2], w.w[3]};
+            }
+        }
+
+    f32x4 o[NB][D / 16];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        m[n] = -__builtin_inff();
+        l[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[n][d] = f32x4{0, 0, 0, 0};
+    }
+
+    // ---- loading ----
+    const int32_t *const table = a.batch.table + it.seq * a.batch.table_stride;
+    const int loader = SHARED ? (int)threadIdx.x : lane;
+    const int load_row = loader / CH, load_chunk = loader % CH; // rows load_row + i * LOADERS / CH
+    constexpr int ROW_STEP = LOADERS / CH;
+    const bool chunk_there = load_chunk * 8 < a.dim;
+    const char *const k_base = a.k + kv_head * a.k_head + load_chunk * 16, *const v_base = a.v + kv_head * a.v_head + load_chunk * 16;
+    constexpr int TILE_STEP = SHARED ? KT : KT * WAVES;
+    const int32_t first_key = from + (SHARED ? 0 : wave * KT);
+
+    u32x4 kreg[LOADS], vreg[LOADS];
+    // Where key `tile key + lane` lies in the caches, from their heads' first channels on: not there (kNoKey) from `until` on,
+    // lost (kNoPage) where the table or the cache has no page for it.
+    constexpr int64_t kNoKey = -1, kNoPage = -2;
+    struct Offsets {
+        int64_t k, v;
+    };
+    const auto offsets_of = [&](int32_t key0) -> Offsets {
+        const int64_t key = (int64_t)key0 + lane;
+        if ((KT < 64 && lane >= KT) || key >= until) return {kNoKey, kNoKey};
+        const uint32_t at = a.batch.page.quotient((uint32_t)key), slot = (uint32_t)key - at * a.batch.page.d;
+        const int32_t page = page_number(a.batch, table, at);
+        if (page < 0) return {kNoPage, kNoPage};
+        return {(int64_t)((uint64_t)(uint32_t)page * a.k_page + (uint64_t)slot * a.k_slot),
+                (int64_t)((uint64_t)(uint32_t)page * a.v_page + (uint64_t)slot * a.v_slot)};
+    };
+    const auto of_lane = [](int64_t x, int from) { return (int64_t)__shfl((long long)x, from); };
+    const auto load_tile = [&](const Offsets &where) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = load_row + i * ROW_STEP;
+            const int64_t k_at = of_lane(where.k, row), v_at = of_lane(where.v, row);
+            kreg[i] = vreg[i] = u32x4{0, 0, 0, 0};
+            if (k_at >= 0 && chunk_there) {
+                kreg[i] = *(const __attribute__((address_space(1))) u32x4 *)(k_base + k_at);
+                vreg[i] = *(const __attribute__((address_space(1))) u32x4 *)(v_base + v_at);
+            }
+        }
+    };
+    // Chunks are stored at places that spread over the banks what is read together: 16 keys of one chunk (keys), 8 keys of two
+    // neighbouring chunks (values).
+    const auto k_place = [](int row, int chunk) { return (row * CH + (chunk ^ (D == 64 ? (row >> 1) & 7 : row & 15))) * 16; };
+    const auto v_place = [](int row, int chunk) { return (row * CH + (chunk ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1))) * 16; };
+    const auto store_tile = [&](char *buf) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = load_row + i * ROW_STEP;
+            *(u32x4 *)(buf + k_place(row, load_chunk)) = kreg[i];
+            *(u32x4 *)(buf + TILE + v_place(row, load_chunk)) = vreg[i];
+        }
+    };
+    // whether this thread's values of the tile hold an infinity or a NaN
+    const auto not_finite = [&]() {
+        // an exponent of ones plus one at its lowest bit carries out of its field; the field's neighbours are masked off before
+        constexpr uint32_t E = Mfma<T>::kExponent, LOW = E & (~E + 1u); // the field and its lowest bit
+        uint32_t carried = 0;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) carried |= (vreg[i][w] & (E | E << 16)) + (LOW | LOW << 16);
+        return (carried & 0x80008000u) != 0;
+    };
+
+    int32_t key0 = first_key;
+    Offsets where{kNoKey, kNoKey}, where_next{kNoKey, kNoKey};
+    char *buf = lds + (SHARED ? 0 : wave * 2 * TILE);
+    bool poisoned = false; // values of the tile in LDS that not all rows see are not all finite
+    const auto publish = [&](int32_t key) { // kreg, vreg -> buf, visible to the readers afterwards
+        store_tile(buf);
+        const bool partly_seen = key + KT > lowest;
+        if constexpr (SHARED) {
+            if (partly_seen) poisoned = __syncthreads_or(not_finite());
+            else {
+                poisoned = false;
+                __syncthreads();
+            }
+        } else {
+            poisoned = partly_seen && __builtin_amdgcn_ballot_w64(not_finite()) != 0;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+    if (key0 < until) {
+        where = offsets_of(key0);
+        load_tile(where);
+        if ((int64_t)key0 + TILE_STEP < until) where_next = offsets_of(key0 + TILE_STEP);
+        publish(key0);
+    }
+    while (key0 < until) {
+        const int64_t next = (int64_t)key0 + TILE_STEP;
+        const uint64_t lost = __builtin_amdgcn_ballot_w64(where.k == kNoPage);
+        if (next < until) {
+            where = where_next;
+            load_tile(where);
+            if (next + TILE_STEP < until) where_next = offsets_of((int32_t)(next + TILE_STEP));
+        }
+
+        // ---- scores ----
+        f32x4 s[NB][KT / 16];
+#pragma unroll
+        for (int kb = 0; kb < KT / 16; ++kb) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) s[n][kb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int st = 0; st < D / 32; ++st) {
+                const u32x4 kf = *(const u32x4 *)(buf + k_place(kb * 16 + col, st * 4 + quad));
+#pragma unroll
+                for (int n = 0; n < NB; ++n) s[n][kb] = Mfma<T>::mul(kf, q[n][st], s[n][kb]);
+            }
+        }
+        if (lost != 0) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int kb = 0; kb < KT / 16; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if ((lost >> (kb * 16 + quad * 4 + r)) & 1) s[n][kb][r] = __builtin_nanf("");
+        }
+        const bool edge = key0 + KT > lowest || key0 + KT > until;
+        if (edge) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int32_t see = std::min(last[n], until - 1) - key0;
+#pragma unroll
+                for (int kb = 0; kb < KT / 16; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (kb * 16 + quad * 4 + r > see) s[n][kb][r] = -__builtin_inff();
+            }
+        }
+
+        // ---- softmax ----
+        u32x4 p[NB][KT / 32];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            float top_score = s[n][0][0];
+#pragma unroll
+            for (int kb = 0; kb < KT / 16; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top_score = __builtin_fmaxf(top_score, s[n][kb][r]);
+            const float m_new = __builtin_fmaxf(m[n], max_of_row(top_score));
+            const float shift = m_new == -__builtin_inff() ? 0.0f : m_new * a.scale_log2; // nothing seen yet: every weight is 0
+            const float alpha = __builtin_amdgcn_exp2f(m[n] * a.scale_log2 - shift);
+            m[n] = m_new;
+            float sum = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KT / 16; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[n][kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][r], a.scale_log2, -shift));
+                    sum += s[n][kb][r];
+                }
+            l[n] = l[n] * alpha + sum;
+#pragma unroll
+            for (int ks = 0; ks < KT / 32; ++ks)
+                p[n][ks] = u32x4{T::narrow(s[n][2 * ks][0], s[n][2 * ks][1]), T::narrow(s[n][2 * ks][2], s[n][2 * ks][3]),
+                                 T::narrow(s[n][2 * ks + 1][0], s[n][2 * ks + 1][1]), T::narrow(s[n][2 * ks + 1][2], s[n][2 * ks + 1][3])};
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) o[n][d] *= alpha;
+        }
+
+        // ---- values ----
+        const auto value_operand = [&](int ks, int d) {
+            // 4 keys x 16 channels for each 16 lanes, transposed on the way: a lane gets one channel of the keys 4 * quad ... + 3
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            const int row = ks * 32 + quad * 4 + (col >> 2), chunk = d * 2 + ((col & 3) >> 1), within = (col & 1) * 8;
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(buf + TILE + v_place(row, chunk) + within));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(buf + TILE + v_place(row + 16, chunk) + within));
+            const u32x2 xu = __builtin_bit_cast(u32x2, x), yu = __builtin_bit_cast(u32x2, y);
+            return u32x4{xu[0], xu[1], yu[0], yu[1]};
+        };
+        if (__builtin_expect(!poisoned, 1)) {
+#pragma unroll
+            for (int ks = 0; ks < KT / 32; ++ks)
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const u32x4 vf = value_operand(ks, d);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) o[n][d] = Mfma<T>::mul(vf, p[n][ks], o[n][d]);
+                }
+        } else {
+            // A weight of zero does not keep an infinity or NaN from the product.  Here such values are taken out of it, and which
+            // of them a row sees is counted by a product of its own: 1 for +inf, 128 for -inf, 16384 for NaN, 64 keys at most.
+            constexpr uint32_t E = Mfma<T>::kExponent, M = Mfma<T>::kMantissa;
+#pragma unroll 1
+            for (int ks = 0; ks < KT / 32; ++ks) {
+                u32x4 seen[NB], weights[NB]; // 1.0 where the row sees the key
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const int32_t see = std::min(last[n], until - 1) - key0 - ks * 32;
+                    const uint32_t one = T::narrow1(1.0f);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int key = (w >> 1) * 16 + quad * 4 + (w & 1) * 2;
+                        seen[n][w] = (one & ~(uint32_t)((see - key) >> 31)) | ((one & ~(uint32_t)((see - key - 1) >> 31)) << 16);
+                    }
+                    weights[n] = ks == 0 ? p[n][0] : p[n][KT / 32 - 1];
+                }
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    __builtin_amdgcn_sched_barrier(0); // one after the other: interleaved they run out of scalar registers
+                    u32x4 vf = value_operand(ks, d), mark;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t finite = 0, marks = 0;
+#pragma unroll
+                        for (int hi = 0; hi < 32; hi += 16) {
+                            const uint32_t h = (vf[w] >> hi) & 0xffffu;
+                            const float code = (h & M) != 0 ? 16384.0f : ((h & 0x8000u) != 0 ? 128.0f : 1.0f);
+                            const uint32_t is = (h & E) == E ? 0xffffu : 0u;
+                            finite |= (h & ~is) << hi;
+                            marks |= (T::narrow1(code) & is) << hi;
+                        }
+                        vf[w] = finite;
+                        mark[w] = marks;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        o[n][d] = Mfma<T>::mul(vf, weights[n], o[n][d]);
+                        const f32x4 found = Mfma<T>::mul(mark, seen[n], f32x4{0, 0, 0, 0});
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t f = (uint32_t)found[r];
+                            // 0, or the infinity or NaN that the found values add up to
+                            float add = (f & 127u) != 0 ? __builtin_inff() : 0.0f;
+                            add -= (f & (16384u - 128u)) != 0 ? __builtin_inff() : 0.0f;
+                            o[n][d][r] += f >= 16384u ? __builtin_nanf("") : add;
+                        }
+                    }
+                }
+            }
+        }
+
+        if (next < until) {
+            if constexpr (SHARED) buf = buf == lds ? lds + 2 * TILE : lds;
+            publish((int32_t)next);
+        }
+        key0 = (int32_t)std::min<int64_t>(next, 0x7fffffff);
+    }
+
+    // ---- what is left: a row's sum over its four lanes, then the row ----
+#pragma unroll
+    for (int n = 0; n < NB; ++n) l[n] = sum_of_row(l[n]);
+
+    const int64_t slot = ((int64_t)item_index * a.kv_heads.d + kv_head) * ROWS; // of the partial results
+    if constexpr (SHARED) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            if (token[n] < 0) continue;
+            if constexpr (SPLIT) {
+                float *const part = a.partial + (slot + row0 + n * 16 + col) * (D + 4);
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) *(f32x4 *)(part + d * 16 + quad * 4) = o[n][d];
+                if (quad == 0) *(f32x2 *)(part + D) = f32x2{m[n], l[n]};
+            } else {
+                const float inverse = 1.0f / l[n];
+                char *const to = a.out + token[n] * a.out_token + head[n] * a.out_head;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    const int at = d * 16 + quad * 4;
+                    if (at >= a.dim) continue;
+                    f32x4 y = o[n][d] * inverse;
+                    if (last[n] < 0) y = f32x4{0, 0, 0, 0}; // sees no key
+                    store_words<8>(to + at * 2, Words<8>{{T::narrow(y[0], y[1]), T::narrow(y[2], y[3])}});
+                }
+            }
+        }
+    } else {
+        // join the wavefronts: [wave][row][D + 4]
+        float *const mine = (float *)lds + wave * 16 * NB * (D + 4);
+        __syncthreads(); // every wavefront is done with its tiles
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            float *const part = mine + (n * 16 + col) * (D + 4);
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) *(f32x4 *)(part + d * 16 + quad * 4) = o[n][d];
+            if (quad == 0) *(f32x2 *)(part + D) = f32x2{m[n], l[n]};
+        }
+        __syncthreads();
+        // thread -> row and four channels
+        for (int at = threadIdx.x; at < 16 * NB * (D / 4); at += 64 * WAVES) {
+            const int row = at / (D / 4), d = at % (D / 4) * 4;
+            const int64_t r = (int64_t)it.tile * ROWS + row;
+            if (r >= rows_all) continue;
+            float top_m = -__builtin_inff();
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) top_m = __builtin_fmaxf(top_m, ((float *)lds)[(w * 16 * NB + row) * (D + 4) + D]);
+            const float shift = top_m == -__builtin_inff() ? 0.0f : top_m * a.scale_log2;
+            f32x4 sum = {0, 0, 0, 0};
+            float all = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float *const part = (const float *)lds + (w * 16 * NB + row) * (D + 4);
+                const float weight = __builtin_amdgcn_exp2f(part[D] * a.scale_log2 - shift);
+                sum += *(const f32x4 *)(part + d) * weight;
+                all += part[D + 1] * weight;
+            }
+            if constexpr (SPLIT) {
+                float *const part = a.partial + (slot + row) * (D + 4);
+                *(f32x4 *)(part + d) = sum;
+                if (d == 0) *(f32x2 *)(part + D) = f32x2{top_m, all};
+            } else {
+                if (d >= a.dim) continue;
+                const uint32_t t = a.group.quotient((uint32_t)r);
+                const int h = kv_head * group + (int)((uint32_t)r - t * a.group.d);
+                f32x4 y = sum * (1.0f / all);
+                if (it.len - it.count + (int32_t)t < 0) y = f32x4{0, 0, 0, 0};
+                store_words<8>(a.out + (it.begin + (int32_t)t) * a.out_token + h * a.out_head + d * 2,
+                               Words<8>{{T::narrow(y[0], y[1]), T::narrow(y[2], y[3])}});
+            }
+        }
+    }
+}
+
+// Joins the chunks of a row: a workgroup a row (token, query head), its wavefronts take chunks in turn.
+template <class T, int D, int ROWS>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttentionArgs a) {
+    constexpr int E = D / 64; // channels a lane
+    __shared__ float joined[4][D + 4];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t heads = a.kv_heads.d * a.group.d;
+    const int32_t token = (int32_t)(blockIdx.x / heads);
+    const int head = (int)(blockIdx.x - (uint32_t)token * heads);
+    const int seq = __builtin_amdgcn_readfirstlane(sequence_of(a.batch, token, lane));
+    if (seq >= a.batch.seqs) return; // rows behind the last sequence are the first launch's
+    const Item it = locate<ROWS, true, false>(a, seq, lane);
+    if (token < it.begin || token >= it.begin + it.count) return;
+    const uint32_t kv_head = a.group.quotient((uint32_t)head);
+    const int64_t r = (int64_t)(token - it.begin) * a.group.d + (head - kv_head * a.group.d);
+    const int64_t tile = r / ROWS;
+    const int row = (int)(r - tile * ROWS);
+    float top_m = -__builtin_inff(), sum[E] = {}, all = 0.0f;
+    const float *const parts =
+        a.partial + ((((int64_t)it.first + tile * it.chunks) * a.kv_heads.d + kv_head) * ROWS + row) * (int64_t)(D + 4);
+    const int64_t step = (int64_t)a.kv_heads.d * ROWS * (D + 4);
+    if ((int64_t)it.first + (tile + 1) * it.chunks > a.items) return; // only where starts do not ascend
+    for (int c = wave; c < it.chunks; c += 4) {
+        const float *const part = parts + c * step;
+        const float pm = part[D], pl = part[D + 1];
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = part[lane * E + e];
+        const float m_new = __builtin_fmaxf(top_m, pm);
+        const float shift = m_new == -__builtin_inff() ? 0.0f : m_new * a.scale_log2;
+        const float old = __builtin_amdgcn_exp2f(top_m * a.scale_log2 - shift), weight = __builtin_amdgcn_exp2f(pm * a.scale_log2 - shift);
+        all = all * old + pl * weight;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] = sum[e] * old + x[e] * weight;
+        top_m = m_new;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) joined[wave][lane * E + e] = sum[e];
+    if (lane == 0) {
+        joined[wave][D] = top_m;
+        joined[wave][D + 1] = all;
+    }
+    __syncthreads();
+    if (threadIdx.x * 2 >= (uint32_t)a.dim) return;
+    float best = joined[0][D];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) best = __builtin_fmaxf(best, joined[w][D]);
+    const float shift = best == -__builtin_inff() ? 0.0f : best * a.scale_log2;
+    float y0 = 0.0f, y1 = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float weight = __builtin_amdgcn_exp2f(joined[w][D] * a.scale_log2 - shift);
+        total += joined[w][D + 1] * weight;
+        y0 += joined[w][2 * threadIdx.x] * weight;
+        y1 += joined[w][2 * threadIdx.x + 1] * weight;
+    }
+    const bool sees = it.len - it.count + (token - it.begin) >= 0;
+    const uint32_t pair = sees ? T::narrow(y0 / total, y1 / total) : 0u;
+    store_words<4>(a.out + token * a.out_token + head * a.out_head + threadIdx.x * 4, Words<4>{{pair}});
+}
+
+namespace {
+
+template <class T, int D, int NB, int WAVES, bool SHARED>
+void launch_one(const AttentionArgs &a, bool split, uint32_t blocks, hipStream_t s) {
+    if (!split) {
+        attention_kernel<T, D, NB, WAVES, SHARED, false><<<blocks, 64 * WAVES, 0, s>>>(a);
+        return;
+    }
+    attention_kernel<T, D, NB, WAVES, SHARED, true><<<blocks, 64 * WAVES, 0, s>>>(a);
+    const uint32_t rows = (uint32_t)(a.tokens * a.kv_heads.d * a.group.d);
+    attention_join_kernel<T, D, 16 * NB *(SHARED ? WAVES : 1)><<<rows, 256, 0, s>>>(a);
+}
+
+template <class T, int D>
+void launch_dim(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks, hipStream_t s) {
+    if constexpr (D == 256) launch_one<T, D, 1, 4, true>(a, p.split, blocks, s);
+    else if (p.rows == 16) launch_one<T, D, 1, 4, false>(a, p.split, blocks, s);
+    else launch_one<T, D, 2, 4, true>(a, p.split, blocks, s);
+}
+
+template <class T>
+void launch_type(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks, hipStream_t s) {
+    if (p.wide_dim == 64) launch_dim<T, 64>(a, p, blocks, s);
+    else if (p.wide_dim == 128) launch_dim<T, 128>(a, p, blocks, s);
+    else launch_dim<T, 256>(a, p, blocks, s);
+}
+
+} // namespace
+
+// Which kernel, and whether the keys are split.  capacity: keys that the page table can name for a sequence.
+int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
+    *p = AttentionPlan{};
+    p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
+    const int64_t group = q_heads / kv_heads, rows_all = tokens * group;
+    if (rows_all > 0x7fffff00) return TDE_ETOOBIG;
+    p->rows = p->wide_dim == 256 ? 64 : (seqs > 0 && rows_all > (int64_t)seqs * 16 ? 128 : 16);
+    const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence and one behind the last
+    const int64_t cus = device_compute_units();
+    p->min_chunk = 256;
+    const int64_t full = rows_all / p->rows > 0 ? rows_all / p->rows : 1; // rather how many there are
+    const int64_t filled = std::max<int64_t>(full, std::min<int64_t>(seqs, tokens)) * kv_heads;
+    p->split = filled < 4 * cus && capacity > p->min_chunk;
+    p->target = std::max<int64_t>(1, 4 * cus / kv_heads);
+    p->items = tiles + (p->split ? p->target : 0);
+    if (p->items > 0x7fffff00 / kv_heads) return TDE_ETOOBIG;
+    if (p->split) {
+        if (rows_all * kv_heads > 0x7fffff00) return TDE_ETOOBIG;
+        p->workspace_bytes = p->items * kv_heads * p->rows * (int64_t)(p->wide_dim + 4) * 4;
+    }
+    return TDE_OK;
+}
+
+int launch_attention(AttentionArgs &a, const AttentionPlan &p, int dtype, hipStream_t s) {
+    a.items = (int32_t)p.items;
+    a.target = p.target;
+    a.min_chunk = p.min_chunk;
+    a.capacity = (int32_t)std::min<int64_t>((int64_t)a.batch.table_pages * a.batch.page.d, 0x7fffff00);
+    const uint32_t blocks = (uint32_t)(p.items * a.kv_heads.d);
+    if (dtype == TDE_BF16) launch_type<Bf16>(a, p, blocks, s);
+    else launch_type<F16>(a, p, blocks, s);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? TDE_OK : hip_failed(e);
+}
+
+} // namespace block
+} // namespace tde
