@@ -43,27 +43,27 @@ __device__ __forceinline__ u32x4 load16(const int8_t *base, int64_t row, int64_t
     return v;
 }
 
-// A wavefront's sums, scaled: WT tokens from t0 on, WN channels from n0 on.  INSIDE: all of them exist.
-template <class T, int WT, int WN, bool INSIDE>
+// A wavefront's sums, scaled: WT tokens from t0 on, WN channels from n0 on, as many as there are.
+template <class T, int WT, int WN>
 __device__ __forceinline__ void store_sums(const LinearArgs &a, const i32x16 (&acc)[WN / 32][WT / 32], int64_t t0, int64_t n0, int lane) {
     const bool biased = a.bias != nullptr;
     float s[WT / 32];
 #pragma unroll
     for (int j = 0; j < WT / 32; ++j) {
         const int64_t t = t0 + j * 32 + (lane & 31);
-        s[j] = INSIDE || t < a.tokens ? a.scales[t] : 0.0f;
+        s[j] = t < a.tokens ? a.scales[t] : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < WN / 32; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int64_t n = n0 + i * 32 + g * 8 + (lane >> 5) * 4;
-            const int count = INSIDE ? 4 : (int)(a.n - n < 4 ? a.n - n : 4);
+            const int count = (int)(a.n - n < 4 ? a.n - n : 4);
             float u[4], b[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                u[r] = INSIDE || r < count ? a.weight_scales[n + r] : 0.0f;
-                b[r] = biased && (INSIDE || r < count) ? a.bias[n + r] : 0.0f;
+                u[r] = r < count ? a.weight_scales[n + r] : 0.0f;
+                b[r] = biased && r < count ? a.bias[n + r] : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < WT / 32; ++j) {
@@ -74,14 +74,55 @@ __device__ __forceinline__ void store_sums(const LinearArgs &a, const i32x16 (&a
                     y[r] = (float)acc[i][j][g * 4 + r] * (s[j] * u[r]);
                     if (biased) y[r] += b[r];
                 }
-                if (INSIDE || (t < a.tokens && count > 0)) store4<T>(a.out + (t * a.n + n) * T::kBytes, y, count, count >= 4);
+                if (t < a.tokens && count > 0) store4<T>(a.out + (t * a.n + n) * T::kBytes, y, count, count >= 4);
             }
         }
 }
+// The same for a tile whose tokens and channels all exist, by way of LDS (`room`, kStoreRoom bytes of the wavefront's own): a lane
+// has 4 channels of 32 different tokens' rows, and leaves with 16 bytes next to its neighbours'.  (Stored as they are, 8 bytes a row,
+// the results of 4096 x 4096 x 4096 take 30 us of 85.)
+template <class T, int WN>
+constexpr int kStoreRoom = 32 * (WN * T::kBytes + 16);
 template <class T, int WT, int WN>
-__device__ __forceinline__ void store_tile(const LinearArgs &a, const i32x16 (&acc)[WN / 32][WT / 32], int64_t t0, int64_t n0, int lane) {
-    if (t0 + WT <= a.tokens && n0 + WN <= a.n) store_sums<T, WT, WN, true>(a, acc, t0, n0, lane);
-    else store_sums<T, WT, WN, false>(a, acc, t0, n0, lane);
+__device__ __forceinline__ void store_rows(const LinearArgs &a, const i32x16 (&acc)[WN / 32][WT / 32], int64_t t0, int64_t n0, int lane, char *room) {
+    const bool biased = a.bias != nullptr;
+    constexpr int PITCH = WN * T::kBytes + 16, LANES = WN * T::kBytes / 16, ROWS = 64 / LANES; // lanes of a row, rows of a store
+    const int row = lane & 31, from = (lane >> 5) * 4;
+#pragma unroll
+    for (int j = 0; j < WT / 32; ++j) {
+        const float s = a.scales[t0 + j * 32 + row];
+#pragma unroll
+        for (int i = 0; i < WN / 32; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int n = i * 32 + g * 8 + from;
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    y[r] = (float)acc[i][j][g * 4 + r] * (s * a.weight_scales[n0 + n + r]);
+                    if (biased) y[r] += a.bias[n0 + n + r];
+                }
+                const Words<4 * T::kBytes> w = narrow_all<T, 4>(y);
+                char *const to = room + row * PITCH + n * T::kBytes;
+                if constexpr (T::kBytes == 4) *(u32x4 *)to = u32x4{w.w[0], w.w[1], w.w[2], w.w[3]};
+                else *(u32x2 *)to = u32x2{w.w[0], w.w[1]};
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int x = 0; x < 32 / ROWS; ++x) {
+            const int at = x * ROWS + lane / LANES;
+            const u32x4 v = *(const u32x4 *)(room + at * PITCH + lane % LANES * 16);
+            store_words<16>(a.out + ((t0 + j * 32 + at) * a.n + n0) * T::kBytes + lane % LANES * 16, Words<16>{{v[0], v[1], v[2], v[3]}});
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+template <class T, int WT, int WN>
+__device__ __forceinline__ void store_tile(const LinearArgs &a, const i32x16 (&acc)[WN / 32][WT / 32], int64_t t0, int64_t n0, int lane, char *room) {
+    if (t0 + WT <= a.tokens && n0 + WN <= a.n) store_rows<T, WT, WN>(a, acc, t0, n0, lane, room);
+    else store_sums<T, WT, WN>(a, acc, t0, n0, lane);
 }
 
 // BT tokens x BN channels a workgroup, WT x WN of them a wavefront; 128 bytes of both operands' rows at a time, double-buffered.
@@ -146,7 +187,8 @@ __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_tile_kernel
         at ^= 1;
     }
 
-    store_tile<T, WT, WN>(a, acc, t0 + wave_t * WT, n0 + wave_n * WN, lane);
+    static_assert(kStoreRoom<T, WN> * THREADS / 64 <= (int)sizeof(lds));
+    store_tile<T, WT, WN>(a, acc, t0 + wave_t * WT, n0 + wave_n * WN, lane, lds[0] + wave * kStoreRoom<T, WN>);
 }
 
 // ---- tiles through LDS without registers ----
@@ -180,14 +222,15 @@ struct TileOrder {
     }
 };
 
-// As linear_tile_kernel, for rows of whole 4 bytes: STAGES tiles in LDS, loaded STAGES - 1 ahead.  A stage is complete when every
-// wavefront has waited for its own loads and passed the barrier, which also says that the stage before has been read.
+// As linear_tile_kernel, for rows of whole 4 bytes: STAGES blocks of 128 bytes of the rows in LDS, loaded STAGES - 1 ahead.  A stage
+// is complete when every wavefront has waited for its own loads and passed the barrier, which also says that the stage before has
+// been read.
 template <class T, int BT, int BN, int WT, int WN, int STAGES>
 __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_staged_kernel(const LinearArgs a, const TileOrder order) {
     constexpr int WAVES = (BT / WT) * (BN / WN);
     constexpr int KB = 128, CH = KB / 16;
-    constexpr int C_LOADS = BT * CH / 64 / WAVES, W_LOADS = BN * CH / 64 / WAVES, LOADS = C_LOADS + W_LOADS;
-    static_assert(C_LOADS * 64 * WAVES == BT * CH && W_LOADS * 64 * WAVES == BN * CH, "a wavefront loads whole groups of 8 rows");
+    constexpr int C_LOADS = BT / 8 / WAVES, W_LOADS = BN / 8 / WAVES, LOADS = C_LOADS + W_LOADS;
+    static_assert(C_LOADS * 8 * WAVES == BT && W_LOADS * 8 * WAVES == BN, "a wavefront loads whole groups of 8 rows");
     static_assert((STAGES - 2) * LOADS < 64, "the counter of outstanding loads has six bits");
     constexpr int STAGE = (BT + BN) * KB;
     __shared__ __align__(16) char lds[STAGES * STAGE];
@@ -196,6 +239,7 @@ __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_staged_kern
     uint32_t t_tile, n_tile;
     order.tile(blockIdx.x, t_tile, n_tile);
     const int64_t t0 = (int64_t)t_tile * BT, n0 = (int64_t)n_tile * BN;
+    // 16 rows of one chunk are read together: their places cover the banks
     const auto place = [](int row, int chunk) { return row * KB + ((chunk ^ (row >> 1)) & 7) * 16; };
 
     // a load moves 8 rows of 128 bytes; which chunk a lane takes follows from the place that it fills
@@ -207,16 +251,16 @@ __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_staged_kern
     };
     const i32x4 codes = resource(a.codes, t0, a.tokens), weight = resource(a.weight, n0, a.n);
     uint32_t c_off[C_LOADS], w_off[W_LOADS];
-    const auto lane_offset = [&](int group) { // 8 rows from 8 * group on
-        const int row = group * 8 + (lane >> 3);
-        return (uint32_t)row * (uint32_t)a.k + (uint32_t)(((lane & 7) ^ (row >> 1)) & 7) * 16u;
+    const auto lane_offset = [&](int rows8) { // rows from 8 * rows8 on
+        const int row = rows8 * 8 + (lane >> 3);
+        return (uint32_t)row * (uint32_t)a.k + (uint32_t)((lane ^ (row >> 1)) & (CH - 1)) * 16u;
     };
 #pragma unroll
     for (int i = 0; i < C_LOADS; ++i) c_off[i] = lane_offset(wave * C_LOADS + i);
 #pragma unroll
     for (int i = 0; i < W_LOADS; ++i) w_off[i] = lane_offset(wave * W_LOADS + i);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    const int blocks = (int)((a.k + KB - 1) / KB);
+    const int blocks = (int)((a.k + KB - 1) / KB), whole = (int)(a.k / KB);
     const auto issue = [&](int block, int stage) {
         const uint32_t at = lds0 + stage * STAGE;
 #pragma unroll
@@ -267,7 +311,6 @@ __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_staged_kern
     for (int i = 0; i < STAGES - 1; ++i)
         if (i < blocks) issue(i, i);
     int stage = 0;
-    const int whole = (int)(a.k / KB);
     for (int block = 0; block < whole; ++block) {
         if (block + STAGES - 2 < blocks) wait_for_loads<(STAGES - 2) * LOADS>();
         else wait_for_loads<0>();
@@ -281,8 +324,9 @@ __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_staged_kern
         __syncthreads();
         multiply(lds + stage * STAGE, (int)(a.k - (int64_t)whole * KB), std::true_type{});
     }
-
-    store_tile<T, WT, WN>(a, acc, t0 + wave_t * WT, n0 + wave_n * WN, lane);
+    __syncthreads(); // the stages have been read
+    static_assert(kStoreRoom<T, WN> * WAVES <= STAGES * STAGE);
+    store_tile<T, WT, WN>(a, acc, t0 + wave_t * WT, n0 + wave_n * WN, lane, lds + wave * kStoreRoom<T, WN>);
 }
 
 // ---- few tokens: bound by the weight's bytes ----
@@ -312,8 +356,11 @@ __global__ void __launch_bounds__(256) linear_dot_kernel(const LinearArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[r][m] = __builtin_amdgcn_sdot4((int)wv[r][i], (int)cv[m][i], sum[r][m], false);
     };
-    int64_t k = 0;
-    for (; k + AHEAD * 1024 <= a.k; k += AHEAD * 1024) {
+    // wavefronts begin at different places: see linear_pieces_kernel
+    constexpr int STEP = AHEAD * 1024;
+    const uint32_t steps = (uint32_t)(a.k / STEP), first = steps == 0 ? 0 : (uint32_t)(n0 / R) % steps;
+    for (uint32_t i = 0; i < steps; ++i) {
+        const int64_t k = (int64_t)(i + first < steps ? i + first : i + first - steps) * STEP;
         u32x4 wv[AHEAD][R], cv[AHEAD][M];
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
@@ -325,7 +372,7 @@ __global__ void __launch_bounds__(256) linear_dot_kernel(const LinearArgs a) {
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) add(wv[h], cv[h]);
     }
-    for (; k < a.k; k += 1024) {
+    for (int64_t k = (int64_t)steps * STEP; k < a.k; k += 1024) {
         u32x4 wv[R], cv[M];
 #pragma unroll
         for (int r = 0; r < R; ++r) wv[r] = load16(w[r], 0, 1, k + lane * 16, a.k);
@@ -354,66 +401,86 @@ __global__ void __launch_bounds__(256) linear_dot_kernel(const LinearArgs a) {
     store_element<T>(a.out + (t * a.n + n) * T::kBytes, y);
 }
 
-// MB x 16 tokens and NB x 16 channels a workgroup; its wavefronts take pieces of 128 bytes of the rows in turn, with operands straight
-// from memory (a lane's 16 bytes are its part of an instruction's operand), and are added up in LDS at the end.
-template <class T, int MB, int NB, int WAVES, int AHEAD>
-__global__ void __launch_bounds__(64 * WAVES) linear_skinny_kernel(const LinearArgs a, int32_t token_tiles) {
-    constexpr int TOKENS = 16 * MB, CHANNELS = 16 * NB;
-    __shared__ __align__(16) int32_t part[WAVES][TOKENS][CHANNELS + 4];
+// MB x 16 tokens and NB x 16 channels a workgroup; its wavefronts take pieces of 128 bytes of the rows in turn, each through LDS of its
+// own (STAGES pieces, no barrier), and are added up at the end.
+template <class T, int MB, int NB, int WAVES, int STAGES>
+__global__ void __launch_bounds__(64 * WAVES) linear_pieces_kernel(const LinearArgs a, int32_t token_tiles) {
+    constexpr int TOKENS = 16 * MB, CHANNELS = 16 * NB, KB = 128;
+    constexpr int LOADS = 2 * (MB + NB), STAGE = (TOKENS + CHANNELS) * KB, RING = STAGES * STAGE;
+    constexpr int PART = TOKENS * (CHANNELS + 4); // sums of a wavefront
+    constexpr int LDS = WAVES * (RING > PART * 4 ? RING : PART * 4);
+    static_assert(STAGES * LOADS < 64, "the counter of outstanding loads has six bits");
+    __shared__ __align__(16) char lds[LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
     const int64_t t0 = (int64_t)(blockIdx.x % token_tiles) * TOKENS, n0 = (int64_t)(blockIdx.x / token_tiles) * CHANNELS;
-    const int8_t *c[MB], *w[NB];
+    const auto place = [](int row, int chunk) { return row * KB + ((chunk ^ (row >> 1)) & 7) * 16; };
+    // rows that do not exist lie behind the resources' ends, as pieces behind the last do: they are not read
+    const auto resource = [&](const int8_t *base, int64_t row, int64_t rows, int most) {
+        const int64_t left = rows - row < most ? rows - row : most;
+        const uint64_t address = reinterpret_cast<uint64_t>(base + row * a.k);
+        return i32x4{__builtin_amdgcn_readfirstlane((int)address), __builtin_amdgcn_readfirstlane((int)((address >> 32) & 0xffff)),
+                     __builtin_amdgcn_readfirstlane((int)(left * a.k)), 0x00020000};
+    };
+    const i32x4 codes = resource(a.codes, t0, a.tokens, TOKENS), weight = resource(a.weight, n0, a.n, CHANNELS);
+    constexpr uint32_t kBehind = 0x40000000;
+    const int pieces = (int)((a.k + KB - 1) / KB);
+    const uint32_t row_off = (uint32_t)(lane >> 3) * (uint32_t)a.k, step = 8u * (uint32_t)a.k;
+    // rows 8 apart take chunks four places apart
+    const uint32_t chunk_even = (uint32_t)((lane ^ (lane >> 4)) & 7) * 16u, chunk_odd = chunk_even ^ 64u;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + wave * RING;
+    // workgroups begin at different pieces: rows that lie a power of two apart share memory channels, piece by piece
+    // (8 x 8192 x 8192: 19.5 us beginning together, 13.8 like this; 8 x 8320 x 8192 14 either way)
+    const int first = (int)(blockIdx.x * 13 % (uint32_t)pieces);
+    const auto turned = [&](int piece) { return piece + first >= pieces ? piece + first - pieces : piece + first; };
+    const auto issue = [&](int piece, int stage) {
+        const uint32_t at = row_off + (piece < pieces ? (uint32_t)turned(piece) * KB : kBehind);
 #pragma unroll
-    for (int m = 0; m < MB; ++m) {
-        const int64_t t = t0 + m * 16 + col;
-        c[m] = a.codes + (t < a.tokens ? t : a.tokens - 1) * a.k;
-    }
+        for (int i = 0; i < 2 * MB; ++i) load_to_lds(codes, at + i * step + (i & 1 ? chunk_odd : chunk_even), 0, lds0 + stage * STAGE + i * 1024);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int64_t at = n0 + n * 16 + col;
-        w[n] = a.weight + (at < a.n ? at : a.n - 1) * a.k;
-    }
+        for (int i = 0; i < 2 * NB; ++i)
+            load_to_lds(weight, at + i * step + (i & 1 ? chunk_odd : chunk_even), 0, lds0 + stage * STAGE + TOKENS * KB + i * 1024);
+    };
     i32x4 acc[NB][MB];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int m = 0; m < MB; ++m) acc[n][m] = i32x4{0, 0, 0, 0};
-    const auto multiply = [&](const u32x4 (&wv)[2][NB], const u32x4 (&cv)[2][MB]) {
+    const auto multiply = [&](int stage, int left) {
+        const char *const from = lds + wave * RING + stage * STAGE;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+            i32x4 w[NB], c[MB];
+#pragma unroll
+            for (int m = 0; m < MB; ++m) c[m] = *(const i32x4 *)(from + place(m * 16 + col, h * 4 + quad));
+#pragma unroll
+            for (int n = 0; n < NB; ++n) w[n] = *(const i32x4 *)(from + TOKENS * KB + place(n * 16 + col, h * 4 + quad));
+            if (left < KB) { // what lies behind the row's end counts as zero
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (h * 64 + quad * 16 + i * 4 >= left) w[n][i] = 0;
+            }
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int m = 0; m < MB; ++m)
-                    acc[n][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wv[h][n]), __builtin_bit_cast(i32x4, cv[h][m]), acc[n][m], 0, 0, 0);
-    };
-    int64_t k = (int64_t)wave * AHEAD * 128;
-    for (; k + AHEAD * 128 <= a.k; k += WAVES * AHEAD * 128) {
-        u32x4 wv[AHEAD][2][NB], cv[AHEAD][2][MB];
-#pragma unroll
-        for (int x = 0; x < AHEAD; ++x)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int n = 0; n < NB; ++n) wv[x][h][n] = load16_inside(w[n] + k + x * 128 + h * 64 + quad * 16);
-#pragma unroll
-                for (int m = 0; m < MB; ++m) cv[x][h][m] = load16_inside(c[m] + k + x * 128 + h * 64 + quad * 16);
-            }
-#pragma unroll
-        for (int x = 0; x < AHEAD; ++x) multiply(wv[x], cv[x]);
-    }
-    for (int x = 0; x < AHEAD && k < a.k; ++x, k += 128) { // the last piece of all, in one wavefront
-        u32x4 wv[2][NB], cv[2][MB];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int n = 0; n < NB; ++n) wv[h][n] = load16(w[n], 0, 1, k + h * 64 + quad * 16, a.k);
-#pragma unroll
-            for (int m = 0; m < MB; ++m) cv[h][m] = load16(c[m], 0, 1, k + h * 64 + quad * 16, a.k);
+                for (int m = 0; m < MB; ++m) acc[n][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[n], c[m], acc[n][m], 0, 0, 0);
         }
-        multiply(wv, cv);
+    };
+#pragma unroll
+    for (int x = 0; x < STAGES; ++x) issue(wave + x * WAVES, x);
+    int stage = 0;
+    for (int piece = wave; piece < pieces; piece += WAVES) {
+        wait_for_loads<(STAGES - 1) * LOADS>();
+        multiply(stage, (int)(a.k - (int64_t)turned(piece) * KB));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the stage has been read
+        issue(piece + STAGES * WAVES, stage);
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
+    wait_for_loads<0>();
+    __syncthreads();
+    int32_t(*const part)[TOKENS][CHANNELS + 4] = reinterpret_cast<int32_t(*)[TOKENS][CHANNELS + 4]>(lds);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -438,6 +505,12 @@ __global__ void __launch_bounds__(64 * WAVES) linear_skinny_kernel(const LinearA
     }
 }
 
+template <class T, int M>
+void launch_dot(const LinearArgs &a, hipStream_t s) {
+    if (a.n >= 8192) linear_dot_kernel<T, M, 4, 2><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
+    else linear_dot_kernel<T, M, 1, 4><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
+}
+
 template <class T, int BT, int BN, int WT, int WN, int STAGES>
 int launch_staged(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + BT - 1) / BT, channel_tiles = (a.n + BN - 1) / BN;
@@ -447,42 +520,73 @@ int launch_staged(const LinearArgs &a, hipStream_t s) {
     return TDE_OK;
 }
 
-template <class T, int M>
-void launch_dot(const LinearArgs &a, hipStream_t s) {
-    if (a.n >= 8192) linear_dot_kernel<T, M, 4, 2><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
-    else linear_dot_kernel<T, M, 1, 4><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
-}
-
-template <class T, int MB, int NB, int WAVES, int AHEAD>
-int launch_skinny(const LinearArgs &a, hipStream_t s) {
+template <class T, int MB, int NB, int WAVES, int STAGES>
+int launch_pieces(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + 16 * MB - 1) / (16 * MB), blocks = token_tiles * ((a.n + 16 * NB - 1) / (16 * NB));
     if (blocks > 0x7fffffff) return TDE_ETOOBIG;
-    linear_skinny_kernel<T, MB, NB, WAVES, AHEAD><<<(uint32_t)blocks, 64 * WAVES, 0, s>>>(a, (int32_t)token_tiles);
+    linear_pieces_kernel<T, MB, NB, WAVES, STAGES><<<(uint32_t)blocks, 64 * WAVES, 0, s>>>(a, (int32_t)token_tiles);
     return TDE_OK;
 }
 
-#ifndef FORCE
-#define FORCE 0
-#endif
+// ---- which kernel ----
+
+// From four tokens on every kernel works on tiles, and which one is best follows from how many rounds its tiles need on the units and
+// what 128 bytes of the rows cost in a round (microseconds, measured with every unit busy) beside what a launch costs at all:
+//
+//   tokens x channels  a round's 128 bytes  launch   e.g. (us, against the next best)
+//   256 x 256          1.9                  5        8192 x 8192 x 8192 487 (256 x 128: 553)
+//   256 x 128          1.17                 4        2048 x 4096 x 4096 41 (128 x 128: 49)
+//   128 x 128          0.66                 4        512 x 8192 x 8192 46 (256 x 128: 61)
+//   64 x 128           0.55                 3.5      1257 x 5000 x 1100 21.9 (64 x 64: 25.1)
+//   64 x 64            0.37 one a unit, 0.62 two a unit at once
+//                                           3.5      128 x 5120 x 7168 18.3 (64 x 32: 22.2)
+//   64 x 32 in pieces  0.25, 0.11 where fewer than half of the units are busy
+//                                           5.5      100 x 8192 x 1280 9.7 (64 x 64: 19.0)
+enum Tile { k256x256, k256x128, k128x128, k64x128, k64x64, kPieces };
+Tile best_tile(int64_t tokens, int64_t n, int64_t k) {
+    const int64_t cus = device_compute_units();
+    const auto tiles = [&](int64_t bt, int64_t bn) { return ((tokens + bt - 1) / bt) * ((n + bn - 1) / bn); };
+    const auto rounds = [&](int64_t t, int64_t at_once) { return (double)((t + at_once - 1) / at_once); };
+    const double blocks = (double)((k + 127) / 128);
+    const int64_t small = tiles(64, 64), pieces = tiles(64, 32);
+    const double cost[] = {
+        5.0 + blocks * 1.9 * rounds(tiles(256, 256), cus),
+        4.0 + blocks * 1.17 * rounds(tiles(256, 128), cus),
+        4.0 + blocks * 0.66 * rounds(tiles(128, 128), cus),
+        3.5 + blocks * 0.55 * rounds(tiles(64, 128), cus),
+        3.5 + blocks * (small <= cus ? 0.37 : 0.62 * rounds(small, 2 * cus)),
+        5.5 + blocks * (pieces * 2 <= cus ? 0.11 : 0.25 * rounds(pieces, cus)),
+    };
+    int best = 0;
+    for (int i = 1; i <= kPieces; ++i)
+        if (cost[i] < cost[best]) best = i;
+    return (Tile)best;
+}
+
 template <class T>
 int launch_typed(const LinearArgs &a, hipStream_t s) {
     int st = TDE_OK;
     const bool words = a.k % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.codes) | reinterpret_cast<uintptr_t>(a.weight)) & 3u) == 0;
-    if (a.tokens <= 4 && FORCE != 5) {
+    if (a.tokens <= 4) {
         if (a.tokens == 1) launch_dot<T, 1>(a, s);
         else if (a.tokens == 2) launch_dot<T, 2>(a, s);
         else launch_dot<T, 4>(a, s);
-    } else if (a.tokens <= 16) {
-        st = a.n >= 8192 ? launch_skinny<T, 1, 2, 8, 2>(a, s) : launch_skinny<T, 1, 1, 16, 2>(a, s);
-    } else if (a.tokens <= 32) {
-        st = a.n >= 8192 ? launch_skinny<T, 2, 2, 8, 2>(a, s) : launch_skinny<T, 2, 1, 16, 2>(a, s);
-    } else if (a.tokens <= 64) {
-        st = launch_skinny<T, 4, 2, 8, 2>(a, s);
+    } else if (words && a.tokens <= 64) {
+        // channels of a workgroup: two blocks of 16 where that leaves a workgroup for half of the units at least (16 x 5120 x 7168 9.0
+        // us, with one block 12.0; 16 x 8192 x 1280 6.7 and 5.9)
+        const bool two = (a.n + 31) / 32 >= device_compute_units() / 2;
+        if (a.tokens <= 16) st = two ? launch_pieces<T, 1, 2, 4, 3>(a, s) : launch_pieces<T, 1, 1, 8, 4>(a, s);
+        else if (a.tokens <= 32) st = two ? launch_pieces<T, 2, 2, 8, 2>(a, s) : launch_pieces<T, 2, 1, 8, 3>(a, s);
+        else st = two ? launch_pieces<T, 4, 2, 8, 1>(a, s) : launch_pieces<T, 4, 1, 4, 3>(a, s);
     } else if (words) {
-        const int64_t tiles256 = ((a.tokens + 255) / 256) * ((a.n + 255) / 256), tiles128 = ((a.tokens + 127) / 128) * ((a.n + 127) / 128);
-        if (FORCE == 1 || (FORCE == 0 && tiles256 >= 128)) st = launch_staged<T, 256, 256, 128, 64, 2>(a, s);
-        else if (FORCE == 2 || (FORCE == 0 && tiles128 >= 200)) st = launch_staged<T, 128, 128, 64, 64, 2>(a, s);
-        else st = launch_staged<T, 64, 64, 32, 32, 4>(a, s);
+        switch (best_tile(a.tokens, a.n, a.k)) {
+        case k256x256: st = launch_staged<T, 256, 256, 128, 64, 2>(a, s); break;
+        case k256x128: st = launch_staged<T, 256, 128, 64, 64, 3>(a, s); break;
+        case k128x128: st = launch_staged<T, 128, 128, 64, 32, 4>(a, s); break;
+        case k64x128: st = launch_staged<T, 64, 128, 32, 32, 5>(a, s); break;
+        case k64x64: st = launch_staged<T, 64, 64, 32, 32, 4>(a, s); break;
+        case kPieces: st = launch_pieces<T, 4, 2, 8, 1>(a, s); break;
+        }
     } else {
         const int64_t token_tiles = (a.tokens + 127) / 128, blocks = token_tiles * ((a.n + 127) / 128);
         if (blocks > 0x7fffffff) return TDE_ETOOBIG;
