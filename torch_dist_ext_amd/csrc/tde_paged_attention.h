@@ -7,6 +7,11 @@
 namespace tde {
 namespace block {
 
+// What joining the parts of a tile needs; chunks 0: nothing to join at this item.
+struct JoinItem {
+    int32_t chunks, tile, begin, count, len;
+};
+
 struct AttentionArgs {
     const char *q, *k, *v;
     char *out;
@@ -22,7 +27,9 @@ struct AttentionArgs {
     int32_t capacity;      // keys that a row of the page table can name
     int32_t dim;
     float scale_log2;      // scale * log2(e)
-    float *partial;        // [items, kv_heads, rows of a tile, D + 2 statistics]
+    float *partial;        // [items, kv_heads, rows of a tile, D + 4]: sums, their maximum and weight
+    JoinItem *joins;       // [items]
+    bool same_places;      // a key's value lies in its cache where the key does in its own
     bool zero_tail;        // rows behind the last sequence become zeros
 };
 
@@ -33,6 +40,7 @@ struct AttentionPlan {
     int64_t items;
     int64_t target;
     int32_t min_chunk;
+    int join_waves; // wavefronts that join a row
     int64_t workspace_bytes;
 };
 

@@ -57,7 +57,6 @@ struct Item {
     int32_t seq;      // seqs: rows behind the last sequence; -1: none
     int32_t tile;     // of the sequence
     int32_t chunk, chunks;
-    int32_t first;    // the sequence's first item
     int32_t begin, count; // its rows of the call
     int32_t len;      // its keys
     int32_t keys;     // of a chunk
@@ -86,14 +85,7 @@ __device__ __forceinline__ int32_t walked(const AttentionArgs &a, int32_t len) {
 
 // Keys of a chunk: all keys that the tiles have between them, over the number of items aimed at, in whole blocks of 64; sequences
 // of any lengths then give chunks of one size, and the number of items is at most target + tiles.
-template <int ROWS>
-__device__ __forceinline__ int32_t keys_of_chunk(const AttentionArgs &a, int lane) {
-    int64_t total = 0;
-    for (int i = lane; i < a.batch.seqs; i += 64) {
-        int32_t begin, count, len;
-        extent(a, i, begin, count, len);
-        total += (int64_t)tiles_of<ROWS>(a, count) * walked(a, len);
-    }
+__device__ __forceinline__ int32_t keys_of_chunk(const AttentionArgs &a, int64_t total) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) total += __shfl_xor((long long)total, m);
     int64_t keys = (total + a.target - 1) / a.target;
@@ -101,15 +93,23 @@ __device__ __forceinline__ int32_t keys_of_chunk(const AttentionArgs &a, int lan
     return (int32_t)clamped(keys, a.min_chunk, 0x7fffffc0);
 }
 
-// The item with number `want` (BY_ITEM), or the first item of sequence `want`; one wavefront, 64 sequences at a time.
-template <int ROWS, bool SPLIT, bool BY_ITEM>
+// The item with number `want`; one wavefront, 64 sequences at a time.
+template <int ROWS, bool SPLIT>
 __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int lane) {
-    Item it{-1, 0, 0, 1, 0, 0, 0, 0, 0x7fffffc0};
-    if (SPLIT) it.keys = keys_of_chunk<ROWS>(a, lane);
+    Item it{-1, 0, 0, 1, 0, 0, 0, 0x7fffffc0};
+    int32_t begin, count, len;
+    extent(a, lane, begin, count, len);
+    if (SPLIT) {
+        int64_t total = (int64_t)tiles_of<ROWS>(a, count) * walked(a, len);
+        for (int i = lane + 64; i < a.batch.seqs; i += 64) {
+            int32_t other, n, keys;
+            extent(a, i, other, n, keys);
+            total += (int64_t)tiles_of<ROWS>(a, n) * walked(a, keys);
+        }
+        it.keys = keys_of_chunk(a, total);
+    }
     int32_t passed = 0;
-    for (int base = 0; base <= a.batch.seqs; base += 64) {
-        int32_t begin, count, len;
-        extent(a, base + lane, begin, count, len);
+    for (int base = 0;;) {
         const int32_t tiles = tiles_of<ROWS>(a, count);
         const int32_t chunks = SPLIT && walked(a, len) > it.keys ? (walked(a, len) - 1) / it.keys + 1 : 1;
         const int32_t items = tiles * chunks;
@@ -119,41 +119,54 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
             const int32_t below = __shfl_up(upto, m);
             if (lane >= m) upto += below;
         }
-        const int32_t all = __builtin_amdgcn_readlane(upto, 63);
-        int at;
-        if (BY_ITEM) at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(passed + upto <= want));
-        else at = want - base;
-        if (BY_ITEM ? at < 64 : at < 64) {
+        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(passed + upto <= want));
+        if (at < 64) {
             it.seq = base + at;
             it.begin = __builtin_amdgcn_readlane(begin, at);
             it.count = __builtin_amdgcn_readlane(count, at);
             it.len = __builtin_amdgcn_readlane(len, at);
             it.chunks = __builtin_amdgcn_readlane(chunks, at);
-            it.first = passed + __builtin_amdgcn_readlane(upto - items, at);
-            const int32_t local = BY_ITEM ? want - it.first : 0;
-            const int32_t all_tiles = __builtin_amdgcn_readlane(tiles, at);
+            const int32_t local = want - passed - __builtin_amdgcn_readlane(upto - items, at);
             it.tile = local / it.chunks;
             it.chunk = local - it.tile * it.chunks;
             // unsplit, a sequence's last tiles, which see most keys, go first
-            if (!SPLIT) it.tile = all_tiles - 1 - it.tile;
+            if (!SPLIT) it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - it.tile;
             return it;
         }
-        passed += all;
+        passed += __builtin_amdgcn_readlane(upto, 63);
+        base += 64;
+        if (base > a.batch.seqs) return it;
+        extent(a, base + lane, begin, count, len);
     }
-    return it;
 }
+
+// x as if it were new here: what follows from it is computed in this place and not, as what never changes, before a loop through which
+// there is no register to keep it.
+__device__ __forceinline__ int in_place(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// 16 bytes a lane from memory to LDS: lane l's go to lds + 16 * l, lanes that are switched off leave their place as it is.  In assembly
+// because the compiler waits for every such load before any read from LDS; nothing returns in registers.  wait_for_loads() is the
+// wait that the data needs.
+__device__ __forceinline__ void load_to_lds(const char *p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 } // namespace
 
-// NB blocks of 16 rows a wavefront.  SHARED: the wavefronts have rows of their own and share the keys of a tile (double-buffered
-// in LDS); otherwise all have the same rows and take the tiles of keys in turn, each through LDS of its own, and are joined at the end.
+// NB blocks of 16 rows a wavefront.  SHARED: the wavefronts have rows of their own and share tiles of keys, double-buffered in LDS;
+// otherwise all have the same rows and take the tiles in turn, each through LDS of its own, and are joined at the end.
 template <class T, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
-__global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel(const AttentionArgs a) {
     constexpr int KT = SHARED && D <= 128 ? 64 : 32; // keys a tile
     constexpr int CH = D / 8;                        // chunks of 16 bytes a row
     constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
-    constexpr int LOADERS = 64 * (SHARED ? WAVES : 1);
-    constexpr int LOADS = KT * CH / LOADERS; // a thread, of keys and of values
+    constexpr int LOADERS = SHARED ? WAVES : 1;
+    constexpr int AT_ONCE = 64 / CH;                  // rows of a load
+    constexpr int LOADS = KT / AT_ONCE / LOADERS;     // a wavefront, of keys and of values
     constexpr int TILE = KT * D * 2;
     constexpr int BUFFERS = SHARED ? 2 : WAVES;
     constexpr int JOIN = SHARED ? 0 : WAVES * 16 * NB * (D + 4) * 4;
@@ -164,7 +177,17 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t item_index = a.kv_heads.quotient(blockIdx.x);
     const int kv_head = (int)(blockIdx.x - item_index * a.kv_heads.d);
-    const Item it = locate<ROWS, SPLIT, true>(a, (int32_t)item_index, lane);
+    const Item it = locate<ROWS, SPLIT>(a, (int32_t)item_index, lane);
+    const bool parts = SPLIT && it.chunks > 1; // this item's rows go to the second launch
+    if (SPLIT && kv_head == 0 && threadIdx.x == 0) {
+        // what the second launch has to know: nothing to join, or the first item of a tile's
+        JoinItem *const j = a.joins + item_index;
+        j->chunks = parts && it.chunk == 0 ? it.chunks : 0;
+        j->tile = it.tile;
+        j->begin = it.begin;
+        j->count = it.count;
+        j->len = it.len;
+    }
     if (it.seq < 0) return;
     const int group = (int)a.group.d;
     const int col = lane & 15, quad = lane >> 4;
@@ -196,10 +219,77 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
     // keys that the tile's rows see, of this item's chunk
     const int64_t top_row = std::min<int64_t>((int64_t)(it.tile + 1) * ROWS, rows_all) - 1;
     const int32_t top = it.len - it.count + (int32_t)a.group.quotient((uint32_t)top_row) + 1; // keys that the tile's last row sees
-    const int32_t lowest = it.len - it.count + (int32_t)a.group.quotient((uint32_t)((int64_t)it.tile * ROWS)) + 1;
+    const int32_t lowest = it.len - it.count + (int32_t)a.group.quotient((uint32_t)((int64_t)it.tile * ROWS)) + 1; // and its first
     const int64_t from64 = SPLIT ? (int64_t)it.chunk * it.keys : 0;
     const int32_t from = (int32_t)std::min<int64_t>(from64, 0x7fffffc0);
     const int32_t until = (int32_t)std::min<int64_t>(SPLIT ? from64 + it.keys : 0x7fffffc0, std::min(top, walked(a, it.len)));
+
+    // ---- loading ----
+    const int32_t *const table = a.batch.table + it.seq * a.batch.table_stride;
+    const char *const k_base = a.k + kv_head * a.k_head, *const v_base = a.v + kv_head * a.v_head;
+    constexpr int TILE_STEP = SHARED ? KT : KT * WAVES;
+    const int32_t first_key = from + (SHARED ? 0 : wave * KT);
+    // Where key `tile key + lane` lies in the caches, from their heads' first channels on: not there (kNoKey) from `until` on,
+    // lost (kNoPage) where the table or the cache has no page for it.
+    constexpr int64_t kNoKey = -1, kNoPage = -2;
+    struct Offsets {
+        int64_t k, v;
+    };
+    const auto offsets_of = [&](int64_t key0) -> Offsets {
+        const int64_t key = key0 + lane;
+        if ((KT < 64 && lane >= KT) || key >= until) return {kNoKey, kNoKey};
+        const uint32_t at = a.batch.page.quotient((uint32_t)key), slot = (uint32_t)key - at * a.batch.page.d;
+        const int32_t page = page_number(a.batch, table, at);
+        if (page < 0) return {kNoPage, kNoPage};
+        return {(int64_t)((uint64_t)(uint32_t)page * a.k_page + (uint64_t)slot * a.k_slot),
+                (int64_t)((uint64_t)(uint32_t)page * a.v_page + (uint64_t)slot * a.v_slot)};
+    };
+    const auto of_lane = [](int64_t x, int from) { return (int64_t)__shfl((long long)x, from); };
+    // Chunks are stored at places that spread over the banks what is read together: 16 keys of one chunk (keys), 8 keys of two
+    // neighbouring chunks (values).  A load fills places in order, so a lane's place says which chunk it takes.
+    const auto k_turn = [](int row) { return D == 64 ? (row >> 1) & 7 : row & 15; };
+    const auto v_turn = [](int row) { return D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1; };
+    // Turns reach M + 1 chunks; what lies beyond is written apart, so that it stays a constant.
+    constexpr int M = CH < 16 ? CH - 1 : 15;
+    const auto k_place = [&](int row, int first, int more) { return (row * CH + (first & ~M) + (((first & M) + more) ^ k_turn(row))) * 16; };
+    const auto v_place = [&](int row, int first, int more) { return (row * CH + (first & ~M) + (((first & M) + more) ^ v_turn(row))) * 16; };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(TDE_LDS char *)lds;
+    const auto load_tile = [&](const Offsets &where, uint32_t buffer) { // buffer: from the start of lds
+        const int wave_at = SHARED ? wave * LOADS * 1024 : 0;
+        const int l = in_place(lane), place = l % CH, load_row = (SHARED ? wave * LOADS * AT_ONCE : 0) + l / CH;
+        const bool whole = a.dim == D && __builtin_amdgcn_ballot_w64(where.k >= 0) == (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
+        if (whole && a.same_places) {
+#pragma unroll 4
+            for (int i = 0; i < LOADS; ++i) {
+                const int row = load_row + i * AT_ONCE;
+                const int64_t key = of_lane(where.k, row);
+                const uint32_t at = lds0 + buffer + wave_at + i * 1024;
+                load_to_lds(k_base + key + (place ^ k_turn(row)) * 16, at);
+                load_to_lds(v_base + key + (place ^ v_turn(row)) * 16, at + TILE);
+            }
+            return;
+        }
+#pragma unroll 2
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = load_row + i * AT_ONCE;
+            const int64_t k_at = of_lane(where.k, row), v_at = of_lane(where.v, row);
+            const int k_chunk = place ^ k_turn(row), v_chunk = place ^ v_turn(row);
+            const uint32_t at = buffer + wave_at + i * 1024;
+            if (k_at >= 0) {
+                if (k_chunk * 8 < a.dim) load_to_lds(k_base + k_at + k_chunk * 16, lds0 + at);
+                if (v_chunk * 8 < a.dim) load_to_lds(v_base + v_at + v_chunk * 16, lds0 + at + TILE);
+            } else { // a weight of zero would not keep what lies there from the sums; scores are replaced
+                *(u32x4 *)(lds + at + TILE + l * 16) = u32x4{0, 0, 0, 0};
+            }
+        }
+    };
+    uint32_t buf = SHARED ? 0 : wave * 2 * TILE;
+    if (a.dim < D) { // channels that the head does not have stay zeros
+        for (int i = threadIdx.x * 16; i < 2 * TILE * BUFFERS; i += 64 * WAVES * 16) *(u32x4 *)(lds + i) = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    Offsets where = offsets_of(first_key);
+    if (first_key < until) load_tile(where, buf);
 
     u32x4 q[NB][D / 32];
 #pragma unroll
@@ -224,116 +314,71 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
         for (int d = 0; d < D / 16; ++d) o[n][d] = f32x4{0, 0, 0, 0};
     }
 
-    // ---- loading ----
-    const int32_t *const table = a.batch.table + it.seq * a.batch.table_stride;
-    const int loader = SHARED ? (int)threadIdx.x : lane;
-    const int load_row = loader / CH, load_chunk = loader % CH; // rows load_row + i * LOADERS / CH
-    constexpr int ROW_STEP = LOADERS / CH;
-    const bool chunk_there = load_chunk * 8 < a.dim;
-    const char *const k_base = a.k + kv_head * a.k_head + load_chunk * 16, *const v_base = a.v + kv_head * a.v_head + load_chunk * 16;
-    constexpr int TILE_STEP = SHARED ? KT : KT * WAVES;
-    const int32_t first_key = from + (SHARED ? 0 : wave * KT);
-
-    u32x4 kreg[LOADS], vreg[LOADS];
-    // Where key `tile key + lane` lies in the caches, from their heads' first channels on: not there (kNoKey) from `until` on,
-    // lost (kNoPage) where the table or the cache has no page for it.
-    constexpr int64_t kNoKey = -1, kNoPage = -2;
-    struct Offsets {
-        int64_t k, v;
-    };
-    const auto offsets_of = [&](int32_t key0) -> Offsets {
-        const int64_t key = (int64_t)key0 + lane;
-        if ((KT < 64 && lane >= KT) || key >= until) return {kNoKey, kNoKey};
-        const uint32_t at = a.batch.page.quotient((uint32_t)key), slot = (uint32_t)key - at * a.batch.page.d;
-        const int32_t page = page_number(a.batch, table, at);
-        if (page < 0) return {kNoPage, kNoPage};
-        return {(int64_t)((uint64_t)(uint32_t)page * a.k_page + (uint64_t)slot * a.k_slot),
-                (int64_t)((uint64_t)(uint32_t)page * a.v_page + (uint64_t)slot * a.v_slot)};
-    };
-    const auto of_lane = [](int64_t x, int from) { return (int64_t)__shfl((long long)x, from); };
-    const auto load_tile = [&](const Offsets &where) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int row = load_row + i * ROW_STEP;
-            const int64_t k_at = of_lane(where.k, row), v_at = of_lane(where.v, row);
-            kreg[i] = vreg[i] = u32x4{0, 0, 0, 0};
-            if (k_at >= 0 && chunk_there) {
-                kreg[i] = *(const __attribute__((address_space(1))) u32x4 *)(k_base + k_at);
-                vreg[i] = *(const __attribute__((address_space(1))) u32x4 *)(v_base + v_at);
-            }
-        }
-    };
-    // Chunks are stored at places that spread over the banks what is read together: 16 keys of one chunk (keys), 8 keys of two
-    // neighbouring chunks (values).
-    const auto k_place = [](int row, int chunk) { return (row * CH + (chunk ^ (D == 64 ? (row >> 1) & 7 : row & 15))) * 16; };
-    const auto v_place = [](int row, int chunk) { return (row * CH + (chunk ^ (D == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1))) * 16; };
-    const auto store_tile = [&](char *buf) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int row = load_row + i * ROW_STEP;
-            *(u32x4 *)(buf + k_place(row, load_chunk)) = kreg[i];
-            *(u32x4 *)(buf + TILE + v_place(row, load_chunk)) = vreg[i];
-        }
-    };
-    // whether this thread's values of the tile hold an infinity or a NaN
-    const auto not_finite = [&]() {
-        // an exponent of ones plus one at its lowest bit carries out of its field; the field's neighbours are masked off before
-        constexpr uint32_t E = Mfma<T>::kExponent, LOW = E & (~E + 1u); // the field and its lowest bit
-        uint32_t carried = 0;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) carried |= (vreg[i][w] & (E | E << 16)) + (LOW | LOW << 16);
-        return (carried & 0x80008000u) != 0;
-    };
-
-    int32_t key0 = first_key;
-    Offsets where{kNoKey, kNoKey}, where_next{kNoKey, kNoKey};
-    char *buf = lds + (SHARED ? 0 : wave * 2 * TILE);
-    bool poisoned = false; // values of the tile in LDS that not all rows see are not all finite
-    const auto publish = [&](int32_t key) { // kreg, vreg -> buf, visible to the readers afterwards
-        store_tile(buf);
-        const bool partly_seen = key + KT > lowest;
-        if constexpr (SHARED) {
-            if (partly_seen) poisoned = __syncthreads_or(not_finite());
-            else {
-                poisoned = false;
-                __syncthreads();
-            }
-        } else {
-            poisoned = partly_seen && __builtin_amdgcn_ballot_w64(not_finite()) != 0;
+    const auto sync = [] { // between what a tile's readers and writers do in LDS
+        if constexpr (SHARED) __syncthreads();
+        else {
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
     };
-    if (key0 < until) {
-        where = offsets_of(key0);
-        load_tile(where);
-        if ((int64_t)key0 + TILE_STEP < until) where_next = offsets_of(key0 + TILE_STEP);
-        publish(key0);
-    }
-    while (key0 < until) {
-        const int64_t next = (int64_t)key0 + TILE_STEP;
-        const uint64_t lost = __builtin_amdgcn_ballot_w64(where.k == kNoPage);
-        if (next < until) {
+    int64_t next = (int64_t)first_key + TILE_STEP;
+    Offsets where_next = offsets_of(next);
+    for (int32_t key0 = first_key; key0 < until;) {
+        wait_for_loads();
+        sync();
+        const uint64_t lost = __builtin_amdgcn_ballot_w64(where.k == kNoPage); // keys without a page
+        if (SHARED && next < until) {
+            load_tile(where_next, buf ^ (2 * TILE));
             where = where_next;
-            load_tile(where);
-            if (next + TILE_STEP < until) where_next = offsets_of((int32_t)(next + TILE_STEP));
+            where_next = offsets_of(next + TILE_STEP);
         }
 
+        // whether values that not all rows see hold an infinity or a NaN
+        bool poisoned = false;
+        if (std::min<int64_t>((int64_t)key0 + KT, until) > lowest) {
+            // an exponent of ones plus one at its lowest bit carries out of its field; the field's neighbours are masked off before
+            constexpr uint32_t E = Mfma<T>::kExponent, LOW = E & (~E + 1u);
+            uint32_t carried = 0;
+            const char *const mine = lds + buf + TILE + in_place(SHARED ? (int)threadIdx.x : lane) * 16;
+#pragma unroll 4
+            for (int i = 0; i < TILE; i += 64 * LOADERS * 16) {
+                const u32x4 v = *(const u32x4 *)(mine + i);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) carried |= (v[w] & (E | E << 16)) + (LOW | LOW << 16);
+            }
+            if constexpr (SHARED) poisoned = __syncthreads_or((carried & 0x80008000u) != 0);
+            else poisoned = __builtin_amdgcn_ballot_w64((carried & 0x80008000u) != 0) != 0;
+        }
+
+        __builtin_amdgcn_sched_barrier(0);
         // ---- scores ----
+        // Operands come in units of two: the next unit's reads go ahead of this one's products, and no further, which
+        // registers would have to pay for.
         f32x4 s[NB][KT / 16];
+        {
+            constexpr int U = 2, UNITS = KT / 16 * (D / 32 / U);
+            u32x4 kf[2][U];
+            const auto read = [&](int unit) {
+                const int kb = unit / (D / 32 / U), st = unit % (D / 32 / U) * U;
 #pragma unroll
-        for (int kb = 0; kb < KT / 16; ++kb) {
+                for (int u = 0; u < U; ++u) kf[unit & 1][u] = *(const u32x4 *)(lds + buf + k_place(kb * 16 + col, (st + u) * 4, quad));
+            };
+            read(0);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) s[n][kb] = f32x4{0, 0, 0, 0};
+            for (int unit = 0; unit < UNITS; ++unit) {
+                const int kb = unit / (D / 32 / U), st = unit % (D / 32 / U) * U;
+                if (unit + 1 < UNITS) read(unit + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int st = 0; st < D / 32; ++st) {
-                const u32x4 kf = *(const u32x4 *)(buf + k_place(kb * 16 + col, st * 4 + quad));
+                for (int n = 0; n < NB; ++n) {
+                    if (st == 0) s[n][kb] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int n = 0; n < NB; ++n) s[n][kb] = Mfma<T>::mul(kf, q[n][st], s[n][kb]);
+                    for (int u = 0; u < U; ++u) s[n][kb] = Mfma<T>::mul(kf[unit & 1][u], q[n][st + u], s[n][kb]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
         if (lost != 0) {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
@@ -341,34 +386,50 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
                 for (int kb = 0; kb < KT / 16; ++kb)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if ((lost >> (kb * 16 + quad * 4 + r)) & 1) s[n][kb][r] = __builtin_nanf("");
+                        if ((lost >> (quad * 4) >> (kb * 16 + r)) & 1) s[n][kb][r] = __builtin_nanf("");
         }
-        const bool edge = key0 + KT > lowest || key0 + KT > until;
-        if (edge) {
+        if ((int64_t)key0 + KT > std::min(lowest, until)) {
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                const int32_t see = std::min(last[n], until - 1) - key0;
+                const int32_t see = std::min(last[n], until - 1) - key0 - quad * 4;
 #pragma unroll
                 for (int kb = 0; kb < KT / 16; ++kb)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (kb * 16 + quad * 4 + r > see) s[n][kb][r] = -__builtin_inff();
+                        if (kb * 16 + r > see) s[n][kb][r] = -__builtin_inff();
             }
         }
 
         // ---- softmax ----
-        u32x4 p[NB][KT / 32];
+        // The maximum that weights refer to only moves once a score exceeds it by 8 octaves: weights stay below 2^8, the largest of a
+        // row at 1 at least, and sums are rarely rescaled.
+        float top_score[NB];
+        bool grown = false;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            float top_score = s[n][0][0];
+            float t = s[n][0][0];
 #pragma unroll
             for (int kb = 0; kb < KT / 16; ++kb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) top_score = __builtin_fmaxf(top_score, s[n][kb][r]);
-            const float m_new = __builtin_fmaxf(m[n], max_of_row(top_score));
-            const float shift = m_new == -__builtin_inff() ? 0.0f : m_new * a.scale_log2; // nothing seen yet: every weight is 0
-            const float alpha = __builtin_amdgcn_exp2f(m[n] * a.scale_log2 - shift);
-            m[n] = m_new;
+                for (int r = 0; r < 4; ++r) t = __builtin_fmaxf(t, s[n][kb][r]);
+            top_score[n] = __builtin_fmaxf(m[n], max_of_row(t));
+            grown = grown || (top_score[n] - m[n]) * a.scale_log2 > 8.0f;
+        }
+        if (__builtin_amdgcn_ballot_w64(grown) != 0) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const float shift = top_score[n] == -__builtin_inff() ? 0.0f : top_score[n] * a.scale_log2;
+                const float alpha = __builtin_amdgcn_exp2f(m[n] * a.scale_log2 - shift);
+                m[n] = top_score[n];
+                l[n] *= alpha;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) o[n][d] *= alpha;
+            }
+        }
+        u32x4 p[NB][KT / 32];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const float shift = m[n] == -__builtin_inff() ? 0.0f : m[n] * a.scale_log2; // nothing seen yet: every weight is 0
             float sum = 0.0f;
 #pragma unroll
             for (int kb = 0; kb < KT / 16; ++kb)
@@ -377,73 +438,61 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
                     s[n][kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][r], a.scale_log2, -shift));
                     sum += s[n][kb][r];
                 }
-            l[n] = l[n] * alpha + sum;
+            l[n] += sum;
 #pragma unroll
             for (int ks = 0; ks < KT / 32; ++ks)
                 p[n][ks] = u32x4{T::narrow(s[n][2 * ks][0], s[n][2 * ks][1]), T::narrow(s[n][2 * ks][2], s[n][2 * ks][3]),
                                  T::narrow(s[n][2 * ks + 1][0], s[n][2 * ks + 1][1]), T::narrow(s[n][2 * ks + 1][2], s[n][2 * ks + 1][3])};
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) o[n][d] *= alpha;
         }
 
+        __builtin_amdgcn_sched_barrier(0);
         // ---- values ----
-        const auto value_operand = [&](int ks, int d) {
-            // 4 keys x 16 channels for each 16 lanes, transposed on the way: a lane gets one channel of the keys 4 * quad ... + 3
+        // 4 keys x 16 channels for each 16 lanes, transposed on the way: a lane gets one channel of the keys 4 * quad ... + 3 and,
+        // 16 keys on, of as many again
+        const auto value_operand = [&](const char *tile, int quad, int col, int ks, int d) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
-            const int row = ks * 32 + quad * 4 + (col >> 2), chunk = d * 2 + ((col & 3) >> 1), within = (col & 1) * 8;
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(buf + TILE + v_place(row, chunk) + within));
-            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(buf + TILE + v_place(row + 16, chunk) + within));
+            const int row = ks * 32 + quad * 4 + (col >> 2), more = (col & 3) >> 1, within = (col & 1) * 8;
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(tile + v_place(row, d * 2, more) + within));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(tile + v_place(row + 16, d * 2, more) + within));
             const u32x2 xu = __builtin_bit_cast(u32x2, x), yu = __builtin_bit_cast(u32x2, y);
             return u32x4{xu[0], xu[1], yu[0], yu[1]};
         };
-        if (__builtin_expect(!poisoned, 1)) {
-#pragma unroll
-            for (int ks = 0; ks < KT / 32; ++ks)
-#pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                    const u32x4 vf = value_operand(ks, d);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) o[n][d] = Mfma<T>::mul(vf, p[n][ks], o[n][d]);
-                }
-        } else {
-            // A weight of zero does not keep an infinity or NaN from the product.  Here such values are taken out of it, and which
+        if (__builtin_expect(poisoned, 0)) {
+            // A weight of zero does not keep an infinity or NaN from the product.  Such values are taken out of the tile, and which
             // of them a row sees is counted by a product of its own: 1 for +inf, 128 for -inf, 16384 for NaN, 64 keys at most.
             constexpr uint32_t E = Mfma<T>::kExponent, M = Mfma<T>::kMantissa;
 #pragma unroll 1
             for (int ks = 0; ks < KT / 32; ++ks) {
-                u32x4 seen[NB], weights[NB]; // 1.0 where the row sees the key
+                const int here_quad = in_place(quad), here_col = in_place(col);
+                u32x4 seen[NB]; // 1.0 where the row sees the key
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     const int32_t see = std::min(last[n], until - 1) - key0 - ks * 32;
                     const uint32_t one = T::narrow1(1.0f);
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const int key = (w >> 1) * 16 + quad * 4 + (w & 1) * 2;
+                        const int key = (w >> 1) * 16 + here_quad * 4 + (w & 1) * 2;
                         seen[n][w] = (one & ~(uint32_t)((see - key) >> 31)) | ((one & ~(uint32_t)((see - key - 1) >> 31)) << 16);
                     }
-                    weights[n] = ks == 0 ? p[n][0] : p[n][KT / 32 - 1];
                 }
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
-                    __builtin_amdgcn_sched_barrier(0); // one after the other: interleaved they run out of scalar registers
-                    u32x4 vf = value_operand(ks, d), mark;
+                    __builtin_amdgcn_sched_barrier(0); // one after the other: interleaved they take too many registers
+                    const u32x4 vf = value_operand(lds + buf + TILE, here_quad, here_col, ks, d);
+                    u32x4 mark;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        uint32_t finite = 0, marks = 0;
+                        uint32_t marks = 0;
 #pragma unroll
                         for (int hi = 0; hi < 32; hi += 16) {
                             const uint32_t h = (vf[w] >> hi) & 0xffffu;
                             const float code = (h & M) != 0 ? 16384.0f : ((h & 0x8000u) != 0 ? 128.0f : 1.0f);
-                            const uint32_t is = (h & E) == E ? 0xffffu : 0u;
-                            finite |= (h & ~is) << hi;
-                            marks |= (T::narrow1(code) & is) << hi;
+                            marks |= (T::narrow1(code) & ((h & E) == E ? 0xffffu : 0u)) << hi;
                         }
-                        vf[w] = finite;
                         mark[w] = marks;
                     }
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
-                        o[n][d] = Mfma<T>::mul(vf, weights[n], o[n][d]);
                         const f32x4 found = Mfma<T>::mul(mark, seen[n], f32x4{0, 0, 0, 0});
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -456,13 +505,51 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
                     }
                 }
             }
+            sync();
+            char *const mine = lds + buf + TILE + in_place(SHARED ? (int)threadIdx.x : lane) * 16;
+#pragma unroll 1
+            for (int i = 0; i < TILE; i += 64 * LOADERS * 16) {
+                u32x4 v = *(const u32x4 *)(mine + i);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    if ((v[w] & E) == E) v[w] &= 0xffff0000u;
+                    if ((v[w] >> 16 & E) == E) v[w] &= 0x0000ffffu;
+                }
+                *(u32x4 *)(mine + i) = v;
+            }
+            sync();
+        }
+        {
+            constexpr int U = 4, UNITS = KT / 32 * (D / 16 / U);
+            u32x4 vf[2][U];
+            const auto read = [&](int unit) {
+                const int ks = unit / (D / 16 / U), d = unit % (D / 16 / U) * U;
+#pragma unroll
+                for (int u = 0; u < U; ++u) vf[unit & 1][u] = value_operand(lds + buf + TILE, quad, col, ks, d + u);
+            };
+            read(0);
+#pragma unroll
+            for (int unit = 0; unit < UNITS; ++unit) {
+                const int ks = unit / (D / 16 / U), d = unit % (D / 16 / U) * U;
+                if (unit + 1 < UNITS) read(unit + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], p[n][ks], o[n][d + u]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
 
-        if (next < until) {
-            if constexpr (SHARED) buf = buf == lds ? lds + 2 * TILE : lds;
-            publish((int32_t)next);
+        if constexpr (SHARED) buf ^= 2 * TILE;
+        else if (next < until) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the tile has been read
+            load_tile(where_next, buf);
+            where = where_next;
+            where_next = offsets_of(next + TILE_STEP);
         }
         key0 = (int32_t)std::min<int64_t>(next, 0x7fffffff);
+        next += TILE_STEP;
     }
 
     // ---- what is left: a row's sum over its four lanes, then the row ----
@@ -474,7 +561,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             if (token[n] < 0) continue;
-            if constexpr (SPLIT) {
+            if (parts) {
                 float *const part = a.partial + (slot + row0 + n * 16 + col) * (D + 4);
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) *(f32x4 *)(part + d * 16 + quad * 4) = o[n][d];
@@ -522,7 +609,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
                 sum += *(const f32x4 *)(part + d) * weight;
                 all += part[D + 1] * weight;
             }
-            if constexpr (SPLIT) {
+            if (parts) {
                 float *const part = a.partial + (slot + row) * (D + 4);
                 *(f32x4 *)(part + d) = sum;
                 if (d == 0) *(f32x2 *)(part + D) = f32x2{top_m, all};
@@ -539,86 +626,110 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kernel(const AttentionAr
     }
 }
 
-// Joins the chunks of a row: a workgroup a row (token, query head), its wavefronts take chunks in turn.
-template <class T, int D, int ROWS>
-__global__ void __launch_bounds__(256) attention_join_kernel(const AttentionArgs a) {
+// Joins the chunks of a tile's rows: RW rows a workgroup, WAVES wavefronts a row, which take chunks in turn, eight at once.
+template <class T, int D, int ROWS, int RW, int WAVES>
+__global__ void __launch_bounds__(64 * RW * WAVES) attention_join_kernel(const AttentionArgs a) {
     constexpr int E = D / 64; // channels a lane
-    __shared__ float joined[4][D + 4];
+    constexpr int AHEAD = 8;
+    __shared__ float joined[RW * WAVES][D + 4];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t heads = a.kv_heads.d * a.group.d;
-    const int32_t token = (int32_t)(blockIdx.x / heads);
-    const int head = (int)(blockIdx.x - (uint32_t)token * heads);
-    const int seq = __builtin_amdgcn_readfirstlane(sequence_of(a.batch, token, lane));
-    if (seq >= a.batch.seqs) return; // rows behind the last sequence are the first launch's
-    const Item it = locate<ROWS, true, false>(a, seq, lane);
-    if (token < it.begin || token >= it.begin + it.count) return;
-    const uint32_t kv_head = a.group.quotient((uint32_t)head);
-    const int64_t r = (int64_t)(token - it.begin) * a.group.d + (head - kv_head * a.group.d);
-    const int64_t tile = r / ROWS;
-    const int row = (int)(r - tile * ROWS);
-    float top_m = -__builtin_inff(), sum[E] = {}, all = 0.0f;
-    const float *const parts =
-        a.partial + ((((int64_t)it.first + tile * it.chunks) * a.kv_heads.d + kv_head) * ROWS + row) * (int64_t)(D + 4);
-    const int64_t step = (int64_t)a.kv_heads.d * ROWS * (D + 4);
-    if ((int64_t)it.first + (tile + 1) * it.chunks > a.items) return; // only where starts do not ascend
-    for (int c = wave; c < it.chunks; c += 4) {
-        const float *const part = parts + c * step;
-        const float pm = part[D], pl = part[D + 1];
-        float x[E];
+    const uint32_t at = blockIdx.x / (ROWS / RW), item = a.kv_heads.quotient(at);
+    const int kv_head = (int)(at - item * a.kv_heads.d);
+    const JoinItem j = a.joins[item];
+    if (j.chunks == 0) return;
+    const int row = (int)(blockIdx.x % (ROWS / RW)) * RW + wave / WAVES;
+    const int64_t r = (int64_t)j.tile * ROWS + row;
+    const bool there = r < (int64_t)j.count * a.group.d;
+    if (WAVES == 1 && !there) return;
+    if (!(RW > 1 && WAVES > 1) && !there) return; // a workgroup of one row, or wavefronts of one each
+    float best = -__builtin_inff(), sum[E] = {}, all = 0.0f;
+    const int64_t step = (int64_t)a.kv_heads.d * ROWS * (D + 4); // from one item's partial results to the next one's
+    const float *const parts = a.partial + (((int64_t)item * a.kv_heads.d + kv_head) * ROWS + row) * (int64_t)(D + 4);
+    // chunks that are items of this call: all of them where starts ascend
+    const int chunks = there ? (int)std::min<int64_t>(j.chunks, a.items - (int64_t)item) : 0;
+    for (int c0 = wave % WAVES; c0 < chunks; c0 += WAVES * AHEAD) {
+        float pm[AHEAD], pl[AHEAD], x[AHEAD][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = part[lane * E + e];
-        const float m_new = __builtin_fmaxf(top_m, pm);
-        const float shift = m_new == -__builtin_inff() ? 0.0f : m_new * a.scale_log2;
-        const float old = __builtin_amdgcn_exp2f(top_m * a.scale_log2 - shift), weight = __builtin_amdgcn_exp2f(pm * a.scale_log2 - shift);
-        all = all * old + pl * weight;
+        for (int i = 0; i < AHEAD; ++i) {
+            const int c = c0 + i * WAVES;
+            const float *const part = parts + (c < chunks ? c : c0) * step;
+            pm[i] = c < chunks ? part[D] : -__builtin_inff();
+            pl[i] = part[D + 1];
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] = sum[e] * old + x[e] * weight;
-        top_m = m_new;
+            for (int e = 0; e < E; ++e) x[i][e] = part[lane * E + e];
+        }
+        float top = best;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) top = __builtin_fmaxf(top, pm[i]);
+        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale_log2;
+        const float old = __builtin_amdgcn_exp2f(best * a.scale_log2 - shift);
+        all *= old;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] *= old;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const float weight = __builtin_amdgcn_exp2f(pm[i] * a.scale_log2 - shift);
+            const bool counts = c0 + i * WAVES < chunks; // what a repeated chunk holds may not be finite
+            all += counts ? pl[i] * weight : 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[e] += counts ? x[i][e] * weight : 0.0f;
+        }
+        best = top;
+    }
+    const uint32_t t = a.group.quotient((uint32_t)r);
+    const int head = kv_head * (int)a.group.d + (int)((uint32_t)r - t * a.group.d);
+    char *const to = a.out + (j.begin + (int32_t)t) * a.out_token + head * a.out_head;
+    const bool sees = j.len - j.count + (int32_t)t >= 0;
+    if constexpr (WAVES > 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) joined[wave][lane * E + e] = sum[e];
+        if (lane == 0) {
+            joined[wave][D] = best;
+            joined[wave][D + 1] = all;
+        }
+        __syncthreads();
+        if (wave % WAVES != 0 || !there) return;
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top = __builtin_fmaxf(top, joined[wave + w][D]);
+        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale_log2;
+        all = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float weight = __builtin_amdgcn_exp2f(joined[wave + w][D] * a.scale_log2 - shift);
+            all += joined[wave + w][D + 1] * weight;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[e] += joined[wave + w][lane * E + e] * weight;
+        }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) joined[wave][lane * E + e] = sum[e];
-    if (lane == 0) {
-        joined[wave][D] = top_m;
-        joined[wave][D + 1] = all;
-    }
-    __syncthreads();
-    if (threadIdx.x * 2 >= (uint32_t)a.dim) return;
-    float best = joined[0][D];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) best = __builtin_fmaxf(best, joined[w][D]);
-    const float shift = best == -__builtin_inff() ? 0.0f : best * a.scale_log2;
-    float y0 = 0.0f, y1 = 0.0f, total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float weight = __builtin_amdgcn_exp2f(joined[w][D] * a.scale_log2 - shift);
-        total += joined[w][D + 1] * weight;
-        y0 += joined[w][2 * threadIdx.x] * weight;
-        y1 += joined[w][2 * threadIdx.x + 1] * weight;
-    }
-    const bool sees = it.len - it.count + (token - it.begin) >= 0;
-    const uint32_t pair = sees ? T::narrow(y0 / total, y1 / total) : 0u;
-    store_words<4>(a.out + token * a.out_token + head * a.out_head + threadIdx.x * 4, Words<4>{{pair}});
+    for (int e = 0; e < E; ++e)
+        if (lane * E + e < a.dim) store_element<T>(to + (lane * E + e) * 2, sees ? sum[e] / all : 0.0f);
 }
 
 namespace {
 
 template <class T, int D, int NB, int WAVES, bool SHARED>
-void launch_one(const AttentionArgs &a, bool split, uint32_t blocks, hipStream_t s) {
-    if (!split) {
+void launch_one(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks, hipStream_t s) {
+    if (!p.split) {
         attention_kernel<T, D, NB, WAVES, SHARED, false><<<blocks, 64 * WAVES, 0, s>>>(a);
         return;
     }
+    constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
     attention_kernel<T, D, NB, WAVES, SHARED, true><<<blocks, 64 * WAVES, 0, s>>>(a);
-    const uint32_t rows = (uint32_t)(a.tokens * a.kv_heads.d * a.group.d);
-    attention_join_kernel<T, D, 16 * NB *(SHARED ? WAVES : 1)><<<rows, 256, 0, s>>>(a);
+    if (p.join_waves == 16) attention_join_kernel<T, D, ROWS, 1, 16><<<blocks * ROWS, 1024, 0, s>>>(a);
+    else attention_join_kernel<T, D, ROWS, 4, 1><<<blocks * (ROWS / 4), 256, 0, s>>>(a);
 }
 
 template <class T, int D>
 void launch_dim(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks, hipStream_t s) {
-    if constexpr (D == 256) launch_one<T, D, 1, 4, true>(a, p.split, blocks, s);
-    else if (p.rows == 16) launch_one<T, D, 1, 4, false>(a, p.split, blocks, s);
-    else launch_one<T, D, 2, 4, true>(a, p.split, blocks, s);
+    constexpr int ALONE = D == 256 ? 2 : 4; // wavefronts that each hold tiles of their own in LDS
+    if (p.rows == 16) launch_one<T, D, 1, ALONE, false>(a, p, blocks, s);
+    else if constexpr (D == 256) launch_one<T, D, 1, 4, true>(a, p, blocks, s);
+    else launch_one<T, D, 2, 4, true>(a, p, blocks, s);
 }
 
 template <class T>
@@ -636,20 +747,18 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
     p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
     const int64_t group = q_heads / kv_heads, rows_all = tokens * group;
     if (rows_all > 0x7fffff00) return TDE_ETOOBIG;
-    p->rows = p->wide_dim == 256 ? 64 : (seqs > 0 && rows_all > (int64_t)seqs * 16 ? 128 : 16);
+    p->rows = rows_all <= (int64_t)seqs * 16 ? 16 : (p->wide_dim == 256 ? 64 : 128);
     const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence and one behind the last
     const int64_t cus = device_compute_units();
     p->min_chunk = 256;
-    const int64_t full = rows_all / p->rows > 0 ? rows_all / p->rows : 1; // rather how many there are
-    const int64_t filled = std::max<int64_t>(full, std::min<int64_t>(seqs, tokens)) * kv_heads;
-    p->split = filled < 4 * cus && capacity > p->min_chunk;
-    p->target = std::max<int64_t>(1, 4 * cus / kv_heads);
+    const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // tiles, rather
+    p->split = likely * kv_heads < (p->rows == 16 ? 4 : 1) * cus && capacity > p->min_chunk;
+    p->target = std::max<int64_t>(1, (p->rows == 16 ? 4 : 2) * cus / kv_heads);
     p->items = tiles + (p->split ? p->target : 0);
-    if (p->items > 0x7fffff00 / kv_heads) return TDE_ETOOBIG;
-    if (p->split) {
-        if (rows_all * kv_heads > 0x7fffff00) return TDE_ETOOBIG;
-        p->workspace_bytes = p->items * kv_heads * p->rows * (int64_t)(p->wide_dim + 4) * 4;
-    }
+    if (p->items > 0x7fffff00 / kv_heads / p->rows) return TDE_ETOOBIG;
+    p->join_waves = p->target / likely >= 32 ? 16 : 1;
+    if (p->split)
+        p->workspace_bytes = p->items * (int64_t)sizeof(JoinItem) + p->items * kv_heads * p->rows * (int64_t)(p->wide_dim + 4) * 4;
     return TDE_OK;
 }
 
@@ -658,6 +767,9 @@ int launch_attention(AttentionArgs &a, const AttentionPlan &p, int dtype, hipStr
     a.target = p.target;
     a.min_chunk = p.min_chunk;
     a.capacity = (int32_t)std::min<int64_t>((int64_t)a.batch.table_pages * a.batch.page.d, 0x7fffff00);
+    a.same_places = a.k_page == a.v_page && a.k_slot == a.v_slot;
+    // the joins' items behind the partial results, which want 16-byte boundaries
+    a.joins = reinterpret_cast<JoinItem *>(a.partial + p.items * a.kv_heads.d * p.rows * (p.wide_dim + 4));
     const uint32_t blocks = (uint32_t)(p.items * a.kv_heads.d);
     if (dtype == TDE_BF16) launch_type<Bf16>(a, p, blocks, s);
     else launch_type<F16>(a, p, blocks, s);
