@@ -160,6 +160,17 @@ def test_starts_that_do_not_ascend_stay_in_bounds(tde):
         tde.paged_attention_out(q, k, v, table, starts, lens, band[1:-1])
         torch.cuda.synchronize()
         assert bool((band[0] == 3).all()) and bool((band[-1] == 3).all())
+    # with keys that are split
+    batch = Batch(new=[1, 1, 30], lens=[4000, 2000, 900], page_size=16, seed=28)
+    q = randn((batch.tokens, 4, 64), torch.bfloat16, 29).cuda()
+    k, v = (randn((batch.pages, 16, 2, 64), torch.bfloat16, 30 + i).cuda() for i in (0, 1))
+    table, _, lens = batch.on("cuda")
+    for starts in ([0, 30, 1, 32], [30, 2, 32, 5], [2, 32, 2, 32], [0, 32, 0, 32]):
+        starts = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        band = torch.full((batch.tokens + 2, 4, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+        tde.paged_attention_out(q, k, v, table, starts, lens, band[1:-1])
+        torch.cuda.synchronize()
+        assert bool((band[0] == 3).all()) and bool((band[-1] == 3).all())
 
 
 def test_offsets_beyond_32_bits(tde):

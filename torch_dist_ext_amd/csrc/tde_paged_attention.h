@@ -7,9 +7,10 @@
 namespace tde {
 namespace block {
 
-// What joining the parts of a tile needs; chunks 0: nothing to join at this item.
+// What joining the parts of a tile needs; chunks 0: nothing to join.
 struct JoinItem {
-    int32_t chunks, tile, begin, count, len;
+    int32_t chunks, item; // their number, and the first one's item
+    int32_t tile, begin, count, len;
 };
 
 struct AttentionArgs {
@@ -22,13 +23,13 @@ struct AttentionArgs {
     Divisor32 kv_heads;
     int64_t tokens;
     int64_t target;        // items that the split of the keys aims at, for each key head (split calls)
-    int32_t items;         // grid: items x key heads
+    int32_t items, tiles;  // at most; grids: items x key heads, and of the second launch tiles x key heads x rows
     int32_t min_chunk;     // keys of an item at least
     int32_t capacity;      // keys that a row of the page table can name
     int32_t dim;
     float scale_log2;      // scale * log2(e)
     float *partial;        // [items, kv_heads, rows of a tile, D + 4]: sums, their maximum and weight
-    JoinItem *joins;       // [items]
+    JoinItem *joins;       // [tiles]
     bool same_places;      // a key's value lies in its cache where the key does in its own
     bool zero_tail;        // rows behind the last sequence become zeros
 };
@@ -37,7 +38,7 @@ struct AttentionPlan {
     int wide_dim;   // 64, 128, 256: what the head is padded to in registers and LDS
     int rows;       // rows (token x query head of a group) of a tile
     bool split;     // the keys of a tile go to several workgroups, whose results a second launch joins
-    int64_t items;
+    int64_t items, tiles;
     int64_t target;
     int32_t min_chunk;
     int join_waves; // wavefronts that join a row

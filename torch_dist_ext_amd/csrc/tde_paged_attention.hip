@@ -15,10 +15,30 @@
 #include "tde_paged_attention.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tde {
 namespace block {
 
+#ifndef PR
+#define PR 0
+#endif
+#if PR == 1
+#define SB1 __builtin_amdgcn_s_setprio(1); __builtin_amdgcn_sched_barrier(0)
+#define SB2 __builtin_amdgcn_sched_barrier(0); __builtin_amdgcn_s_setprio(0)
+#elif PR == 2
+#define SB1 
+#define SB2 __builtin_amdgcn_sched_barrier(0)
+#elif PR == 3
+#define SB1 __builtin_amdgcn_sched_barrier(0)
+#define SB2 
+#elif PR == 4
+#define SB1
+#define SB2
+#else
+#define SB1 __builtin_amdgcn_sched_barrier(0)
+#define SB2 __builtin_amdgcn_sched_barrier(0)
+#endif
 #define TDE_LDS __attribute__((address_space(3)))
 
 namespace {
@@ -41,14 +61,23 @@ struct Mfma<F16> {
     static constexpr uint32_t kExponent = 0x7c00u, kMantissa = 0x03ffu;
 };
 
-// Maximum over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48).
+// Over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48): swaps of rows of 16 lanes and of halves, of a value
+// with itself, leave a pair's two values side by side.
+template <class F>
+__device__ __forceinline__ float over_row(float x, F f) {
+    // (elements of the pair by way of variables: a bit_cast of the second one reads the first)
+    const auto rows = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t r0 = rows[0], r1 = rows[1];
+    x = f(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+    const auto halves = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t h0 = halves[0], h1 = halves[1];
+    return f(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
+}
 __device__ __forceinline__ float max_of_row(float x) {
-    x = __builtin_fmaxf(x, __shfl_xor(x, 16));
-    return __builtin_fmaxf(x, __shfl_xor(x, 32));
+    return over_row(x, [](float a, float b) { return __builtin_fmaxf(a, b); });
 }
 __device__ __forceinline__ float sum_of_row(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    return over_row(x, [](float a, float b) { return a + b; });
 }
 
 // What a workgroup works on.  The items of a call: for every sequence its tiles of rows, for every tile its chunks of keys, in that
@@ -57,6 +86,7 @@ struct Item {
     int32_t seq;      // seqs: rows behind the last sequence; -1: none
     int32_t tile;     // of the sequence
     int32_t chunk, chunks;
+    int32_t tile_of_call; // number of its tile among the call's; for an item that is none the number of tiles and how many too far it is
     int32_t begin, count; // its rows of the call
     int32_t len;      // its keys
     int32_t keys;     // of a chunk
@@ -96,7 +126,7 @@ __device__ __forceinline__ int32_t keys_of_chunk(const AttentionArgs &a, int64_t
 // The item with number `want`; one wavefront, 64 sequences at a time.
 template <int ROWS, bool SPLIT>
 __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int lane) {
-    Item it{-1, 0, 0, 1, 0, 0, 0, 0x7fffffc0};
+    Item it{-1, 0, 0, 1, 0, 0, 0, 0, 0x7fffffc0};
     int32_t begin, count, len;
     extent(a, lane, begin, count, len);
     if (SPLIT) {
@@ -108,16 +138,19 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
         }
         it.keys = keys_of_chunk(a, total);
     }
-    int32_t passed = 0;
+    int32_t passed = 0, tiles_passed = 0;
     for (int base = 0;;) {
         const int32_t tiles = tiles_of<ROWS>(a, count);
         const int32_t chunks = SPLIT && walked(a, len) > it.keys ? (walked(a, len) - 1) / it.keys + 1 : 1;
         const int32_t items = tiles * chunks;
-        int32_t upto = items; // inclusive sum over the lanes
+        int32_t upto = items, tiles_upto = tiles; // inclusive sums over the lanes
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
-            const int32_t below = __shfl_up(upto, m);
-            if (lane >= m) upto += below;
+            const int32_t below = __shfl_up(upto, m), tiles_below = SPLIT ? __shfl_up(tiles_upto, m) : 0;
+            if (lane >= m) {
+                upto += below;
+                tiles_upto += tiles_below;
+            }
         }
         const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(passed + upto <= want));
         if (at < 64) {
@@ -129,13 +162,18 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
             const int32_t local = want - passed - __builtin_amdgcn_readlane(upto - items, at);
             it.tile = local / it.chunks;
             it.chunk = local - it.tile * it.chunks;
+            it.tile_of_call = tiles_passed + __builtin_amdgcn_readlane(tiles_upto - tiles, at) + it.tile;
             // unsplit, a sequence's last tiles, which see most keys, go first
             if (!SPLIT) it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - it.tile;
             return it;
         }
         passed += __builtin_amdgcn_readlane(upto, 63);
+        tiles_passed += __builtin_amdgcn_readlane(tiles_upto, 63);
         base += 64;
-        if (base > a.batch.seqs) return it;
+        if (base > a.batch.seqs) {
+            it.tile_of_call = tiles_passed + (want - passed);
+            return it;
+        }
         extent(a, base + lane, begin, count, len);
     }
 }
@@ -150,10 +188,18 @@ __device__ __forceinline__ int in_place(int x) {
 // 16 bytes a lane from memory to LDS: lane l's go to lds + 16 * l, lanes that are switched off leave their place as it is.  In assembly
 // because the compiler waits for every such load before any read from LDS; nothing returns in registers.  wait_for_loads() is the
 // wait that the data needs.
+// STREAM: read once, not to be kept in the caches.
+template <bool STREAM>
 __device__ __forceinline__ void load_to_lds(const char *p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
+    if constexpr (STREAM) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(p), "s"(lds) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
 }
-__device__ __forceinline__ void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Until at most N loads are outstanding.
+template <int N>
+__device__ __forceinline__ void wait_for_loads() {
+    static_assert(N < 64, "the counter has six bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
 } // namespace
 
@@ -179,10 +225,12 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     const int kv_head = (int)(blockIdx.x - item_index * a.kv_heads.d);
     const Item it = locate<ROWS, SPLIT>(a, (int32_t)item_index, lane);
     const bool parts = SPLIT && it.chunks > 1; // this item's rows go to the second launch
-    if (SPLIT && kv_head == 0 && threadIdx.x == 0) {
-        // what the second launch has to know: nothing to join, or the first item of a tile's
-        JoinItem *const j = a.joins + item_index;
-        j->chunks = parts && it.chunk == 0 ? it.chunks : 0;
+    if (SPLIT && kv_head == 0 && threadIdx.x == 0 && (it.seq < 0 || it.chunk == 0) && it.tile_of_call < a.tiles) {
+        // What the second launch has to know of each tile that there may be.  Items are at most a.target more than tiles, so the
+        // items that are none are enough for the tiles that are none.
+        JoinItem *const j = a.joins + it.tile_of_call;
+        j->chunks = parts ? it.chunks : 0;
+        j->item = (int32_t)item_index;
         j->tile = it.tile;
         j->begin = it.begin;
         j->count = it.count;
@@ -229,6 +277,17 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     const char *const k_base = a.k + kv_head * a.k_head, *const v_base = a.v + kv_head * a.v_head;
     constexpr int TILE_STEP = SHARED ? KT : KT * WAVES;
     const int32_t first_key = from + (SHARED ? 0 : wave * KT);
+    // Lane l holds the table's entry window + l: 64 pages, and a tile needs no more.  Nothing else in the loop is loaded by way of
+    // registers: the compiler would wait for it, and with it for every load to LDS that was issued before.
+    int32_t window = -64, entries = -1;
+    const auto look_up = [&](int32_t key0) { // before offsets_of(key0)
+        const uint32_t first = a.batch.page.quotient((uint32_t)key0);
+        const uint32_t end = a.batch.page.quotient((uint32_t)std::min<int64_t>((int64_t)key0 + KT, until) - 1);
+        if (end - (uint32_t)window < 64) return;
+        window = (int32_t)first;
+        entries = page_number(a.batch, table, first + lane);
+        asm volatile("" : "+v"(entries)); // waited for here
+    };
     // Where key `tile key + lane` lies in the caches, from their heads' first channels on: not there (kNoKey) from `until` on,
     // lost (kNoPage) where the table or the cache has no page for it.
     constexpr int64_t kNoKey = -1, kNoPage = -2;
@@ -237,9 +296,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     };
     const auto offsets_of = [&](int64_t key0) -> Offsets {
         const int64_t key = key0 + lane;
-        if ((KT < 64 && lane >= KT) || key >= until) return {kNoKey, kNoKey};
-        const uint32_t at = a.batch.page.quotient((uint32_t)key), slot = (uint32_t)key - at * a.batch.page.d;
-        const int32_t page = page_number(a.batch, table, at);
+        const bool there = (KT == 64 || lane < KT) && key < until;
+        const uint32_t at = a.batch.page.quotient((uint32_t)(there ? key : key0)), slot = (uint32_t)key - at * a.batch.page.d;
+        const int32_t page = __shfl(entries, (int)(at - (uint32_t)window));
+        if (!there) return {kNoKey, kNoKey};
         if (page < 0) return {kNoPage, kNoPage};
         return {(int64_t)((uint64_t)(uint32_t)page * a.k_page + (uint64_t)slot * a.k_slot),
                 (int64_t)((uint64_t)(uint32_t)page * a.v_page + (uint64_t)slot * a.v_slot)};
@@ -254,42 +314,64 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     const auto k_place = [&](int row, int first, int more) { return (row * CH + (first & ~M) + (((first & M) + more) ^ k_turn(row))) * 16; };
     const auto v_place = [&](int row, int first, int more) { return (row * CH + (first & ~M) + (((first & M) + more) ^ v_turn(row))) * 16; };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(TDE_LDS char *)lds;
-    const auto load_tile = [&](const Offsets &where, uint32_t buffer) { // buffer: from the start of lds
-        const int wave_at = SHARED ? wave * LOADS * 1024 : 0;
+    // Keys (VALUES false) or values of a tile, to `to` from the start of lds.  Returns whether exactly LOADS loads were issued.
+    const auto load = [&](int64_t where, uint32_t to, auto values) -> bool {
+        constexpr bool VALUES = decltype(values)::value;
         const int l = in_place(lane), place = l % CH, load_row = (SHARED ? wave * LOADS * AT_ONCE : 0) + l / CH;
-        const bool whole = a.dim == D && __builtin_amdgcn_ballot_w64(where.k >= 0) == (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1);
-        if (whole && a.same_places) {
+        const char *const base = VALUES ? v_base : k_base;
+        const uint32_t at = to + (SHARED ? wave * LOADS * 1024 : 0);
+        const auto chunk_of = [&](int row) { return place ^ (VALUES ? v_turn(row) : k_turn(row)); };
+        if (a.dim == D && __builtin_amdgcn_ballot_w64(where >= 0) == (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1)) {
 #pragma unroll 4
             for (int i = 0; i < LOADS; ++i) {
                 const int row = load_row + i * AT_ONCE;
-                const int64_t key = of_lane(where.k, row);
-                const uint32_t at = lds0 + buffer + wave_at + i * 1024;
-                load_to_lds(k_base + key + (place ^ k_turn(row)) * 16, at);
-                load_to_lds(v_base + key + (place ^ v_turn(row)) * 16, at + TILE);
+                load_to_lds<!SHARED>(base + of_lane(where, row) + chunk_of(row) * 16, lds0 + at + i * 1024);
             }
-            return;
+            return true;
         }
 #pragma unroll 2
         for (int i = 0; i < LOADS; ++i) {
             const int row = load_row + i * AT_ONCE;
-            const int64_t k_at = of_lane(where.k, row), v_at = of_lane(where.v, row);
-            const int k_chunk = place ^ k_turn(row), v_chunk = place ^ v_turn(row);
-            const uint32_t at = buffer + wave_at + i * 1024;
-            if (k_at >= 0) {
-                if (k_chunk * 8 < a.dim) load_to_lds(k_base + k_at + k_chunk * 16, lds0 + at);
-                if (v_chunk * 8 < a.dim) load_to_lds(v_base + v_at + v_chunk * 16, lds0 + at + TILE);
-            } else { // a weight of zero would not keep what lies there from the sums; scores are replaced
-                *(u32x4 *)(lds + at + TILE + l * 16) = u32x4{0, 0, 0, 0};
+            const int64_t key = of_lane(where, row);
+            if (key >= 0) {
+                if (chunk_of(row) * 8 < a.dim) load_to_lds<!SHARED>(base + key + chunk_of(row) * 16, lds0 + at + i * 1024);
+            } else if (VALUES) { // a weight of zero would not keep what lies there from the sums; scores are replaced
+                *(u32x4 *)(lds + at + i * 1024 + l * 16) = u32x4{0, 0, 0, 0};
             }
         }
+        return false;
+    };
+    constexpr std::false_type kKeys{};
+    constexpr std::true_type kValues{};
+    const auto load_both = [&](const Offsets &where, uint32_t to) { // keys and values of a tile
+        if (a.same_places && a.dim == D && __builtin_amdgcn_ballot_w64(where.k >= 0) == (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1)) {
+            const int l = in_place(lane), place = l % CH, load_row = (SHARED ? wave * LOADS * AT_ONCE : 0) + l / CH;
+            const uint32_t at = lds0 + to + (SHARED ? wave * LOADS * 1024 : 0);
+#pragma unroll 4
+            for (int i = 0; i < LOADS; ++i) {
+                const int row = load_row + i * AT_ONCE;
+                const int64_t key = of_lane(where.k, row);
+                load_to_lds<!SHARED>(k_base + key + (place ^ k_turn(row)) * 16, at + i * 1024);
+                load_to_lds<!SHARED>(v_base + key + (place ^ v_turn(row)) * 16, at + TILE + i * 1024);
+            }
+            return;
+        }
+        load(where.k, to, kKeys);
+        load(where.v, to + TILE, kValues);
     };
     uint32_t buf = SHARED ? 0 : wave * 2 * TILE;
     if (a.dim < D) { // channels that the head does not have stay zeros
         for (int i = threadIdx.x * 16; i < 2 * TILE * BUFFERS; i += 64 * WAVES * 16) *(u32x4 *)(lds + i) = u32x4{0, 0, 0, 0};
         __syncthreads();
     }
-    Offsets where = offsets_of(first_key);
-    if (first_key < until) load_tile(where, buf);
+    Offsets where{kNoKey, kNoKey};
+    bool keys_exact = false, values_exact = false; // of the loads that are outstanding
+    if (first_key < until) {
+        look_up(first_key);
+        where = offsets_of(first_key);
+        keys_exact = load(where.k, buf, kKeys);
+        values_exact = load(where.v, buf + TILE, kValues);
+    }
 
     u32x4 q[NB][D / 32];
 #pragma unroll
@@ -322,32 +404,22 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         }
     };
     int64_t next = (int64_t)first_key + TILE_STEP;
-    Offsets where_next = offsets_of(next);
     for (int32_t key0 = first_key; key0 < until;) {
-        wait_for_loads();
-        sync();
+        const bool more = next < until;
         const uint64_t lost = __builtin_amdgcn_ballot_w64(where.k == kNoPage); // keys without a page
-        if (SHARED && next < until) {
-            load_tile(where_next, buf ^ (2 * TILE));
-            where = where_next;
-            where_next = offsets_of(next + TILE_STEP);
-        }
-
-        // whether values that not all rows see hold an infinity or a NaN
-        bool poisoned = false;
-        if (std::min<int64_t>((int64_t)key0 + KT, until) > lowest) {
-            // an exponent of ones plus one at its lowest bit carries out of its field; the field's neighbours are masked off before
-            constexpr uint32_t E = Mfma<T>::kExponent, LOW = E & (~E + 1u);
-            uint32_t carried = 0;
-            const char *const mine = lds + buf + TILE + in_place(SHARED ? (int)threadIdx.x : lane) * 16;
-#pragma unroll 4
-            for (int i = 0; i < TILE; i += 64 * LOADERS * 16) {
-                const u32x4 v = *(const u32x4 *)(mine + i);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) carried |= (v[w] & (E | E << 16)) + (LOW | LOW << 16);
+        if constexpr (SHARED) {
+            wait_for_loads<0>();
+            sync();
+            if (more) {
+                look_up((int32_t)next);
+                where = offsets_of(next);
+                load_both(where, buf ^ (2 * TILE));
             }
-            if constexpr (SHARED) poisoned = __syncthreads_or((carried & 0x80008000u) != 0);
-            else poisoned = __builtin_amdgcn_ballot_w64((carried & 0x80008000u) != 0) != 0;
+        } else {
+            // the keys are there; the values that were issued behind them may come later
+            if (values_exact) wait_for_loads<LOADS>();
+            else wait_for_loads<0>();
+            sync();
         }
 
         __builtin_amdgcn_sched_barrier(0);
@@ -361,21 +433,22 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             const auto read = [&](int unit) {
                 const int kb = unit / (D / 32 / U), st = unit % (D / 32 / U) * U;
 #pragma unroll
-                for (int u = 0; u < U; ++u) kf[unit & 1][u] = *(const u32x4 *)(lds + buf + k_place(kb * 16 + col, (st + u) * 4, quad));
+                for (int u = 0; u < U; ++u) // 16 rows on, turns are the same
+                    kf[unit & 1][u] = *(const u32x4 *)(lds + (buf + k_place(col, (st + u) * 4, quad)) + kb * 16 * CH * 16);
             };
             read(0);
 #pragma unroll
             for (int unit = 0; unit < UNITS; ++unit) {
                 const int kb = unit / (D / 32 / U), st = unit % (D / 32 / U) * U;
                 if (unit + 1 < UNITS) read(unit + 1);
-                __builtin_amdgcn_sched_barrier(0);
+                SB1;
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     if (st == 0) s[n][kb] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int u = 0; u < U; ++u) s[n][kb] = Mfma<T>::mul(kf[unit & 1][u], q[n][st + u], s[n][kb]);
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                SB2;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -398,6 +471,13 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
                     for (int r = 0; r < 4; ++r)
                         if (kb * 16 + r > see) s[n][kb][r] = -__builtin_inff();
             }
+        }
+
+        if (!SHARED && more) { // the keys have been read: the next ones take their place
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            look_up((int32_t)next);
+            where = offsets_of(next);
+            keys_exact = load(where.k, buf, kKeys);
         }
 
         // ---- softmax ----
@@ -447,13 +527,35 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 
         __builtin_amdgcn_sched_barrier(0);
         // ---- values ----
+        if constexpr (!SHARED) {
+            if (more && keys_exact) wait_for_loads<LOADS>();
+            else wait_for_loads<0>();
+            sync();
+        }
+        // whether values that not all rows see hold an infinity or a NaN
+        bool poisoned = false;
+        if (std::min<int64_t>((int64_t)key0 + KT, until) > lowest) {
+            // an exponent of ones plus one at its lowest bit carries out of its field; the field's neighbours are masked off before
+            constexpr uint32_t E = Mfma<T>::kExponent, LOW = E & (~E + 1u);
+            uint32_t carried = 0;
+            const char *const mine = lds + buf + TILE + in_place(SHARED ? (int)threadIdx.x : lane) * 16;
+#pragma unroll 4
+            for (int i = 0; i < TILE; i += 64 * LOADERS * 16) {
+                const u32x4 v = *(const u32x4 *)(mine + i);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) carried |= (v[w] & (E | E << 16)) + (LOW | LOW << 16);
+            }
+            if constexpr (SHARED) poisoned = __syncthreads_or((carried & 0x80008000u) != 0);
+            else poisoned = __builtin_amdgcn_ballot_w64((carried & 0x80008000u) != 0) != 0;
+        }
+
         // 4 keys x 16 channels for each 16 lanes, transposed on the way: a lane gets one channel of the keys 4 * quad ... + 3 and,
         // 16 keys on, of as many again
-        const auto value_operand = [&](const char *tile, int quad, int col, int ks, int d) {
+        const auto value_operand = [&](uint32_t tile, int quad, int col, int ks, int d) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
-            const int row = ks * 32 + quad * 4 + (col >> 2), more = (col & 3) >> 1, within = (col & 1) * 8;
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(tile + v_place(row, d * 2, more) + within));
-            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(tile + v_place(row + 16, d * 2, more) + within));
+            const uint32_t at = tile + v_place(quad * 4 + (col >> 2), d * 2, (col & 3) >> 1) + (col & 1) * 8; // 16 rows on, turns are the same
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(lds + at + ks * 32 * CH * 16));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((TDE_LDS s16x4 *)(lds + at + (ks * 32 + 16) * CH * 16));
             const u32x2 xu = __builtin_bit_cast(u32x2, x), yu = __builtin_bit_cast(u32x2, y);
             return u32x4{xu[0], xu[1], yu[0], yu[1]};
         };
@@ -478,7 +580,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
                     __builtin_amdgcn_sched_barrier(0); // one after the other: interleaved they take too many registers
-                    const u32x4 vf = value_operand(lds + buf + TILE, here_quad, here_col, ks, d);
+                    const u32x4 vf = value_operand(buf + TILE, here_quad, here_col, ks, d);
                     u32x4 mark;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
@@ -525,28 +627,26 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             const auto read = [&](int unit) {
                 const int ks = unit / (D / 16 / U), d = unit % (D / 16 / U) * U;
 #pragma unroll
-                for (int u = 0; u < U; ++u) vf[unit & 1][u] = value_operand(lds + buf + TILE, quad, col, ks, d + u);
+                for (int u = 0; u < U; ++u) vf[unit & 1][u] = value_operand(buf + TILE, quad, col, ks, d + u);
             };
             read(0);
 #pragma unroll
             for (int unit = 0; unit < UNITS; ++unit) {
                 const int ks = unit / (D / 16 / U), d = unit % (D / 16 / U) * U;
                 if (unit + 1 < UNITS) read(unit + 1);
-                __builtin_amdgcn_sched_barrier(0);
+                SB1;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int n = 0; n < NB; ++n) o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], p[n][ks], o[n][d + u]);
-                __builtin_amdgcn_sched_barrier(0);
+                SB2;
             }
         }
 
         if constexpr (SHARED) buf ^= 2 * TILE;
-        else if (next < until) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the tile has been read
-            load_tile(where_next, buf);
-            where = where_next;
-            where_next = offsets_of(next + TILE_STEP);
+        else if (more) { // and so do the next values
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            values_exact = load(where.v, buf + TILE, kValues);
         }
         key0 = (int32_t)std::min<int64_t>(next, 0x7fffffff);
         next += TILE_STEP;
@@ -634,10 +734,13 @@ __global__ void __launch_bounds__(64 * RW * WAVES) attention_join_kernel(const A
     __shared__ float joined[RW * WAVES][D + 4];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t at = blockIdx.x / (ROWS / RW), item = a.kv_heads.quotient(at);
-    const int kv_head = (int)(at - item * a.kv_heads.d);
-    const JoinItem j = a.joins[item];
-    if (j.chunks == 0) return;
+    const uint32_t at = blockIdx.x / (ROWS / RW), tile = a.kv_heads.quotient(at);
+    const int kv_head = (int)(at - tile * a.kv_heads.d);
+    const JoinItem j = a.joins[tile];
+    if (j.chunks <= 0) return;
+    // Where starts do not ascend an entry may never have been written; whatever it holds, what follows stays inside the call's arrays.
+    if (j.item < 0 || j.item >= a.items || j.tile < 0 || j.begin < 0 || j.count < 0 || j.count > a.tokens - j.begin) return;
+    const int32_t item = j.item;
     const int row = (int)(blockIdx.x % (ROWS / RW)) * RW + wave / WAVES;
     const int64_t r = (int64_t)j.tile * ROWS + row;
     const bool there = r < (int64_t)j.count * a.group.d;
@@ -646,7 +749,7 @@ __global__ void __launch_bounds__(64 * RW * WAVES) attention_join_kernel(const A
     float best = -__builtin_inff(), sum[E] = {}, all = 0.0f;
     const int64_t step = (int64_t)a.kv_heads.d * ROWS * (D + 4); // from one item's partial results to the next one's
     const float *const parts = a.partial + (((int64_t)item * a.kv_heads.d + kv_head) * ROWS + row) * (int64_t)(D + 4);
-    // chunks that are items of this call: all of them where starts ascend
+    // of those that are items of this call: all of them where starts ascend
     const int chunks = there ? (int)std::min<int64_t>(j.chunks, a.items - (int64_t)item) : 0;
     for (int c0 = wave % WAVES; c0 < chunks; c0 += WAVES * AHEAD) {
         float pm[AHEAD], pl[AHEAD], x[AHEAD][E];
@@ -720,8 +823,9 @@ void launch_one(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks,
     }
     constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
     attention_kernel<T, D, NB, WAVES, SHARED, true><<<blocks, 64 * WAVES, 0, s>>>(a);
-    if (p.join_waves == 16) attention_join_kernel<T, D, ROWS, 1, 16><<<blocks * ROWS, 1024, 0, s>>>(a);
-    else attention_join_kernel<T, D, ROWS, 4, 1><<<blocks * (ROWS / 4), 256, 0, s>>>(a);
+    const uint32_t joins = (uint32_t)a.tiles * a.kv_heads.d;
+    if (p.join_waves == 16) attention_join_kernel<T, D, ROWS, 1, 16><<<joins * ROWS, 1024, 0, s>>>(a);
+    else attention_join_kernel<T, D, ROWS, 4, 1><<<joins * (ROWS / 4), 256, 0, s>>>(a);
 }
 
 template <class T, int D>
@@ -750,20 +854,28 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
     p->rows = rows_all <= (int64_t)seqs * 16 ? 16 : (p->wide_dim == 256 ? 64 : 128);
     const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence and one behind the last
     const int64_t cus = device_compute_units();
-    p->min_chunk = 256;
+#ifndef TG
+#define TG 4
+#endif
+#ifndef MC
+#define MC 256
+#endif
+    p->min_chunk = MC;
     const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // tiles, rather
-    p->split = likely * kv_heads < (p->rows == 16 ? 4 : 1) * cus && capacity > p->min_chunk;
-    p->target = std::max<int64_t>(1, (p->rows == 16 ? 4 : 2) * cus / kv_heads);
+    p->split = likely * kv_heads < (p->rows == 16 ? TG : 1) * cus && capacity > p->min_chunk;
+    p->target = std::max<int64_t>(1, (p->rows == 16 ? TG : 2) * cus / kv_heads);
+    p->tiles = tiles;
     p->items = tiles + (p->split ? p->target : 0);
-    if (p->items > 0x7fffff00 / kv_heads / p->rows) return TDE_ETOOBIG;
+    if (p->items > 0x7fffff00 / kv_heads || (p->split && tiles > 0x7fffff00 / kv_heads / p->rows)) return TDE_ETOOBIG;
     p->join_waves = p->target / likely >= 32 ? 16 : 1;
     if (p->split)
-        p->workspace_bytes = p->items * (int64_t)sizeof(JoinItem) + p->items * kv_heads * p->rows * (int64_t)(p->wide_dim + 4) * 4;
+        p->workspace_bytes = p->tiles * (int64_t)sizeof(JoinItem) + p->items * kv_heads * p->rows * (int64_t)(p->wide_dim + 4) * 4;
     return TDE_OK;
 }
 
 int launch_attention(AttentionArgs &a, const AttentionPlan &p, int dtype, hipStream_t s) {
     a.items = (int32_t)p.items;
+    a.tiles = (int32_t)p.tiles;
     a.target = p.target;
     a.min_chunk = p.min_chunk;
     a.capacity = (int32_t)std::min<int64_t>((int64_t)a.batch.table_pages * a.batch.page.d, 0x7fffff00);
