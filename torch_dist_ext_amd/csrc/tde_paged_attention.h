@@ -24,6 +24,7 @@ struct AttentionArgs {
     int64_t tokens;
     int64_t target;        // items that the split of the keys aims at, for each key head (split calls)
     int32_t items, tiles;  // at most; grids: items x key heads, and of the second launch tiles x key heads x rows
+    int32_t round;         // items of a key head that have a unit each
     int32_t min_chunk;     // keys of an item at least
     int32_t capacity;      // keys that a row of the page table can name
     int32_t dim;

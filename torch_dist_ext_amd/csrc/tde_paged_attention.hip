@@ -9,7 +9,8 @@
 // An instruction's result has its 16 columns -- the rows -- along the lanes, so a row's maximum, sum and rescaling factor are one value
 // a lane, and a lane's scores of two key blocks are, converted to T, its operand of the second product without any exchange: the
 // product's keys only need the same order on both sides, and V' is read from LDS with transposing loads in just that order.
-// The weights p <= 1 are rounded to T for the second product (its operands are T); l sums them before the rounding.
+// The weights are rounded to T for the second product, whose operands are T, and their sum is that of the rounded ones: one more
+// product, with a row of ones.
 //
 // Where the rows of a call fill few workgroups the keys are split as well (see locate) and a second launch joins the parts.
 #include "tde_paged_attention.h"
@@ -20,25 +21,6 @@
 namespace tde {
 namespace block {
 
-#ifndef PR
-#define PR 0
-#endif
-#if PR == 1
-#define SB1 __builtin_amdgcn_s_setprio(1); __builtin_amdgcn_sched_barrier(0)
-#define SB2 __builtin_amdgcn_sched_barrier(0); __builtin_amdgcn_s_setprio(0)
-#elif PR == 2
-#define SB1 
-#define SB2 __builtin_amdgcn_sched_barrier(0)
-#elif PR == 3
-#define SB1 __builtin_amdgcn_sched_barrier(0)
-#define SB2 
-#elif PR == 4
-#define SB1
-#define SB2
-#else
-#define SB1 __builtin_amdgcn_sched_barrier(0)
-#define SB2 __builtin_amdgcn_sched_barrier(0)
-#endif
 #define TDE_LDS __attribute__((address_space(3)))
 
 namespace {
@@ -61,23 +43,16 @@ struct Mfma<F16> {
     static constexpr uint32_t kExponent = 0x7c00u, kMantissa = 0x03ffu;
 };
 
-// Over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48): swaps of rows of 16 lanes and of halves, of a value
+// Maximum over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48): swaps of rows of 16 lanes and of halves, of a value
 // with itself, leave a pair's two values side by side.
-template <class F>
-__device__ __forceinline__ float over_row(float x, F f) {
-    // (elements of the pair by way of variables: a bit_cast of the second one reads the first)
+// (Elements of a pair by way of variables: a bit_cast of the second one reads the first.)
+__device__ __forceinline__ float max_of_row(float x) {
     const auto rows = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
     const uint32_t r0 = rows[0], r1 = rows[1];
-    x = f(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+    x = __builtin_fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
     const auto halves = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
     const uint32_t h0 = halves[0], h1 = halves[1];
-    return f(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
-}
-__device__ __forceinline__ float max_of_row(float x) {
-    return over_row(x, [](float a, float b) { return __builtin_fmaxf(a, b); });
-}
-__device__ __forceinline__ float sum_of_row(float x) {
-    return over_row(x, [](float a, float b) { return a + b; });
+    return __builtin_fmaxf(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
 }
 
 // What a workgroup works on.  The items of a call: for every sequence its tiles of rows, for every tile its chunks of keys, in that
@@ -164,7 +139,15 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
             it.chunk = local - it.tile * it.chunks;
             it.tile_of_call = tiles_passed + __builtin_amdgcn_readlane(tiles_upto - tiles, at) + it.tile;
             // unsplit, a sequence's last tiles, which see most keys, go first
-            if (!SPLIT) it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - it.tile;
+            if (!SPLIT) {
+                const int32_t all = __builtin_amdgcn_readlane(tiles, at);
+#ifdef SNAKE
+                const int32_t round = it.tile / a.round, first = round * a.round;
+                const int32_t size = all - first < a.round ? all - first : a.round;
+                if (round SNAKE) it.tile = first + size - 1 - (it.tile - first);
+#endif
+                it.tile = all - 1 - it.tile;
+            }
             return it;
         }
         passed += __builtin_amdgcn_readlane(upto, 63);
@@ -193,6 +176,14 @@ template <bool STREAM>
 __device__ __forceinline__ void load_to_lds(const char *p, uint32_t lds) {
     if constexpr (STREAM) asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(p), "s"(lds) : "memory", "m0");
     else asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
+}
+template <bool STREAM>
+__device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t lane_offset, uint32_t lds) {
+    base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base) |
+           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(base >> 32)) << 32;
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    if constexpr (STREAM) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(lane_offset), "s"(base), "s"(lds) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 // Until at most N loads are outstanding.
 template <int N>
@@ -280,6 +271,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     // Lane l holds the table's entry window + l: 64 pages, and a tile needs no more.  Nothing else in the loop is loaded by way of
     // registers: the compiler would wait for it, and with it for every load to LDS that was issued before.
     int32_t window = -64, entries = -1;
+    uint64_t missing = 0; // entries that are no page
     const auto look_up = [&](int32_t key0) { // before offsets_of(key0)
         const uint32_t first = a.batch.page.quotient((uint32_t)key0);
         const uint32_t end = a.batch.page.quotient((uint32_t)std::min<int64_t>((int64_t)key0 + KT, until) - 1);
@@ -287,6 +279,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         window = (int32_t)first;
         entries = page_number(a.batch, table, first + lane);
         asm volatile("" : "+v"(entries)); // waited for here
+        missing = __builtin_amdgcn_ballot_w64(entries < 0);
     };
     // Where key `tile key + lane` lies in the caches, from their heads' first channels on: not there (kNoKey) from `until` on,
     // lost (kNoPage) where the table or the cache has no page for it.
@@ -314,63 +307,68 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     const auto k_place = [&](int row, int first, int more) { return (row * CH + (first & ~M) + (((first & M) + more) ^ k_turn(row))) * 16; };
     const auto v_place = [&](int row, int first, int more) { return (row * CH + (first & ~M) + (((first & M) + more) ^ v_turn(row))) * 16; };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(TDE_LDS char *)lds;
-    // Keys (VALUES false) or values of a tile, to `to` from the start of lds.  Returns whether exactly LOADS loads were issued.
-    const auto load = [&](int64_t where, uint32_t to, auto values) -> bool {
-        constexpr bool VALUES = decltype(values)::value;
-        const int l = in_place(lane), place = l % CH, load_row = (SHARED ? wave * LOADS * AT_ONCE : 0) + l / CH;
-        const char *const base = VALUES ? v_base : k_base;
-        const uint32_t at = to + (SHARED ? wave * LOADS * 1024 : 0);
-        const auto chunk_of = [&](int row) { return place ^ (VALUES ? v_turn(row) : k_turn(row)); };
-        if (a.dim == D && __builtin_amdgcn_ballot_w64(where >= 0) == (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1)) {
+    const int load_row = SHARED ? wave * LOADS * AT_ONCE : 0; // the wavefront's first
+    // The rows of a load lie in one page wherever pages hold whole numbers of them: then a load is a scalar address and an offset of the
+    // lane that never changes but for its turn.
+    const bool whole_pages = a.dim == D && a.batch.page.d % AT_ONCE == 0;
+    const uint32_t k_lane = (uint32_t)(lane / CH) * a.k_slot, v_lane = (uint32_t)(lane / CH) * a.v_slot;
+    const uint32_t k_chunk = (uint32_t)((lane % CH) ^ k_turn(lane / CH)) * 16, v_chunk = (uint32_t)((lane % CH) ^ v_turn(lane / CH)) * 16;
+    // Loads the keys and/or values of a tile (look_up has been called for it) to `to` from the start of lds.  Returns whether exactly
+    // LOADS loads were issued for each; lost: keys without a page.
+    const auto load = [&](int32_t key0, uint32_t to, uint64_t &lost, auto keys, auto values) -> bool {
+        constexpr bool KEYS = decltype(keys)::value, VALUES = decltype(values)::value;
+        const uint32_t at = to + load_row * CH * 16;
+        const uint32_t first = a.batch.page.quotient((uint32_t)key0) - (uint32_t)window;
+        const uint32_t end = a.batch.page.quotient((uint32_t)key0 + KT - 1) - (uint32_t)window;
+        if (whole_pages && until - key0 >= KT && (missing >> first << first << (63 - end)) == 0) {
 #pragma unroll 4
             for (int i = 0; i < LOADS; ++i) {
                 const int row = load_row + i * AT_ONCE;
-                load_to_lds<!SHARED>(base + of_lane(where, row) + chunk_of(row) * 16, lds0 + at + i * 1024);
+                const uint32_t key = (uint32_t)(key0 + row), page = a.batch.page.quotient(key), slot = key - page * a.batch.page.d;
+                const uint32_t number = (uint32_t)__builtin_amdgcn_readlane(entries, (int)(page - (uint32_t)window));
+                if constexpr (KEYS)
+                    load_to_lds<!SHARED>((uint64_t)k_base + (uint64_t)number * a.k_page + (uint64_t)slot * a.k_slot,
+                                         (k_chunk ^ (uint32_t)k_turn(row) * 16) + k_lane, lds0 + at + i * 1024);
+                if constexpr (VALUES)
+                    load_to_lds<!SHARED>((uint64_t)v_base + (uint64_t)number * a.v_page + (uint64_t)slot * a.v_slot,
+                                         (v_chunk ^ (uint32_t)v_turn(row) * 16) + v_lane, lds0 + at + TILE + i * 1024);
             }
+            lost = 0;
             return true;
         }
+        const Offsets where = offsets_of(key0);
+        const int l = in_place(lane);
 #pragma unroll 2
         for (int i = 0; i < LOADS; ++i) {
-            const int row = load_row + i * AT_ONCE;
-            const int64_t key = of_lane(where, row);
-            if (key >= 0) {
-                if (chunk_of(row) * 8 < a.dim) load_to_lds<!SHARED>(base + key + chunk_of(row) * 16, lds0 + at + i * 1024);
+            const int row = load_row + l / CH + i * AT_ONCE;
+            const int64_t k_at = of_lane(where.k, row), v_at = of_lane(where.v, row);
+            const int kc = (l % CH) ^ k_turn(row), vc = (l % CH) ^ v_turn(row);
+            if (k_at >= 0) {
+                if (KEYS && kc * 8 < a.dim) load_to_lds<!SHARED>(k_base + k_at + kc * 16, lds0 + at + i * 1024);
+                if (VALUES && vc * 8 < a.dim) load_to_lds<!SHARED>(v_base + v_at + vc * 16, lds0 + at + TILE + i * 1024);
             } else if (VALUES) { // a weight of zero would not keep what lies there from the sums; scores are replaced
-                *(u32x4 *)(lds + at + i * 1024 + l * 16) = u32x4{0, 0, 0, 0};
+                *(u32x4 *)(lds + at + TILE + i * 1024 + l * 16) = u32x4{0, 0, 0, 0};
             }
         }
+        lost = __builtin_amdgcn_ballot_w64(where.k == kNoPage);
         return false;
     };
-    constexpr std::false_type kKeys{};
-    constexpr std::true_type kValues{};
-    const auto load_both = [&](const Offsets &where, uint32_t to) { // keys and values of a tile
-        if (a.same_places && a.dim == D && __builtin_amdgcn_ballot_w64(where.k >= 0) == (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1)) {
-            const int l = in_place(lane), place = l % CH, load_row = (SHARED ? wave * LOADS * AT_ONCE : 0) + l / CH;
-            const uint32_t at = lds0 + to + (SHARED ? wave * LOADS * 1024 : 0);
-#pragma unroll 4
-            for (int i = 0; i < LOADS; ++i) {
-                const int row = load_row + i * AT_ONCE;
-                const int64_t key = of_lane(where.k, row);
-                load_to_lds<!SHARED>(k_base + key + (place ^ k_turn(row)) * 16, at + i * 1024);
-                load_to_lds<!SHARED>(v_base + key + (place ^ v_turn(row)) * 16, at + TILE + i * 1024);
-            }
-            return;
-        }
-        load(where.k, to, kKeys);
-        load(where.v, to + TILE, kValues);
-    };
+    constexpr std::true_type kYes{};
+    constexpr std::false_type kNo{};
     uint32_t buf = SHARED ? 0 : wave * 2 * TILE;
     if (a.dim < D) { // channels that the head does not have stay zeros
         for (int i = threadIdx.x * 16; i < 2 * TILE * BUFFERS; i += 64 * WAVES * 16) *(u32x4 *)(lds + i) = u32x4{0, 0, 0, 0};
         __syncthreads();
     }
-    Offsets where{kNoKey, kNoKey};
+    uint64_t lost_next = 0;
     bool keys_exact = false, values_exact = false; // of the loads that are outstanding
     if (first_key < until) {
         look_up(first_key);
-        where = offsets_of(first_key);
-        keys_exact = load(where.k, buf, kKeys);
-        values_exact = load(where.v, buf + TILE, kValues);
+        if constexpr (SHARED) load(first_key, buf, lost_next, kYes, kYes);
+        else {
+            keys_exact = load(first_key, buf, lost_next, kYes, kNo);
+            values_exact = load(first_key, buf, lost_next, kNo, kYes);
+        }
     }
 
     u32x4 q[NB][D / 32];
@@ -386,12 +384,12 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             }
         }
 
-    f32x4 o[NB][D / 16];
-    float m[NB], l[NB];
+    f32x4 o[NB][D / 16], l[NB]; // l: sums of weights, each of the four elements the whole row's
+    float m[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         m[n] = -__builtin_inff();
-        l[n] = 0.0f;
+        l[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) o[n][d] = f32x4{0, 0, 0, 0};
     }
@@ -406,14 +404,13 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     int64_t next = (int64_t)first_key + TILE_STEP;
     for (int32_t key0 = first_key; key0 < until;) {
         const bool more = next < until;
-        const uint64_t lost = __builtin_amdgcn_ballot_w64(where.k == kNoPage); // keys without a page
+        const uint64_t lost = lost_next; // keys without a page
         if constexpr (SHARED) {
             wait_for_loads<0>();
             sync();
             if (more) {
                 look_up((int32_t)next);
-                where = offsets_of(next);
-                load_both(where, buf ^ (2 * TILE));
+                load((int32_t)next, buf ^ (2 * TILE), lost_next, kYes, kYes);
             }
         } else {
             // the keys are there; the values that were issued behind them may come later
@@ -441,14 +438,13 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             for (int unit = 0; unit < UNITS; ++unit) {
                 const int kb = unit / (D / 32 / U), st = unit % (D / 32 / U) * U;
                 if (unit + 1 < UNITS) read(unit + 1);
-                SB1;
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     if (st == 0) s[n][kb] = f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int u = 0; u < U; ++u) s[n][kb] = Mfma<T>::mul(kf[unit & 1][u], q[n][st + u], s[n][kb]);
                 }
-                SB2;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -476,8 +472,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         if (!SHARED && more) { // the keys have been read: the next ones take their place
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             look_up((int32_t)next);
-            where = offsets_of(next);
-            keys_exact = load(where.k, buf, kKeys);
+            keys_exact = load((int32_t)next, buf, lost_next, kYes, kNo);
         }
 
         // ---- softmax ----
@@ -510,15 +505,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const float shift = m[n] == -__builtin_inff() ? 0.0f : m[n] * a.scale_log2; // nothing seen yet: every weight is 0
-            float sum = 0.0f;
 #pragma unroll
             for (int kb = 0; kb < KT / 16; ++kb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[n][kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][r], a.scale_log2, -shift));
-                    sum += s[n][kb][r];
-                }
-            l[n] += sum;
+                for (int r = 0; r < 4; ++r) s[n][kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][r], a.scale_log2, -shift));
 #pragma unroll
             for (int ks = 0; ks < KT / 32; ++ks)
                 p[n][ks] = u32x4{T::narrow(s[n][2 * ks][0], s[n][2 * ks][1]), T::narrow(s[n][2 * ks][2], s[n][2 * ks][3]),
@@ -621,6 +611,11 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             }
             sync();
         }
+        const uint32_t ones = T::narrow(1.0f, 1.0f);
+#pragma unroll
+        for (int ks = 0; ks < KT / 32; ++ks)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) l[n] = Mfma<T>::mul(u32x4{ones, ones, ones, ones}, p[n][ks], l[n]);
         {
             constexpr int U = 4, UNITS = KT / 32 * (D / 16 / U);
             u32x4 vf[2][U];
@@ -634,28 +629,24 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             for (int unit = 0; unit < UNITS; ++unit) {
                 const int ks = unit / (D / 16 / U), d = unit % (D / 16 / U) * U;
                 if (unit + 1 < UNITS) read(unit + 1);
-                SB1;
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int n = 0; n < NB; ++n) o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], p[n][ks], o[n][d + u]);
-                SB2;
             }
         }
 
         if constexpr (SHARED) buf ^= 2 * TILE;
         else if (more) { // and so do the next values
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            values_exact = load(where.v, buf + TILE, kValues);
+            values_exact = load((int32_t)next, buf, lost_next, kNo, kYes);
         }
         key0 = (int32_t)std::min<int64_t>(next, 0x7fffffff);
         next += TILE_STEP;
     }
 
-    // ---- what is left: a row's sum over its four lanes, then the row ----
-#pragma unroll
-    for (int n = 0; n < NB; ++n) l[n] = sum_of_row(l[n]);
-
+    // ---- what is left ----
     const int64_t slot = ((int64_t)item_index * a.kv_heads.d + kv_head) * ROWS; // of the partial results
     if constexpr (SHARED) {
 #pragma unroll
@@ -665,9 +656,9 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
                 float *const part = a.partial + (slot + row0 + n * 16 + col) * (D + 4);
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) *(f32x4 *)(part + d * 16 + quad * 4) = o[n][d];
-                if (quad == 0) *(f32x2 *)(part + D) = f32x2{m[n], l[n]};
+                if (quad == 0) *(f32x2 *)(part + D) = f32x2{m[n], l[n][0]};
             } else {
-                const float inverse = 1.0f / l[n];
+                const float inverse = 1.0f / l[n][0];
                 char *const to = a.out + token[n] * a.out_token + head[n] * a.out_head;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
@@ -688,7 +679,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             float *const part = mine + (n * 16 + col) * (D + 4);
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) *(f32x4 *)(part + d * 16 + quad * 4) = o[n][d];
-            if (quad == 0) *(f32x2 *)(part + D) = f32x2{m[n], l[n]};
+            if (quad == 0) *(f32x2 *)(part + D) = f32x2{m[n], l[n][0]};
         }
         __syncthreads();
         // thread -> row and four channels
@@ -854,6 +845,12 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
     p->rows = rows_all <= (int64_t)seqs * 16 ? 16 : (p->wide_dim == 256 ? 64 : 128);
     const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence and one behind the last
     const int64_t cus = device_compute_units();
+#ifndef WS
+#define WS 4
+#endif
+#ifndef WT
+#define WT 2
+#endif
 #ifndef TG
 #define TG 4
 #endif
@@ -862,8 +859,8 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
 #endif
     p->min_chunk = MC;
     const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // tiles, rather
-    p->split = likely * kv_heads < (p->rows == 16 ? TG : 1) * cus && capacity > p->min_chunk;
-    p->target = std::max<int64_t>(1, (p->rows == 16 ? TG : 2) * cus / kv_heads);
+    p->split = likely * kv_heads < (p->rows == 16 ? TG * 4 : WS) * cus / 4 && capacity > p->min_chunk;
+    p->target = std::max<int64_t>(1, (p->rows == 16 ? TG : WT) * cus / kv_heads);
     p->tiles = tiles;
     p->items = tiles + (p->split ? p->target : 0);
     if (p->items > 0x7fffff00 / kv_heads || (p->split && tiles > 0x7fffff00 / kv_heads / p->rows)) return TDE_ETOOBIG;
@@ -876,6 +873,7 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
 int launch_attention(AttentionArgs &a, const AttentionPlan &p, int dtype, hipStream_t s) {
     a.items = (int32_t)p.items;
     a.tiles = (int32_t)p.tiles;
+    a.round = std::max<int32_t>(1, device_compute_units() / (int32_t)a.kv_heads.d);
     a.target = p.target;
     a.min_chunk = p.min_chunk;
     a.capacity = (int32_t)std::min<int64_t>((int64_t)a.batch.table_pages * a.batch.page.d, 0x7fffff00);
