@@ -24,14 +24,12 @@ struct AttentionArgs {
     int64_t tokens;
     int64_t target;        // items that the split of the keys aims at, for each key head (split calls)
     int32_t items, tiles;  // at most; grids: items x key heads, and of the second launch tiles x key heads x rows
-    int32_t round;         // items of a key head that have a unit each
     int32_t min_chunk;     // keys of an item at least
     int32_t capacity;      // keys that a row of the page table can name
     int32_t dim;
     float scale_log2;      // scale * log2(e)
     float *partial;        // [items, kv_heads, rows of a tile, D + 4]: sums, their maximum and weight
     JoinItem *joins;       // [tiles]
-    bool same_places;      // a key's value lies in its cache where the key does in its own
     bool zero_tail;        // rows behind the last sequence become zeros
 };
 

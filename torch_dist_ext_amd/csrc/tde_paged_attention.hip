@@ -139,15 +139,7 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
             it.chunk = local - it.tile * it.chunks;
             it.tile_of_call = tiles_passed + __builtin_amdgcn_readlane(tiles_upto - tiles, at) + it.tile;
             // unsplit, a sequence's last tiles, which see most keys, go first
-            if (!SPLIT) {
-                const int32_t all = __builtin_amdgcn_readlane(tiles, at);
-#ifdef SNAKE
-                const int32_t round = it.tile / a.round, first = round * a.round;
-                const int32_t size = all - first < a.round ? all - first : a.round;
-                if (round SNAKE) it.tile = first + size - 1 - (it.tile - first);
-#endif
-                it.tile = all - 1 - it.tile;
-            }
+            if (!SPLIT) it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - it.tile;
             return it;
         }
         passed += __builtin_amdgcn_readlane(upto, 63);
@@ -823,8 +815,8 @@ template <class T, int D>
 void launch_dim(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks, hipStream_t s) {
     constexpr int ALONE = D == 256 ? 2 : 4; // wavefronts that each hold tiles of their own in LDS
     if (p.rows == 16) launch_one<T, D, 1, ALONE, false>(a, p, blocks, s);
-    else if constexpr (D == 256) launch_one<T, D, 1, 4, true>(a, p, blocks, s);
-    else launch_one<T, D, 2, 4, true>(a, p, blocks, s);
+    else if (p.rows == 64) launch_one<T, D, 1, 4, true>(a, p, blocks, s);
+    else if constexpr (D <= 128) launch_one<T, D, 2, 4, true>(a, p, blocks, s);
 }
 
 template <class T>
@@ -836,35 +828,31 @@ void launch_type(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks
 
 } // namespace
 
-// Which kernel, and whether the keys are split.  capacity: keys that the page table can name for a sequence.
+// Which kernel, and whether the keys are split.  capacity: keys that the page table can name for a sequence.  (Times on 256 units.)
+//
+// Rows of a tile: 16, with every wavefront on keys of its own, where sequences have no more rows than that on average (decode steps:
+// bound by the cache's bytes); 128 where they give three workgroups a unit, else 64: a wavefront then has half the work
+// between two barriers, which is what few workgroups wait for (mixed batch of 576 workgroups of 128 rows 74 us, of 64 rows 62; one
+// chunk of 4096 rows behind 4096, 1024 workgroups, 444 and 630).  Heads of more than 128 channels: 64, for the registers.
+//
+// Keys are split where a launch would not give every unit its workgroups (four of 16 rows each, one else), into about as many
+// items as that and twice as many of the larger tiles, and none of less than 256 keys (one decode row over 131072 keys 24 us).
 int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
     *p = AttentionPlan{};
     p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
-    const int64_t group = q_heads / kv_heads, rows_all = tokens * group;
+    const int64_t group = q_heads / kv_heads, rows_all = tokens * group, cus = device_compute_units();
     if (rows_all > 0x7fffff00) return TDE_ETOOBIG;
-    p->rows = rows_all <= (int64_t)seqs * 16 ? 16 : (p->wide_dim == 256 ? 64 : 128);
+    if (rows_all <= (int64_t)seqs * 16) p->rows = 16;
+    else p->rows = p->wide_dim <= 128 && rows_all / 128 * kv_heads >= 3 * cus ? 128 : 64;
     const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence and one behind the last
-    const int64_t cus = device_compute_units();
-#ifndef WS
-#define WS 4
-#endif
-#ifndef WT
-#define WT 2
-#endif
-#ifndef TG
-#define TG 4
-#endif
-#ifndef MC
-#define MC 256
-#endif
-    p->min_chunk = MC;
-    const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // tiles, rather
-    p->split = likely * kv_heads < (p->rows == 16 ? TG * 4 : WS) * cus / 4 && capacity > p->min_chunk;
-    p->target = std::max<int64_t>(1, (p->rows == 16 ? TG : WT) * cus / kv_heads);
+    const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // rather
+    p->min_chunk = 256;
+    p->split = likely * kv_heads < (p->rows == 16 ? 4 : 1) * cus && capacity > p->min_chunk;
+    p->target = std::max<int64_t>(1, (p->rows == 16 ? 4 : 2) * cus / kv_heads);
     p->tiles = tiles;
     p->items = tiles + (p->split ? p->target : 0);
     if (p->items > 0x7fffff00 / kv_heads || (p->split && tiles > 0x7fffff00 / kv_heads / p->rows)) return TDE_ETOOBIG;
-    p->join_waves = p->target / likely >= 32 ? 16 : 1;
+    p->join_waves = p->target / likely >= 32 ? 16 : 1; // of a row: where it may have many parts
     if (p->split)
         p->workspace_bytes = p->tiles * (int64_t)sizeof(JoinItem) + p->items * kv_heads * p->rows * (int64_t)(p->wide_dim + 4) * 4;
     return TDE_OK;
@@ -873,11 +861,9 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
 int launch_attention(AttentionArgs &a, const AttentionPlan &p, int dtype, hipStream_t s) {
     a.items = (int32_t)p.items;
     a.tiles = (int32_t)p.tiles;
-    a.round = std::max<int32_t>(1, device_compute_units() / (int32_t)a.kv_heads.d);
     a.target = p.target;
     a.min_chunk = p.min_chunk;
     a.capacity = (int32_t)std::min<int64_t>((int64_t)a.batch.table_pages * a.batch.page.d, 0x7fffff00);
-    a.same_places = a.k_page == a.v_page && a.k_slot == a.v_slot;
     // the joins' items behind the partial results, which want 16-byte boundaries
     a.joins = reinterpret_cast<JoinItem *>(a.partial + p.items * a.kv_heads.d * p.rows * (p.wide_dim + 4));
     const uint32_t blocks = (uint32_t)(p.items * a.kv_heads.d);
