@@ -63,14 +63,16 @@ template <int BYTES>
 struct Words {
     uint32_t w[BYTES / 4];
 };
-template <int BYTES>
+// STREAM: passed by the caches, for what is read or written once.
+template <int BYTES, bool STREAM = false>
 __device__ __forceinline__ Words<BYTES> load_words(const void *p) {
     Words<BYTES> r;
     if constexpr (BYTES % 16 == 0) {
         typedef u32x4 __attribute__((aligned(2))) loose;
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
-            const u32x4 v = ((const __attribute__((address_space(1))) loose *)p)[i];
+            const auto *const from = (const __attribute__((address_space(1))) loose *)p + i;
+            const u32x4 v = STREAM ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
             for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
         }
@@ -86,13 +88,17 @@ __device__ __forceinline__ Words<BYTES> load_words(const void *p) {
     }
     return r;
 }
-template <int BYTES>
+template <int BYTES, bool STREAM = false>
 __device__ __forceinline__ void store_words(void *p, const Words<BYTES> &r) {
     if constexpr (BYTES % 16 == 0) {
         typedef u32x4 __attribute__((aligned(2))) loose;
 #pragma unroll
-        for (int i = 0; i < BYTES / 16; ++i)
-            ((__attribute__((address_space(1))) loose *)p)[i] = u32x4{r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
+        for (int i = 0; i < BYTES / 16; ++i) {
+            auto *const to = (__attribute__((address_space(1))) loose *)p + i;
+            const loose v = u32x4{r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]};
+            if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+            else *to = v;
+        }
     } else if constexpr (BYTES == 8) {
         typedef u32x2 __attribute__((aligned(2))) loose;
         *(__attribute__((address_space(1))) loose *)p = u32x2{r.w[0], r.w[1]};

@@ -5,9 +5,8 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin)      for the rotated channels' pairs: (d, d + rot/2), or (2d, 2d + 1) if interleaved
 //   T(.)                                          one rounding, at the end; the sum of squares is held in fp32
 //
-// Bound by memory: every row is read and written once.  A row's chunks of 16 bytes (8 where the head's length or the rotation's
-// halves need it) lie in neighbouring lanes, so several rows share a wavefront and the partner of a chunk in the other half
-// of the rotation is a lane of the same wavefront.  All rows of a wavefront belong to one token: its position, its row of the
+// Bound by memory: every row is read and written once.  A lane has two chunks of 16 bytes of a row (8 where the head's length or the
+// rotation's halves need it), so several rows share a wavefront.  All rows of a wavefront belong to one token: its position, its row of the
 // rotation's table and its page are looked up once, with scalar or shared loads, while the rows are on their way.
 #include "tde_block.h"
 #include "tde_head_rows.h"
@@ -49,7 +48,22 @@ __device__ __forceinline__ char *destination(const HeadRowsArgs &a, const Place 
     return a.out[cls] + place.page * a.out_page[cls] + place.slot * a.out_token[cls] + h * a.out_head[cls];
 }
 
-template <class T, int VE, int R, bool INTERLEAVED, bool PAGED>
+// VE floats of the table; NaN where the position is not in it.
+template <int N>
+__device__ __forceinline__ void load_floats(const float *p, bool known, float (&x)[N]) {
+    Words<N * 4> w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w.w[i] = 0x7fc00000u;
+    if (known) w = load_words<N * 4>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __builtin_bit_cast(float, w.w[i]);
+}
+
+// A lane has two chunks of VE channels of a row: chunk p and its partner in the other half of the rotation, or, behind the rotated
+// channels and with interleaved pairs, one in each half of what there is (neighbouring lanes then load neighbouring chunks; with two
+// neighbours a lane, a chunk of 8192 rows took 53 us in place of 40).  Rotating needs no other lane, and R rows of a token share
+// the lane's cosines, sines and gammas.
+template <class T, int VE, int R, bool INTERLEAVED, bool PAGED, bool STREAM>
 __global__ void __launch_bounds__(256) head_rows_kernel(const HeadRowsArgs a) {
     constexpr int BYTES = VE * T::kBytes;
     const int lane = threadIdx.x & 63;
@@ -59,107 +73,147 @@ __global__ void __launch_bounds__(256) head_rows_kernel(const HeadRowsArgs a) {
     if (token >= a.tokens) return;
     const int part = (int)(wave - row * a.waves_per_token.d);
     const int rows_at_once = 64 >> a.lanes_log2;
-    const int chunk = lane & ((1 << a.lanes_log2) - 1);
-    const int d0 = chunk * VE;
-    const bool active = d0 < a.dim;
+    const int place = lane & ((1 << a.lanes_log2) - 1);
+    const int pairs = a.half / VE; // lanes with a partner in the other half
+    const int chunks = a.dim / VE;
+    const int rest = INTERLEAVED ? 0 : 2 * pairs; // first of the chunks without a partner, in halves of `apart`
+    const int apart = (chunks - rest + 1) / 2;
+    int c0 = place, c1 = place + pairs;
+    if (INTERLEAVED || place >= pairs) {
+        const int u = place - (INTERLEAVED ? 0 : pairs);
+        c0 = u < apart ? rest + u : chunks;
+        c1 = u < apart ? rest + u + apart : chunks;
+    }
+    const bool has0 = c0 < chunks, has1 = c1 < chunks;
+    const int at0 = c0 * BYTES, at1 = c1 * BYTES;
     const int heads = a.heads[0] + a.heads[1] + a.heads[2];
 
-    Words<BYTES> raw[R];
+    Words<BYTES> raw[R][2];
     int cls[R], head[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         int h = (part * R + r) * rows_at_once + (lane >> a.lanes_log2);
-        const bool there = active && h < heads;
+        const bool there = h < heads;
         cls[r] = h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2);
         h -= cls[r] == 0 ? 0 : (cls[r] == 1 ? a.heads[0] : a.heads[0] + a.heads[1]);
         head[r] = there ? h : -1;
         const char *src = cls[r] == 0 ? a.in[0] : (cls[r] == 1 ? a.in[1] : a.in[2]);
         const int64_t per_token = cls[r] == 0 ? a.in_token[0] : (cls[r] == 1 ? a.in_token[1] : a.in_token[2]);
         const int64_t per_head = cls[r] == 0 ? a.in_head[0] : (cls[r] == 1 ? a.in_head[1] : a.in_head[2]);
-        if (there) raw[r] = load_words<BYTES>(src + token * per_token + h * per_head + d0 * T::kBytes);
-        else raw[r] = Words<BYTES>{};
+        src += token * per_token + h * per_head;
+        raw[r][0] = raw[r][1] = Words<BYTES>{};
+        if (there && has0) raw[r][0] = load_words<BYTES, STREAM>(src + at0);
+        if (there && has1) raw[r][1] = load_words<BYTES, STREAM>(src + at1);
     }
 
-    Place place{0, -1, 0};
-    if (PAGED) place = place_of(a.batch, token, lane);
-    const bool placed = !PAGED || place.position >= 0;
-    const int64_t position = a.positions != nullptr ? explicit_position(a, token) : place.position;
+    Place where{0, -1, 0};
+    if (PAGED) where = place_of(a.batch, token, lane);
+    const bool placed = !PAGED || where.position >= 0;
+    const int64_t position = a.positions != nullptr ? explicit_position(a, token) : where.position;
 
-    // cosines and sines of this lane's chunk; outside the table they are NaN, and so become the rotated channels
+    // Cosines and sines of the lane's pairs.  Interleaved: the first half of them belongs to the first chunk.
     const int rot = 2 * a.half;
-    const bool turned = active && d0 < rot;
+    const bool turned0 = c0 * VE < rot, turned1 = has1 && c1 * VE < rot;
     float cs[VE], sn[VE];
     {
         const bool known = position >= 0 && position < a.table_rows;
-        const float *row_of = a.cos_sin + (known ? position : 0) * a.table_stride;
-        constexpr int N = INTERLEAVED ? VE / 2 : VE;
-        const int j = INTERLEAVED ? d0 / 2 : (d0 < a.half ? d0 : d0 - a.half);
+        const float *const row_of = a.cos_sin + (known ? position : 0) * a.table_stride;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            cs[i] = 1.0f;
-            sn[i] = 0.0f;
-        }
-        if (turned) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                cs[i] = known ? row_of[j + i] : __builtin_nanf("");
-                sn[i] = known ? row_of[a.half + j + i] : __builtin_nanf("");
+        for (int i = 0; i < VE; ++i) cs[i] = sn[i] = 0.0f;
+        if constexpr (!INTERLEAVED) {
+            if (turned0) {
+                load_floats(row_of + place * VE, known, cs);
+                load_floats(row_of + a.half + place * VE, known, sn);
             }
+        } else {
+            constexpr int N = VE / 2;
+            const auto load_half = [&](int chunk, int from) {
+                float c[N], s[N];
+                load_floats(row_of + chunk * N, known, c);
+                load_floats(row_of + a.half + chunk * N, known, s);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    cs[from + i] = c[i];
+                    sn[from + i] = s[i];
+                }
+            };
+            if (turned0) load_half(c0, 0);
+            if (turned1) load_half(c1, N);
         }
     }
-    float gamma_q[VE], gamma_k[VE];
-    {
-        Words<BYTES> g{};
-        if (active && a.gamma[0] != nullptr) g = load_words<BYTES>(a.gamma[0] + d0 * T::kBytes);
-        widen_all<T, VE>(g, gamma_q);
-        if (active && a.gamma[1] != nullptr) g = load_words<BYTES>(a.gamma[1] + d0 * T::kBytes);
-        widen_all<T, VE>(g, gamma_k);
+    Words<BYTES> gamma[2][2]{}; // of queries and keys
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        if (a.gamma[g] != nullptr && has0) gamma[g][0] = load_words<BYTES>(a.gamma[g] + at0);
+        if (a.gamma[g] != nullptr && has1) gamma[g][1] = load_words<BYTES>(a.gamma[g] + at1);
     }
 
-    // the lane of the partner chunk
-    const int partner = INTERLEAVED || !turned ? lane : (d0 < a.half ? lane + a.half / VE : lane - a.half / VE);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        float x[VE];
-        widen_all<T, VE>(raw[r], x);
-        const bool normed = cls[r] == 0 ? a.gamma[0] != nullptr : (cls[r] == 1 && a.gamma[1] != nullptr);
+        float x0[VE], x1[VE];
+        widen_all<T, VE>(raw[r][0], x0);
+        widen_all<T, VE>(raw[r][1], x1);
         if (a.gamma[0] != nullptr || a.gamma[1] != nullptr) {
             float sq = 0.0f;
 #pragma unroll
-            for (int i = 0; i < VE; ++i) sq = __builtin_fmaf(x[i], x[i], sq);
+            for (int i = 0; i < VE; ++i) sq = __builtin_fmaf(x0[i], x0[i], sq);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) sq = __builtin_fmaf(x1[i], x1[i], sq);
             sq = sum_over_lanes(sq, a.lanes_log2);
             const float scale = 1.0f / __builtin_sqrtf(sq / (float)a.dim + a.eps);
+            const bool normed = cls[r] == 0 ? a.gamma[0] != nullptr : (cls[r] == 1 && a.gamma[1] != nullptr);
+            float g0[VE], g1[VE];
+            {
+                Words<BYTES> w0, w1;
 #pragma unroll
-            for (int i = 0; i < VE; ++i) x[i] = normed ? x[i] * scale * (cls[r] == 0 ? gamma_q[i] : gamma_k[i]) : x[i];
-        }
-        if (rot != 0) {
-            float y[VE];
-            if constexpr (INTERLEAVED) {
-#pragma unroll
-                for (int i = 0; i < VE / 2; ++i) {
-                    y[2 * i] = __builtin_fmaf(x[2 * i], cs[i], -(x[2 * i + 1] * sn[i]));
-                    y[2 * i + 1] = __builtin_fmaf(x[2 * i + 1], cs[i], x[2 * i] * sn[i]);
+                for (int i = 0; i < BYTES / 4; ++i) {
+                    w0.w[i] = cls[r] == 0 ? gamma[0][0].w[i] : gamma[1][0].w[i];
+                    w1.w[i] = cls[r] == 0 ? gamma[0][1].w[i] : gamma[1][1].w[i];
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const float other = __shfl(x[i], partner);
-                    const float s = other * sn[i];
-                    y[i] = __builtin_fmaf(x[i], cs[i], d0 < a.half ? -s : s);
-                }
+                widen_all<T, VE>(w0, g0);
+                widen_all<T, VE>(w1, g1);
             }
 #pragma unroll
-            for (int i = 0; i < VE; ++i) x[i] = turned ? y[i] : x[i];
+            for (int i = 0; i < VE; ++i) {
+                x0[i] = normed ? x0[i] * scale * g0[i] : x0[i];
+                x1[i] = normed ? x1[i] * scale * g1[i] : x1[i];
+            }
+        }
+        if constexpr (!INTERLEAVED) {
+            if (turned0) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    const float u = x0[i], v = x1[i];
+                    x0[i] = __builtin_fmaf(u, cs[i], -(v * sn[i]));
+                    x1[i] = __builtin_fmaf(v, cs[i], u * sn[i]);
+                }
+            }
+        } else {
+            const auto turn = [&](float (&x)[VE], int from) {
+#pragma unroll
+                for (int i = 0; i < VE / 2; ++i) {
+                    const float u = x[2 * i], v = x[2 * i + 1], c = cs[from + i], s = sn[from + i];
+                    x[2 * i] = __builtin_fmaf(u, c, -(v * s));
+                    x[2 * i + 1] = __builtin_fmaf(v, c, u * s);
+                }
+            };
+            if (turned0) turn(x0, 0);
+            if (turned1) turn(x1, VE / 2);
         }
         if (head[r] < 0) continue;
-        Words<BYTES> out = narrow_all<T, VE>(x);
-        if (cls[r] == 2) out = raw[r]; // values go as they are
+        Words<BYTES> y0 = narrow_all<T, VE>(x0), y1 = narrow_all<T, VE>(x1);
+        if (cls[r] == 2) { // values go as they are
+            y0 = raw[r][0];
+            y1 = raw[r][1];
+        }
         if (!placed) {
             if (cls[r] != 0) continue;
-            out = Words<BYTES>{};
+            y0 = y1 = Words<BYTES>{};
         }
-        char *to = destination<PAGED>(a, place, token, cls[r], head[r]);
-        if (to != nullptr) store_words<BYTES>(to + d0 * T::kBytes, out);
+        char *to = destination<PAGED>(a, where, token, cls[r], head[r]);
+        if (to == nullptr) continue;
+        if (has0) store_words<BYTES, STREAM>(to + at0, y0);
+        if (has1) store_words<BYTES, STREAM>(to + at1, y1);
     }
 }
 
@@ -218,14 +272,14 @@ __global__ void __launch_bounds__(256) head_elements_kernel(const HeadRowsArgs a
 
 namespace {
 
-template <class T, int VE, int R>
+template <class T, int VE, int R, bool STREAM>
 void launch_rows(const HeadRowsArgs &a, uint32_t blocks, hipStream_t s) {
     if (a.paged) {
-        if (a.interleaved) head_rows_kernel<T, VE, R, true, true><<<blocks, 256, 0, s>>>(a);
-        else head_rows_kernel<T, VE, R, false, true><<<blocks, 256, 0, s>>>(a);
+        if (a.interleaved) head_rows_kernel<T, VE, R, true, true, STREAM><<<blocks, 256, 0, s>>>(a);
+        else head_rows_kernel<T, VE, R, false, true, STREAM><<<blocks, 256, 0, s>>>(a);
     } else {
-        if (a.interleaved) head_rows_kernel<T, VE, R, true, false><<<blocks, 256, 0, s>>>(a);
-        else head_rows_kernel<T, VE, R, false, false><<<blocks, 256, 0, s>>>(a);
+        if (a.interleaved) head_rows_kernel<T, VE, R, true, false, STREAM><<<blocks, 256, 0, s>>>(a);
+        else head_rows_kernel<T, VE, R, false, false, STREAM><<<blocks, 256, 0, s>>>(a);
     }
 }
 
@@ -244,11 +298,14 @@ template <class T>
 int launch_typed(HeadRowsArgs &a, const HeadRowsPlan &plan, hipStream_t s) {
     constexpr int V = 16 / T::kBytes;
     if (plan.chunk_bytes == 16) {
-        if (plan.rows == 4) launch_rows<T, V, 4>(a, plan.blocks, s);
-        else launch_rows<T, V, 1>(a, plan.blocks, s);
+        switch (plan.rows) {
+        case 1: launch_rows<T, V, 1, false>(a, plan.blocks, s); break;
+        case 2: launch_rows<T, V, 2, true>(a, plan.blocks, s); break;
+        case 3: launch_rows<T, V, 3, true>(a, plan.blocks, s); break;
+        default: launch_rows<T, V, 5, true>(a, plan.blocks, s); break;
+        }
     } else if (plan.chunk_bytes == 8) {
-        if (plan.rows == 4) launch_rows<T, V / 2, 4>(a, plan.blocks, s);
-        else launch_rows<T, V / 2, 1>(a, plan.blocks, s);
+        launch_rows<T, V / 2, 1, false>(a, plan.blocks, s);
     } else {
         launch_elements<T>(a, plan.blocks, s);
     }
@@ -263,7 +320,7 @@ int plan_head_rows(int elem, int dim, int half, bool interleaved, int64_t tokens
     p->chunk_bytes = 0;
     for (int bytes = 16; bytes >= 8; bytes /= 2) {
         const int ve = bytes / elem;
-        if (dim % ve == 0 && (interleaved ? 2 * half : half) % ve == 0 && dim / ve <= 64) {
+        if (dim % ve == 0 && (interleaved ? 2 * half : half) % ve == 0 && (dim / ve + 1) / 2 <= 64) {
             p->chunk_bytes = bytes;
             break;
         }
@@ -272,13 +329,24 @@ int plan_head_rows(int elem, int dim, int half, bool interleaved, int64_t tokens
     p->lanes_log2 = 6;
     p->rows = 1;
     if (p->chunk_bytes != 0) {
-        const int lanes = dim * elem / p->chunk_bytes;
+        const int lanes = (dim * elem / p->chunk_bytes + 1) / 2;
         p->lanes_log2 = 0;
         while ((1 << p->lanes_log2) < lanes) ++p->lanes_log2;
-        const int at_once = 64 >> p->lanes_log2;
-        const int64_t waves4 = (heads_all + 4 * at_once - 1) / (4 * at_once);
-        p->rows = tokens * waves4 >= 4096 ? 4 : 1;
-        waves = p->rows == 4 ? waves4 : (heads_all + at_once - 1) / at_once;
+        const int64_t at_once = 64 >> p->lanes_log2;
+        const auto waves_of = [&](int rows) { return (heads_all + rows * at_once - 1) / (rows * at_once); };
+        // Rows that share a lane's cosines and sines: as many as make the fewest wavefronts' work, counting those loads as two rows,
+        // once there is work for every unit at least four times over; before that one, and more wavefronts.
+        if (p->chunk_bytes == 16 && tokens * waves_of(5) >= 4096) {
+            int64_t best = 0;
+            for (int rows : {2, 3, 5}) {
+                const int64_t cost = waves_of(rows) * (rows + 2);
+                if (best == 0 || cost < best) {
+                    best = cost;
+                    p->rows = rows;
+                }
+            }
+        }
+        waves = waves_of(p->rows);
     }
     p->waves_per_token = (uint32_t)waves;
     if (waves != 0 && tokens > (int64_t)0x7ffffff0 / waves) return TDE_ETOOBIG;
