@@ -196,11 +196,19 @@ __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_tile_kernel
 // 16 bytes a lane from a buffer to LDS: lane l's go to lds + 16 * l.  Written in assembly because the compiler, which cannot tell one
 // stage of a tile from the next, waits for every such load before any read from LDS; it returns nothing in registers.  It counts
 // like any load, so a wait that the compiler places only becomes longer.  wait_for_stage() is the wait that the data needs.
+// STREAM: read once, not to be kept in the caches.
+template <bool STREAM = false>
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t lane_offset, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-                 :
-                 : "v"(lane_offset), "s"(rsrc), "s"(offset), "s"(lds)
-                 : "memory", "m0");
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen nt lds"
+                     :
+                     : "v"(lane_offset), "s"(rsrc), "s"(offset), "s"(lds)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                     :
+                     : "v"(lane_offset), "s"(rsrc), "s"(offset), "s"(lds)
+                     : "memory", "m0");
 }
 // Until at most N loads are outstanding.
 template <int N>
@@ -331,13 +339,15 @@ __global__ void __launch_bounds__((BT / WT) * (BN / WN) * 64) linear_staged_kern
 
 // ---- few tokens: bound by the weight's bytes ----
 
+template <bool STREAM>
 __device__ __forceinline__ u32x4 load16_inside(const int8_t *p) {
     typedef u32x4 __attribute__((aligned(1))) loose;
-    return *(const __attribute__((address_space(1))) loose *)p;
+    const auto *const from = (const __attribute__((address_space(1))) loose *)p;
+    return STREAM ? __builtin_nontemporal_load(from) : *from;
 }
 
 // Up to M tokens by dot products of four bytes: a wavefront has R channels and goes along their rows, 1 KiB of each at a time.
-template <class T, int M, int R, int AHEAD>
+template <class T, int M, int R, int AHEAD, bool STREAM>
 __global__ void __launch_bounds__(256) linear_dot_kernel(const LinearArgs a) {
     const int lane = threadIdx.x & 63;
     const int64_t n0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * R;
@@ -365,9 +375,9 @@ __global__ void __launch_bounds__(256) linear_dot_kernel(const LinearArgs a) {
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) wv[h][r] = load16_inside(w[r] + k + h * 1024 + lane * 16);
+            for (int r = 0; r < R; ++r) wv[h][r] = load16_inside<STREAM>(w[r] + k + h * 1024 + lane * 16);
 #pragma unroll
-            for (int m = 0; m < M; ++m) cv[h][m] = load16_inside(c[m] + k + h * 1024 + lane * 16);
+            for (int m = 0; m < M; ++m) cv[h][m] = load16_inside<false>(c[m] + k + h * 1024 + lane * 16);
         }
 #pragma unroll
         for (int h = 0; h < AHEAD; ++h) add(wv[h], cv[h]);
@@ -403,7 +413,7 @@ __global__ void __launch_bounds__(256) linear_dot_kernel(const LinearArgs a) {
 
 // MB x 16 tokens and NB x 16 channels a workgroup; its wavefronts take pieces of 128 bytes of the rows in turn, each through LDS of its
 // own (STAGES pieces, no barrier), and are added up at the end.
-template <class T, int MB, int NB, int WAVES, int STAGES>
+template <class T, int MB, int NB, int WAVES, int STAGES, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES) linear_pieces_kernel(const LinearArgs a, int32_t token_tiles) {
     constexpr int TOKENS = 16 * MB, CHANNELS = 16 * NB, KB = 128;
     constexpr int LOADS = 2 * (MB + NB), STAGE = (TOKENS + CHANNELS) * KB, RING = STAGES * STAGE;
@@ -439,7 +449,7 @@ __global__ void __launch_bounds__(64 * WAVES) linear_pieces_kernel(const LinearA
         for (int i = 0; i < 2 * MB; ++i) load_to_lds(codes, at + i * step + (i & 1 ? chunk_odd : chunk_even), 0, lds0 + stage * STAGE + i * 1024);
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i)
-            load_to_lds(weight, at + i * step + (i & 1 ? chunk_odd : chunk_even), 0, lds0 + stage * STAGE + TOKENS * KB + i * 1024);
+            load_to_lds<STREAM>(weight, at + i * step + (i & 1 ? chunk_odd : chunk_even), 0, lds0 + stage * STAGE + TOKENS * KB + i * 1024);
     };
     i32x4 acc[NB][MB];
 #pragma unroll
@@ -505,10 +515,103 @@ __global__ void __launch_bounds__(64 * WAVES) linear_pieces_kernel(const LinearA
     }
 }
 
+// The same for rows that begin anywhere: operands come straight from memory to registers (a lane's 16 bytes are its part of an
+// instruction's operand), which takes loads of 16 bytes from 16 rows at once.  Bound by those loads, which the hardware splits where
+// they do not begin on words: 10 x 5121 x 7168 takes 32 us, 32 tokens 56 (tiles by way of registers and LDS: 62 either way, and 100 x
+// 5121 x 4096 61 against 91); rows of whole words take 9 and 11.
+template <class T, int MB, int NB, int WAVES, int AHEAD>
+__global__ void __launch_bounds__(64 * WAVES) linear_loose_kernel(const LinearArgs a, int32_t token_tiles) {
+    constexpr int TOKENS = 16 * MB, CHANNELS = 16 * NB;
+    __shared__ __align__(16) int32_t part[WAVES][TOKENS][CHANNELS + 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const int64_t t0 = (int64_t)(blockIdx.x % token_tiles) * TOKENS, n0 = (int64_t)(blockIdx.x / token_tiles) * CHANNELS;
+    const int8_t *c[MB], *w[NB];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+        const int64_t t = t0 + m * 16 + col;
+        c[m] = a.codes + (t < a.tokens ? t : a.tokens - 1) * a.k;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int64_t at = n0 + n * 16 + col;
+        w[n] = a.weight + (at < a.n ? at : a.n - 1) * a.k;
+    }
+    i32x4 acc[NB][MB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[n][m] = i32x4{0, 0, 0, 0};
+    const auto multiply = [&](const u32x4 (&wv)[2][NB], const u32x4 (&cv)[2][MB]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int m = 0; m < MB; ++m)
+                    acc[n][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wv[h][n]), __builtin_bit_cast(i32x4, cv[h][m]), acc[n][m], 0, 0, 0);
+    };
+    int64_t k = (int64_t)wave * AHEAD * 128;
+    for (; k + AHEAD * 128 <= a.k; k += WAVES * AHEAD * 128) {
+        u32x4 wv[AHEAD][2][NB], cv[AHEAD][2][MB];
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) wv[x][h][n] = load16_inside<false>(w[n] + k + x * 128 + h * 64 + quad * 16);
+#pragma unroll
+                for (int m = 0; m < MB; ++m) cv[x][h][m] = load16_inside<false>(c[m] + k + x * 128 + h * 64 + quad * 16);
+            }
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) multiply(wv[x], cv[x]);
+    }
+    for (int x = 0; x < AHEAD && k < a.k; ++x, k += 128) { // the last piece of all, in one wavefront
+        u32x4 wv[2][NB], cv[2][MB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) wv[h][n] = load16(w[n], 0, 1, k + h * 64 + quad * 16, a.k);
+#pragma unroll
+            for (int m = 0; m < MB; ++m) cv[h][m] = load16(c[m], 0, 1, k + h * 64 + quad * 16, a.k);
+        }
+        multiply(wv, cv);
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) *(i32x4 *)&part[wave][m * 16 + col][n * 16 + quad * 4] = acc[n][m];
+    __syncthreads();
+    for (int at = threadIdx.x; at < TOKENS * CHANNELS / 4; at += 64 * WAVES) {
+        const int64_t t = t0 + at / (CHANNELS / 4), n = n0 + at % (CHANNELS / 4) * 4;
+        if (t >= a.tokens || n >= a.n) continue;
+        i32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) sum += *(const i32x4 *)&part[v][at / (CHANNELS / 4)][at % (CHANNELS / 4) * 4];
+        const int count = (int)(a.n - n < 4 ? a.n - n : 4);
+        const float s = a.scales[t];
+        float y[4] = {};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < count) {
+                y[r] = (float)sum[r] * (s * a.weight_scales[n + r]);
+                if (a.bias != nullptr) y[r] += a.bias[n + r];
+            }
+        store4<T>(a.out + (t * a.n + n) * T::kBytes, y, count, count == 4);
+    }
+}
+
+// Weights from 32 MB on pass by the caches: they would push out what fits there, and come faster (one token x 8192 x 8192 12.0 us, by way
+// of the caches 13.7).  A smaller one may still be there from the last call (one token x 8192 x 1280 3.7 us, streamed 4.1).
+bool streams(const LinearArgs &a) { return a.n * a.k >= (int64_t)32 << 20; }
+
 template <class T, int M>
 void launch_dot(const LinearArgs &a, hipStream_t s) {
-    if (a.n >= 8192) linear_dot_kernel<T, M, 4, 2><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
-    else linear_dot_kernel<T, M, 1, 4><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
+    // four channels a wavefront share the codes' loads; one where that leaves few wavefronts
+    if (a.n >= 8192 && streams(a)) linear_dot_kernel<T, M, 4, 2, true><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
+    else if (a.n >= 8192) linear_dot_kernel<T, M, 4, 2, false><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
+    else if (streams(a)) linear_dot_kernel<T, M, 1, 4, true><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
+    else linear_dot_kernel<T, M, 1, 4, false><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
 }
 
 template <class T, int BT, int BN, int WT, int WN, int STAGES>
@@ -524,7 +627,17 @@ template <class T, int MB, int NB, int WAVES, int STAGES>
 int launch_pieces(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + 16 * MB - 1) / (16 * MB), blocks = token_tiles * ((a.n + 16 * NB - 1) / (16 * NB));
     if (blocks > 0x7fffffff) return TDE_ETOOBIG;
-    linear_pieces_kernel<T, MB, NB, WAVES, STAGES><<<(uint32_t)blocks, 64 * WAVES, 0, s>>>(a, (int32_t)token_tiles);
+    if (streams(a) && token_tiles == 1)
+        linear_pieces_kernel<T, MB, NB, WAVES, STAGES, true><<<(uint32_t)blocks, 64 * WAVES, 0, s>>>(a, (int32_t)token_tiles);
+    else linear_pieces_kernel<T, MB, NB, WAVES, STAGES, false><<<(uint32_t)blocks, 64 * WAVES, 0, s>>>(a, (int32_t)token_tiles);
+    return TDE_OK;
+}
+
+template <class T, int MB>
+int launch_loose(const LinearArgs &a, hipStream_t s) {
+    const int64_t token_tiles = (a.tokens + 16 * MB - 1) / (16 * MB), blocks = token_tiles * ((a.n + 15) / 16);
+    if (blocks > 0x7fffffff) return TDE_ETOOBIG;
+    linear_loose_kernel<T, MB, 1, 8, 2><<<(uint32_t)blocks, 512, 0, s>>>(a, (int32_t)token_tiles);
     return TDE_OK;
 }
 
@@ -587,6 +700,8 @@ int launch_typed(const LinearArgs &a, hipStream_t s) {
         case k64x64: st = launch_staged<T, 64, 64, 32, 32, 4>(a, s); break;
         case kPieces: st = launch_pieces<T, 4, 2, 8, 1>(a, s); break;
         }
+    } else if (a.tokens <= 32) {
+        st = a.tokens <= 16 ? launch_loose<T, 1>(a, s) : launch_loose<T, 2>(a, s);
     } else {
         const int64_t token_tiles = (a.tokens + 127) / 128, blocks = token_tiles * ((a.n + 127) / 128);
         if (blocks > 0x7fffffff) return TDE_ETOOBIG;
