@@ -168,3 +168,49 @@ def attention(batch, q, k_cache, v_cache, scale):
             bound[t, kv * group:(kv + 1) * group] = (size * (h + rel) * 1.02 + o.abs() * (h + rel) * 1.02 + smallest(dtype)
                                                      + smallest(dtype) * v.abs().nan_to_num(0.0, 0.0, 0.0).sum(0))
     return out, bound
+
+
+def attention_at_once(batch, q, k_cache, v_cache, scale):
+    """The same for long chunks, on the tensors' device: products over a sequence's rows.  Values that are not finite reach exactly the
+    rows whose keys include them (every weight stays above zero here); keys are finite wherever a row sees them."""
+    dtype, device = q.dtype, q.device
+    heads, kv_heads, dim = q.size(1), k_cache.size(2), q.size(2)
+    group, h = heads // kv_heads, half_step(q.dtype)
+    out, bound = torch.zeros(q.shape, dtype=torch.float64, device=device), torch.zeros(q.shape, dtype=torch.float64, device=device)
+    at = 0
+    for b, (new, length) in enumerate(zip(batch.new, batch.lens)):
+        first, at = at, at + new
+        length = max(0, length)
+        if not new:
+            continue
+        lost = next((p * batch.page for p in range(-(-length // batch.page)) if batch.page_of(b, p * batch.page) is None), length)
+        j = torch.arange(lost)
+        pages = batch.table[b].long()[j // batch.page].to(device)
+        positions = torch.arange(length - new, length, device=device)
+        sees = torch.arange(lost, device=device)[None, :] <= positions[:, None]
+        counts = (positions + 1).double()[:, None]
+        for kv in range(kv_heads):
+            k = k_cache[pages, (j % batch.page).to(device), kv].double()
+            v = v_cache[pages, (j % batch.page).to(device), kv].double()
+            k = torch.where(sees.any(0)[:, None], k, 0.0)
+            finite = v.nan_to_num(0.0, 0.0, 0.0)
+            kt, kt_abs = k.t().contiguous(), k.abs().t().contiguous()
+            mask = sees.double()
+            nan, up, down = ((mask @ x.double()) > 0 for x in (v.isnan(), v == math.inf, v == -math.inf))
+            beyond = mask @ finite.abs()
+            for head in range(kv * group, (kv + 1) * group):
+                rows = q[first:at, head].double()
+                s = torch.where(sees, rows @ kt * scale, -math.inf)
+                w = torch.where(sees.any(1)[:, None], torch.softmax(s, dim=-1), 0.0)
+                assert bool((w[sees] > 0).all())
+                o = w @ finite
+                reach = torch.where(sees, rows.abs() @ kt_abs, 0.0).amax(-1, keepdim=True) * scale
+                rel = 2 * (reach * (dim + 6) * U32 + (counts + 16) * U32)
+                bound[first:at, head] = (w @ finite.abs() + o.abs()) * (h + rel) * 1.02 + smallest(dtype) + smallest(dtype) * beyond
+                bound[first:at, head][positions < 0] = 0.0
+                o = torch.where(up, math.inf, torch.where(down, -math.inf, o))
+                o[nan | (up & down)] = math.nan
+                o[positions >= lost] = math.nan
+                o[positions < 0] = 0.0
+                out[first:at, head] = o
+    return out.cpu(), bound.nan_to_num(0.0).cpu()
