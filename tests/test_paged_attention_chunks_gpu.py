@@ -1,4 +1,5 @@
-"""paged_attention where a call has rows enough for its largest tiles (128 rows: with 256 units from about 98 thousand rows of queries on)."""
+"""paged_attention where a call has rows enough for its largest tiles (128 rows: with 256 units from about 98 thousand rows of queries on,
+a third of that with heads of more than 128 channels)."""
 import pytest
 import torch
 
@@ -76,3 +77,23 @@ def test_strides_and_an_output_between_others(tde):
     end = int(batch.starts[-1])
     assert_close(out[:end, 1:, :128], want[:end], bound[:end])
     assert bool((out[end:] == 7).all()) and bool((out[:, 0] == 7).all()) and bool((out[..., 128] == 7).all())
+
+
+@pytest.mark.parametrize("new,lens", [([1, 1], [100, 16]), ([40, 3], [90, 7])])
+def test_slots_far_apart(tde, new, lens):
+    """Caches ordered by slot, where eight rows of a load lie 4.7 GB apart."""
+    pages, dim = 5_200_000, 64
+    k, v = (torch.zeros((8, pages, 1, dim), dtype=torch.bfloat16, device="cuda").transpose(0, 1) for _ in (0, 1))
+    assert k.stride(1) * 2 * 7 > 2 ** 32
+    batch = Batch(new, lens, page_size=8, seed=9)
+    q, ks, vs = inputs(batch, 4, 1, dim, torch.bfloat16, 10)
+    k[-batch.pages:], v[-batch.pages:] = ks, vs
+    table, starts, lens_ = batch.on("cuda")
+    table = torch.where(table >= 0, table + (pages - batch.pages), table)
+    got = tde.paged_attention(q, k, v, table, starts, lens_)
+    assert_close(got, *attention(batch, q.cpu(), ks.cpu(), vs.cpu(), dim ** -0.5))
+    added = randn((batch.tokens, 1, dim), torch.bfloat16, 11)
+    tde.append_kv(added, added, k, v, table, starts, lens_)
+    for t, b, p in batch.rows():
+        assert torch.equal(k[pages - batch.pages + batch.page_of(b, p), p % 8], added[t])
+        assert torch.equal(v[pages - batch.pages + batch.page_of(b, p), p % 8], added[t])

@@ -115,30 +115,51 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
     }
     int32_t passed = 0, tiles_passed = 0;
     for (int base = 0;;) {
-        const int32_t tiles = tiles_of<ROWS>(a, count);
+        int32_t tiles = tiles_of<ROWS>(a, count);
         const int32_t chunks = SPLIT && walked(a, len) > it.keys ? (walked(a, len) - 1) / it.keys + 1 : 1;
-        const int32_t items = tiles * chunks;
-        int32_t upto = items, tiles_upto = tiles; // inclusive sums over the lanes
+        int32_t upto = 0, tiles_upto = 0; // inclusive sums over the lanes, of items and tiles
+        const auto add_up = [&] {
+            upto = tiles * chunks;
+            tiles_upto = tiles;
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int32_t below = __shfl_up(upto, m), tiles_below = SPLIT ? __shfl_up(tiles_upto, m) : 0;
-            if (lane >= m) {
-                upto += below;
-                tiles_upto += tiles_below;
+            for (int m = 1; m < 64; m <<= 1) {
+                const int32_t below = __shfl_up(upto, m), tiles_below = SPLIT ? __shfl_up(tiles_upto, m) : 0;
+                if (lane >= m) {
+                    upto += below;
+                    tiles_upto += tiles_below;
+                }
             }
-        }
-        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(passed + upto <= want));
+            return __builtin_popcountll(__builtin_amdgcn_ballot_w64(passed + upto <= want));
+        };
+        int at = add_up();
         if (at < 64) {
-            it.seq = base + at;
+            int32_t place = lane; // of the sequence among these
+            if (!SPLIT) {
+                // Unsplit, what sees most keys goes first: the longest of these sequences, and (below) a sequence's last tiles; short
+                // items then fill the units that are free early (20 sequences of up to 700 tokens behind 3000: 154 us in the call's
+                // order, 132 in this one; 100 of up to 60 tokens, where counting takes its share: 96 and 100).
+                const int32_t there = std::min(64, a.batch.seqs + 1 - base);
+                int32_t rank = 0;
+                for (int i = 0; i < there; ++i) {
+                    const int32_t other = __builtin_amdgcn_readlane(len, i);
+                    rank += (int32_t)(other > len) | ((int32_t)(other == len) & (int32_t)(i < lane));
+                }
+                place = __builtin_amdgcn_ds_permute((lane < there ? rank : lane) * 4, lane);
+                begin = __shfl(begin, place);
+                count = __shfl(count, place);
+                len = __shfl(len, place);
+                tiles = __shfl(tiles, place);
+                at = add_up();
+            }
+            it.seq = base + __builtin_amdgcn_readlane(place, at);
             it.begin = __builtin_amdgcn_readlane(begin, at);
             it.count = __builtin_amdgcn_readlane(count, at);
             it.len = __builtin_amdgcn_readlane(len, at);
             it.chunks = __builtin_amdgcn_readlane(chunks, at);
-            const int32_t local = want - passed - __builtin_amdgcn_readlane(upto - items, at);
+            const int32_t local = want - passed - __builtin_amdgcn_readlane(upto - tiles * chunks, at);
             it.tile = local / it.chunks;
             it.chunk = local - it.tile * it.chunks;
             it.tile_of_call = tiles_passed + __builtin_amdgcn_readlane(tiles_upto - tiles, at) + it.tile;
-            // unsplit, a sequence's last tiles, which see most keys, go first
             if (!SPLIT) it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - it.tile;
             return it;
         }
@@ -301,10 +322,14 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     const uint32_t lds0 = (uint32_t)(uintptr_t)(TDE_LDS char *)lds;
     const int load_row = SHARED ? wave * LOADS * AT_ONCE : 0; // the wavefront's first
     // The rows of a load lie in one page wherever pages hold whole numbers of them: then a load is a scalar address and an offset of the
-    // lane that never changes but for its turn.
-    const bool whole_pages = a.dim == D && a.batch.page.d % AT_ONCE == 0;
+    // lane that never changes but for its turn.  Where 16 rows lie in one page the address is looked up once for them.  (Lanes'
+    // offsets have 32 bits: slots far apart go the other way.  Two blocks of rows leave no scalar registers for loads one by one.)
+    constexpr int SPAN = 16;
+    const bool whole_spans = NB == 2 || a.batch.page.d % SPAN == 0;
+    const bool whole_pages = a.batch.page.d % (NB == 2 ? SPAN : AT_ONCE) == 0 && (a.k_slot | a.v_slot) < 1u << 27;
     const uint32_t k_lane = (uint32_t)(lane / CH) * a.k_slot, v_lane = (uint32_t)(lane / CH) * a.v_slot;
     const uint32_t k_chunk = (uint32_t)((lane % CH) ^ k_turn(lane / CH)) * 16, v_chunk = (uint32_t)((lane % CH) ^ v_turn(lane / CH)) * 16;
+    const uint32_t dim_bytes = (uint32_t)in_place(a.dim * 2);
     // Loads the keys and/or values of a tile (look_up has been called for it) to `to` from the start of lds.  Returns whether exactly
     // LOADS loads were issued for each; lost: keys without a page.
     const auto load = [&](int32_t key0, uint32_t to, uint64_t &lost, auto keys, auto values) -> bool {
@@ -313,17 +338,27 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         const uint32_t first = a.batch.page.quotient((uint32_t)key0) - (uint32_t)window;
         const uint32_t end = a.batch.page.quotient((uint32_t)key0 + KT - 1) - (uint32_t)window;
         if (whole_pages && until - key0 >= KT && (missing >> first << first << (63 - end)) == 0) {
-#pragma unroll 4
+            uint64_t k_at = 0, v_at = 0;
+            uint32_t k_row = 0, v_row = 0;
+#pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int row = load_row + i * AT_ONCE;
-                const uint32_t key = (uint32_t)(key0 + row), page = a.batch.page.quotient(key), slot = key - page * a.batch.page.d;
-                const uint32_t number = (uint32_t)__builtin_amdgcn_readlane(entries, (int)(page - (uint32_t)window));
-                if constexpr (KEYS)
-                    load_to_lds<!SHARED>((uint64_t)k_base + (uint64_t)number * a.k_page + (uint64_t)slot * a.k_slot,
-                                         (k_chunk ^ (uint32_t)k_turn(row) * 16) + k_lane, lds0 + at + i * 1024);
-                if constexpr (VALUES)
-                    load_to_lds<!SHARED>((uint64_t)v_base + (uint64_t)number * a.v_page + (uint64_t)slot * a.v_slot,
-                                         (v_chunk ^ (uint32_t)v_turn(row) * 16) + v_lane, lds0 + at + TILE + i * 1024);
+                if (i % (SPAN / AT_ONCE) == 0 || !whole_spans) {
+                    const uint32_t key = (uint32_t)(key0 + row), page = a.batch.page.quotient(key), slot = key - page * a.batch.page.d;
+                    const uint32_t number = (uint32_t)__builtin_amdgcn_readlane(entries, (int)(page - (uint32_t)window));
+                    if constexpr (KEYS) k_at = (uint64_t)k_base + (uint64_t)number * a.k_page + (uint64_t)slot * a.k_slot;
+                    if constexpr (VALUES) v_at = (uint64_t)v_base + (uint64_t)number * a.v_page + (uint64_t)slot * a.v_slot;
+                    k_row = k_lane;
+                    v_row = v_lane;
+                } else {
+                    k_row += AT_ONCE * a.k_slot;
+                    v_row += AT_ONCE * a.v_slot;
+                }
+                // Channels that the head does not have: the keys' stay zeros (every load has lanes with channels, so none is left out),
+                // the values', which no output takes, repeat the first ones.
+                const uint32_t kc = k_chunk ^ (uint32_t)k_turn(row) * 16, vc = v_chunk ^ (uint32_t)v_turn(row) * 16;
+                if (KEYS && kc < dim_bytes) load_to_lds<!SHARED>(k_at, kc + k_row, lds0 + at + i * 1024);
+                if (VALUES) load_to_lds<!SHARED>(v_at, (vc < dim_bytes ? vc : 0) + v_row, lds0 + at + TILE + i * 1024);
             }
             lost = 0;
             return true;
@@ -800,11 +835,11 @@ namespace {
 
 template <class T, int D, int NB, int WAVES, bool SHARED>
 void launch_one(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks, hipStream_t s) {
+    constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
     if (!p.split) {
         attention_kernel<T, D, NB, WAVES, SHARED, false><<<blocks, 64 * WAVES, 0, s>>>(a);
         return;
     }
-    constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
     attention_kernel<T, D, NB, WAVES, SHARED, true><<<blocks, 64 * WAVES, 0, s>>>(a);
     const uint32_t joins = (uint32_t)a.tiles * a.kv_heads.d;
     if (p.join_waves == 16) attention_join_kernel<T, D, ROWS, 1, 16><<<joins * ROWS, 1024, 0, s>>>(a);
@@ -816,7 +851,7 @@ void launch_dim(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks,
     constexpr int ALONE = D == 256 ? 2 : 4; // wavefronts that each hold tiles of their own in LDS
     if (p.rows == 16) launch_one<T, D, 1, ALONE, false>(a, p, blocks, s);
     else if (p.rows == 64) launch_one<T, D, 1, 4, true>(a, p, blocks, s);
-    else if constexpr (D <= 128) launch_one<T, D, 2, 4, true>(a, p, blocks, s);
+    else attention_kernel<T, D, D <= 128 ? 2 : 1, D <= 128 ? 4 : 8, true, false><<<blocks, D <= 128 ? 256 : 512, 0, s>>>(a); // 128, never split
 }
 
 template <class T>
@@ -833,7 +868,9 @@ void launch_type(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks
 // Rows of a tile: 16, with every wavefront on keys of its own, where sequences have no more rows than that on average (decode steps:
 // bound by the cache's bytes); 128 where they give three workgroups a unit, else 64: a wavefront then has half the work
 // between two barriers, which is what few workgroups wait for (mixed batch of 576 workgroups of 128 rows 74 us, of 64 rows 62; one
-// chunk of 4096 rows behind 4096, 1024 workgroups, 444 and 630).  Heads of more than 128 channels: 64, for the registers.
+// chunk of 4096 rows behind 4096, 1024 workgroups, 425 and 630).  Heads of more than 128 channels have registers for one block of
+// rows a wavefront: 128 rows are eight wavefronts, two a SIMD, wherever they give every unit a workgroup (12 sequences of up to 800 tokens behind
+// 3000, 8 heads, 300 workgroups: 198 us, of 64 rows 235; 2048 tokens behind 2048, 128 workgroups: 191 and 164).
 //
 // Keys are split where a launch would not give every unit its workgroups (four of 16 rows each, one else), into about as many
 // items as that and twice as many of the larger tiles, and none of less than 256 keys (one decode row over 131072 keys 24 us).
@@ -843,11 +880,11 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
     const int64_t group = q_heads / kv_heads, rows_all = tokens * group, cus = device_compute_units();
     if (rows_all > 0x7fffff00) return TDE_ETOOBIG;
     if (rows_all <= (int64_t)seqs * 16) p->rows = 16;
-    else p->rows = p->wide_dim <= 128 && rows_all / 128 * kv_heads >= 3 * cus ? 128 : 64;
+    else p->rows = rows_all / 128 * kv_heads >= (p->wide_dim <= 128 ? 3 : 1) * cus ? 128 : 64;
     const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence and one behind the last
     const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // rather
     p->min_chunk = 256;
-    p->split = likely * kv_heads < (p->rows == 16 ? 4 : 1) * cus && capacity > p->min_chunk;
+    p->split = p->rows < 128 && likely * kv_heads < (p->rows == 16 ? 4 : 1) * cus && capacity > p->min_chunk;
     p->target = std::max<int64_t>(1, (p->rows == 16 ? 4 : 2) * cus / kv_heads);
     p->tiles = tiles;
     p->items = tiles + (p->split ? p->target : 0);
