@@ -160,6 +160,8 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
             it.tile = local / it.chunks;
             it.chunk = local - it.tile * it.chunks;
             it.tile_of_call = tiles_passed + __builtin_amdgcn_readlane(tiles_upto - tiles, at) + it.tile;
+            // sums that overflow, which only overlapping sequences can give, name no tile
+            if ((uint32_t)it.tile >= (uint32_t)__builtin_amdgcn_readlane(tiles, at)) it.seq = -1;
             if (!SPLIT) it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - it.tile;
             return it;
         }
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     const int kv_head = (int)(blockIdx.x - item_index * a.kv_heads.d);
     const Item it = locate<ROWS, SPLIT>(a, (int32_t)item_index, lane);
     const bool parts = SPLIT && it.chunks > 1; // this item's rows go to the second launch
-    if (SPLIT && kv_head == 0 && threadIdx.x == 0 && (it.seq < 0 || it.chunk == 0) && it.tile_of_call < a.tiles) {
+    if (SPLIT && kv_head == 0 && threadIdx.x == 0 && (it.seq < 0 || it.chunk == 0) && (uint32_t)it.tile_of_call < (uint32_t)a.tiles) {
         // What the second launch has to know of each tile that there may be.  Items are at most a.target more than tiles, so the
         // items that are none are enough for the tiles that are none.
         JoinItem *const j = a.joins + it.tile_of_call;
