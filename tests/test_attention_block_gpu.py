@@ -111,6 +111,46 @@ def test_decode_step_in_one_graph(tde):
         assert not got[live:].any()
 
 
+@pytest.mark.parametrize("backend", ["aot_eager", "inductor"])
+def test_under_torch_compile(tde, backend):
+    """A decode step with other operators around, traced through the operators' fake kernels: outputs and changed caches as without."""
+    if backend == "inductor":
+        pytest.importorskip("triton")
+        import torch._inductor.config as inductor_config
+        inductor_config.compile_threads = 1      # compile in this process: no pool of worker processes
+    from torch._dynamo.exc import BackendCompilerFailed
+    torch.manual_seed(7)
+    heads, dim, page, seqs, dtype = 4, 64, 16, 3, torch.bfloat16
+    batch = Batch([1] * seqs, [40, 17, 1], page, seed=8)
+    caches = [torch.randn(batch.pages, page, 1, dim).to(dtype).cuda() for _ in (0, 1)]
+    codes, scales = torch.randint(-127, 128, (seqs, 96)).to(torch.int8).cuda(), torch.rand(seqs).cuda() * 0.01
+    w, u = torch.randint(-127, 128, ((heads + 2) * dim, 96)).to(torch.int8).cuda(), torch.rand((heads + 2) * dim).cuda() * 1e-2
+    g, cs = torch.ones(dim, dtype=dtype).cuda(), table(64, dim).cuda()
+    page_table, starts, lens = batch.on("cuda")
+
+    def step(codes, k_cache, v_cache, out):
+        qkv = tde.int8_linear(codes, scales, w, u).view(seqs, -1, dim)
+        q, k, v = qkv.split([heads, 1, 1], dim=1)
+        first, _ = tde.qk_norm_rope(q, k, g, g, 1e-6, lens - 1, cs)
+        tde.append_kv(k, v * 2, k_cache, v_cache, page_table, starts, lens)
+        q = tde.append_kv(k, v, k_cache, v_cache, page_table, starts, lens, cos_sin=cs, q=q, q_gamma=g, k_gamma=g)
+        tde.paged_attention_out(q, k_cache, v_cache, page_table, starts, lens, out)
+        return tde.paged_attention(q, k_cache, v_cache, page_table, starts, lens).float() + 1, first
+
+    results = []
+    for f in (step, torch.compile(step, backend=backend, fullgraph=True)):
+        k_cache, v_cache, out = caches[0].clone(), caches[1].clone(), torch.zeros((seqs, heads, dim), dtype=dtype, device="cuda")
+        try:
+            y, first = f(codes, k_cache, v_cache, out)
+        except BackendCompilerFailed as e:   # the code generator, not this library
+            pytest.skip("torch.compile backend unavailable here: %s" % str(e)[:200])
+        torch.cuda.synchronize()
+        results.append((y, first, k_cache, v_cache, out))
+    for got, want in zip(results[1], results[0]):
+        assert torch.equal(got, want)
+    assert not torch.equal(results[0][2], caches[0]) and torch.equal(results[0][0], results[0][4].float() + 1)
+
+
 def test_parameters_give_plain_tensors(tde):
     """A gamma that requires a gradient: the operators have none, and their outputs do not pretend to."""
     qkv = torch.randn(3, 4, 64, device="cuda", dtype=torch.bfloat16)

@@ -155,6 +155,16 @@ allreduce_rms = torch.ops.torch_dist_ext.allreduce_rms
 #     sequence become zeros; paged_attention_out(..., out, scale=None) writes to `out` and leaves them as they are.
 int8_linear = torch.ops.torch_dist_ext.int8_linear.default
 qk_norm_rope = torch.ops.torch_dist_ext.qk_norm_rope.default
-append_kv = torch.ops.torch_dist_ext.append_kv.default
+_append_kv = torch.ops.torch_dist_ext.append_kv.default
+_append_kv_queries = torch.ops.torch_dist_ext.append_kv.queries
 paged_attention = torch.ops.torch_dist_ext.paged_attention.default
 paged_attention_out = torch.ops.torch_dist_ext.paged_attention_out.default
+
+
+def append_kv(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos_sin=None, positions=None, q=None, q_gamma=None, k_gamma=None,
+              eps=1e-6, interleaved=False):
+    if q is not None:
+        return _append_kv_queries(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, q, cos_sin, positions, q_gamma, k_gamma, eps, interleaved)
+    if q_gamma is not None:
+        raise RuntimeError("append_kv: q_gamma without q")
+    return _append_kv(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos_sin, positions, k_gamma, eps, interleaved)

@@ -194,10 +194,9 @@ std::tuple<Tensor, Tensor> qk_norm_rope_meta(const Tensor &q, const Tensor &k, c
 
 // ---- append_kv ------------------------------------------------------------------------------------------------------
 
-c10::optional<Tensor> append_kv(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &page_table,
-                                const Tensor &q_starts, const Tensor &kv_lens, const c10::optional<Tensor> &cos_sin,
-                                const c10::optional<Tensor> &positions, const c10::optional<Tensor> &q, const c10::optional<Tensor> &q_gamma,
-                                const c10::optional<Tensor> &k_gamma, double eps, bool interleaved) {
+Tensor run_append(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &page_table,
+                  const Tensor &q_starts, const Tensor &kv_lens, const Tensor *q, const Tensor *cos_sin, const Tensor *positions,
+                  const Tensor *q_gamma, const Tensor *k_gamma, double eps, bool interleaved) {
     constexpr const char *op = "append_kv";
     tde_head_rows r{};
     common_of(r, k, eps, op);
@@ -207,30 +206,45 @@ c10::optional<Tensor> append_kv(const Tensor &k, const Tensor &v, const Tensor &
     r.k_cache = cache_of(k_cache, k, r.kv_heads, r.dim, op, "k_cache");
     r.v_cache = cache_of(v_cache, k, r.kv_heads, r.dim, op, "v_cache");
     r.batch = batch_of(page_table, q_starts, kv_lens, k_cache, v_cache, k, op);
-    r.k_gamma = gamma_of(given_or_null(k_gamma), k, r.dim, op, "k_gamma");
-    rotation_of(r, given_or_null(cos_sin), given_or_null(positions), k, r.tokens, interleaved, op);
+    r.k_gamma = gamma_of(k_gamma, k, r.dim, op, "k_gamma");
+    rotation_of(r, cos_sin, positions, k, r.tokens, interleaved, op);
     const CallDevice device(k);
-    const Tensor *queries = given_or_null(q);
-    c10::optional<Tensor> q_out;
-    if (queries != nullptr) {
-        r.q = heads_of(*queries, k, op, "q");
-        TORCH_CHECK(queries->size(0) == k.size(0) && queries->size(2) == k.size(2), op, ": q and k differ in tokens or dim");
-        r.q_heads = (int32_t)queries->size(1);
-        r.q_gamma = gamma_of(given_or_null(q_gamma), k, r.dim, op, "q_gamma");
-        q_out = device.new_like(*queries);
-        r.q_out = heads_of(*q_out, k, op, "q_out");
-    } else {
-        TORCH_CHECK(given_or_null(q_gamma) == nullptr, op, ": q_gamma without q");
+    Tensor q_out;
+    if (q != nullptr) {
+        r.q = heads_of(*q, k, op, "q");
+        TORCH_CHECK(q->size(0) == k.size(0) && q->size(2) == k.size(2), op, ": q and k differ in tokens or dim");
+        r.q_heads = (int32_t)q->size(1);
+        r.q_gamma = gamma_of(q_gamma, k, r.dim, op, "q_gamma");
+        q_out = device.new_like(*q);
+        r.q_out = heads_of(q_out, k, op, "q_out");
     }
     check_status(tde_append_kv(&r, device.stream()), op);
     return q_out;
 }
 
-c10::optional<Tensor> append_kv_meta(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
-                                     const Tensor &, const c10::optional<Tensor> &, const c10::optional<Tensor> &,
-                                     const c10::optional<Tensor> &q, const c10::optional<Tensor> &, const c10::optional<Tensor> &, double, bool) {
-    if (!q.has_value()) return c10::nullopt;
-    return at::empty_symint(q->sym_sizes(), q->options());
+// Two overloads, with queries and without: an optional output beside changed inputs is nothing that compiled graphs can hold.
+void append_kv(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &page_table, const Tensor &q_starts,
+               const Tensor &kv_lens, const c10::optional<Tensor> &cos_sin, const c10::optional<Tensor> &positions,
+               const c10::optional<Tensor> &k_gamma, double eps, bool interleaved) {
+    run_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, nullptr, given_or_null(cos_sin), given_or_null(positions), nullptr,
+               given_or_null(k_gamma), eps, interleaved);
+}
+
+Tensor append_kv_queries(const Tensor &k, const Tensor &v, const Tensor &k_cache, const Tensor &v_cache, const Tensor &page_table,
+                         const Tensor &q_starts, const Tensor &kv_lens, const Tensor &q, const c10::optional<Tensor> &cos_sin,
+                         const c10::optional<Tensor> &positions, const c10::optional<Tensor> &q_gamma, const c10::optional<Tensor> &k_gamma,
+                         double eps, bool interleaved) {
+    return run_append(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, &q, given_or_null(cos_sin), given_or_null(positions),
+                      given_or_null(q_gamma), given_or_null(k_gamma), eps, interleaved);
+}
+
+void append_kv_meta(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                    const c10::optional<Tensor> &, const c10::optional<Tensor> &, const c10::optional<Tensor> &, double, bool) {}
+
+Tensor append_kv_queries_meta(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                              const Tensor &q, const c10::optional<Tensor> &, const c10::optional<Tensor> &, const c10::optional<Tensor> &,
+                              const c10::optional<Tensor> &, double, bool) {
+    return at::empty_symint(q.sym_sizes(), q.options());
 }
 
 // ---- paged_attention ------------------------------------------------------------------------------------------------
@@ -303,8 +317,10 @@ TORCH_LIBRARY_FRAGMENT(torch_dist_ext, m) {
     m.def("qk_norm_rope(Tensor q, Tensor k, Tensor q_gamma, Tensor k_gamma, float eps, Tensor positions, Tensor cos_sin, "
           "bool interleaved=False) -> (Tensor, Tensor)");
     m.def("append_kv(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor q_starts, Tensor kv_lens, "
-          "Tensor? cos_sin=None, Tensor? positions=None, Tensor? q=None, Tensor? q_gamma=None, Tensor? k_gamma=None, float eps=1e-06, "
-          "bool interleaved=False) -> Tensor?");
+          "Tensor? cos_sin=None, Tensor? positions=None, Tensor? k_gamma=None, float eps=1e-06, bool interleaved=False) -> ()");
+    m.def("append_kv.queries(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor q_starts, "
+          "Tensor kv_lens, Tensor q, Tensor? cos_sin=None, Tensor? positions=None, Tensor? q_gamma=None, Tensor? k_gamma=None, "
+          "float eps=1e-06, bool interleaved=False) -> Tensor");
     m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor q_starts, Tensor kv_lens, "
           "float? scale=None) -> Tensor");
     m.def("paged_attention_out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor q_starts, Tensor kv_lens, "
@@ -315,6 +331,7 @@ TORCH_LIBRARY_IMPL(torch_dist_ext, CUDA, m) {
     m.impl("int8_linear", &int8_linear);
     m.impl("qk_norm_rope", &qk_norm_rope);
     m.impl("append_kv", &append_kv);
+    m.impl("append_kv.queries", &append_kv_queries);
     m.impl("paged_attention", &paged_attention);
     m.impl("paged_attention_out", &paged_attention_out);
 }
@@ -324,6 +341,7 @@ TORCH_LIBRARY_IMPL(torch_dist_ext, Autograd, m) {
     m.impl("int8_linear", torch::CppFunction::makeFallthrough());
     m.impl("qk_norm_rope", torch::CppFunction::makeFallthrough());
     m.impl("append_kv", torch::CppFunction::makeFallthrough());
+    m.impl("append_kv.queries", torch::CppFunction::makeFallthrough());
     m.impl("paged_attention", torch::CppFunction::makeFallthrough());
     m.impl("paged_attention_out", torch::CppFunction::makeFallthrough());
 }
@@ -332,6 +350,7 @@ TORCH_LIBRARY_IMPL(torch_dist_ext, Meta, m) {
     m.impl("int8_linear", &int8_linear_meta);
     m.impl("qk_norm_rope", &qk_norm_rope_meta);
     m.impl("append_kv", &append_kv_meta);
+    m.impl("append_kv.queries", &append_kv_queries_meta);
     m.impl("paged_attention", &paged_attention_meta);
     m.impl("paged_attention_out", &paged_attention_out_meta);
 }
