@@ -29,7 +29,7 @@ def on_gpu(shape, low, high, g):
     (1000, 516, 9000), (2050, 1028, 4100), (260, 1156, 7165),  # 128 x 128
     (1257, 1004, 1100), (129, 1284, 7000),                     # 64 x 128
     (701, 700, 700), (66, 516, 2000), (100, 2052, 1290),       # 64 x 64, pieces
-    (5, 1013, 900), (31, 1025, 257), (33, 515, 300), (300, 259, 1025),   # rows that do not begin on words
+    (5, 1013, 900), (31, 1025, 257), (33, 515, 300), (300, 259, 1025), (1500, 131, 2100), (2000, 517, 1411),   # rows that do not begin on words, tiles of 64 and 128
 ])
 def test_every_tile(tde, tokens, k, n, dtype):
     g = torch.Generator(device="cuda").manual_seed(tokens + k + n)

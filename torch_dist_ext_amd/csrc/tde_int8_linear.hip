@@ -517,8 +517,8 @@ __global__ void __launch_bounds__(64 * WAVES) linear_pieces_kernel(const LinearA
 
 // The same for rows that begin anywhere: operands come straight from memory to registers (a lane's 16 bytes are its part of an
 // instruction's operand), which takes loads of 16 bytes from 16 rows at once.  Bound by those loads, which the hardware splits where
-// they do not begin on words: 10 x 5121 x 7168 takes 32 us, 32 tokens 56 (tiles by way of registers and LDS: 62 either way, and 100 x
-// 5121 x 4096 61 against 91); rows of whole words take 9 and 11.
+// they do not begin on words: 10 x 5121 x 7168 takes 32 us (tiles by way of registers and LDS 49, rows of whole words 9), 24 x 4099 x 4096 18
+// (29), 32 x 1001 x 2000 7 (11); with 7168 channels 32 tokens would be faster in tiles (56 and 45), from 33 on all are.
 template <class T, int MB, int NB, int WAVES, int AHEAD>
 __global__ void __launch_bounds__(64 * WAVES) linear_loose_kernel(const LinearArgs a, int32_t token_tiles) {
     constexpr int TOKENS = 16 * MB, CHANNELS = 16 * NB;
@@ -633,6 +633,14 @@ int launch_pieces(const LinearArgs &a, hipStream_t s) {
     return TDE_OK;
 }
 
+template <class T, int BT, int BN, int WT, int WN>
+int launch_tile(const LinearArgs &a, hipStream_t s) {
+    const int64_t token_tiles = (a.tokens + BT - 1) / BT, blocks = token_tiles * ((a.n + BN - 1) / BN);
+    if (blocks > 0x7fffffff) return TDE_ETOOBIG;
+    linear_tile_kernel<T, BT, BN, WT, WN><<<(uint32_t)blocks, (BT / WT) * (BN / WN) * 64, 0, s>>>(a, (int32_t)token_tiles);
+    return TDE_OK;
+}
+
 template <class T, int MB>
 int launch_loose(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + 16 * MB - 1) / (16 * MB), blocks = token_tiles * ((a.n + 15) / 16);
@@ -703,9 +711,10 @@ int launch_typed(const LinearArgs &a, hipStream_t s) {
     } else if (a.tokens <= 32) {
         st = a.tokens <= 16 ? launch_loose<T, 1>(a, s) : launch_loose<T, 2>(a, s);
     } else {
-        const int64_t token_tiles = (a.tokens + 127) / 128, blocks = token_tiles * ((a.n + 127) / 128);
-        if (blocks > 0x7fffffff) return TDE_ETOOBIG;
-        linear_tile_kernel<T, 128, 128, 64, 64><<<(uint32_t)blocks, 256, 0, s>>>(a, (int32_t)token_tiles);
+        // 128 x 128 by eight wavefronts where such tiles occupy two thirds of the units (1000 x 4099 x 4096, 256 of them, 49 us; 64 x 64
+        // 61), else 64 x 64 (600 x 3001 x 3000, 120 of the larger ones, 32 us against 40; 64 x 5121 x 7168 49 against 62)
+        const int64_t large = ((a.tokens + 127) / 128) * ((a.n + 127) / 128);
+        st = large * 3 >= (int64_t)device_compute_units() * 2 ? launch_tile<T, 128, 128, 64, 32>(a, s) : launch_tile<T, 64, 64, 32, 32>(a, s);
     }
     if (st != TDE_OK) return st;
     const hipError_t e = hipGetLastError();
