@@ -301,7 +301,8 @@ typedef struct tde_cache {
    keys in the cache, those of its new rows included: row q_starts[b] + i has position kv_lens[b] - new_b + i, and key j of
    the sequence lies in slot j % page_size of page page_table[b][j / page_size].
    The contents are not checked on the host and cannot lead a kernel out of bounds:
-   - rows from q_starts[seqs] on belong to no sequence; rows of a sequence with fewer keys than rows may have a negative position;
+   - rows in front of q_starts[0] and from q_starts[seqs] on belong to no sequence and have no position; neither have the first rows of a sequence with
+     fewer keys than rows;
    - a page number outside [0, cache_pages), or a key beyond the table's row, names no page;
    - q_starts is expected to ascend within [0, tokens]; where it does not, what the rows concerned get is unspecified. */
 typedef struct tde_paged_batch {
@@ -340,14 +341,14 @@ int tde_qk_norm_rope(const tde_head_rows *rows, void *hip_stream);
 
 /* k, normed and rotated, and v as it is, into their slots of the caches; with q_heads > 0 the queries, normed and rotated, to q_out
    in the same launch.  Rows without a position, and rows whose page does not exist, change nothing in the caches; q_out's rows
-   without a position become zeros.  Two rows of one call with one slot (a page named twice) leave either's channels in it. */
+   without a position (those of no sequence among them) become zeros.  Two rows of one call with one slot (a page named twice) leave either's channels in it. */
 int tde_append_kv(const tde_head_rows *rows, void *hip_stream);
 
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] over the keys j of the row's sequence up to its own position, for every query head;
    key head h serves query heads h * q_heads / kv_heads and the following.  Scores, softmax and sums in fp32, the weights rounded to
    `dtype` for the product with the values.  What the caches hold in slots that a row does not see -- behind a
    sequence's last key, or later rows of the call -- does not reach it, whatever it is.  A key without a page makes the rows that see
-   it NaN.  Rows without a position (see tde_paged_batch) become zeros; rows behind the last sequence become zeros if zero_tail, else
+   it NaN.  Rows of a sequence without a position (see tde_paged_batch) become zeros; rows of no sequence become zeros if zero_tail, else
    they are left as they are. */
 typedef struct tde_attention {
     int32_t dtype;            /* TDE_BF16, TDE_F16 */

@@ -15,7 +15,7 @@ namespace tde {
 namespace block {
 
 // The token's place: its sequence's cache position and the slot's page.  position < 0: the row belongs to no sequence's range (it
-// lies behind the last one, or its sequence is shorter than its new tokens).
+// lies in front of the first one or behind the last, or its sequence is shorter than its new tokens).
 struct Place {
     int64_t position;
     int32_t page, slot; // page < 0: not in the cache

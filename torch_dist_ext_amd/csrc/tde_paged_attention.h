@@ -30,7 +30,7 @@ struct AttentionArgs {
     float scale_log2;      // scale * log2(e)
     float *partial;        // [items, kv_heads, rows of a tile, D + 4]: sums, their maximum and weight
     JoinItem *joins;       // [tiles]
-    bool zero_tail;        // rows behind the last sequence become zeros
+    bool zero_tail;        // rows of no sequence become zeros
 };
 
 struct AttentionPlan {
