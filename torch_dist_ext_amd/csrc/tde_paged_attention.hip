@@ -56,9 +56,9 @@ __device__ __forceinline__ float max_of_row(float x) {
 }
 
 // What a workgroup works on.  The items of a call: for every sequence its tiles of rows, for every tile its chunks of keys, in that
-// order; the rows of no sequence, in front of the first one and behind the last, are one more "sequence" without keys.
+// order; the rows of no sequence, behind the last one and in front of the first, are two more "sequences" without keys.
 struct Item {
-    int32_t seq;      // seqs: rows of no sequence; -1: none
+    int32_t seq;      // from seqs on: rows of no sequence; -1: none
     int32_t tile;     // of the sequence
     int32_t chunk, chunks;
     int32_t tile_of_call; // number of its tile among the call's; for an item that is none the number of tiles and how many too far it is
@@ -69,19 +69,15 @@ struct Item {
 
 __device__ __forceinline__ int64_t clamped(int64_t x, int64_t low, int64_t high) { return x < low ? low : (x > high ? high : x); }
 
-// Rows in front of the first sequence.
-__device__ __forceinline__ int32_t rows_in_front(const AttentionArgs &a) { return (int32_t)clamped(a.batch.starts[0], 0, a.tokens); }
-
-// The rows and keys of sequence i, whatever the arrays hold: rows inside the call's, lengths not negative.  The rows of no sequence begin
-// with those in front; row t of the others is begin + (t - rows_in_front).
+// The rows and keys of sequence i, whatever the arrays hold: rows inside the call's, lengths not negative.
 __device__ __forceinline__ void extent(const AttentionArgs &a, int i, int32_t &begin, int32_t &count, int32_t &len) {
     begin = count = len = 0;
-    if (i > a.batch.seqs) return;
-    const int64_t s = clamped(a.batch.starts[i], 0, a.tokens);
-    const int64_t e = i == a.batch.seqs ? a.tokens : clamped(a.batch.starts[i + 1], 0, a.tokens);
+    if (i > a.batch.seqs + 1) return;
+    const bool front = i == a.batch.seqs + 1;
+    const int64_t s = front ? 0 : clamped(a.batch.starts[i], 0, a.tokens);
+    const int64_t e = i == a.batch.seqs ? a.tokens : clamped(a.batch.starts[front ? 0 : i + 1], 0, a.tokens);
     begin = (int32_t)s;
     count = (int32_t)(e > s ? e - s : 0);
-    if (i == a.batch.seqs) count = (int32_t)clamped((int64_t)count + rows_in_front(a), 0, a.tokens); // both parts where starts ascend
     if (i < a.batch.seqs) len = a.batch.lens[i] > 0 ? a.batch.lens[i] : 0;
 }
 
@@ -143,7 +139,7 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
                 // Unsplit, what sees most keys goes first: the longest of these sequences, and (below) a sequence's last tiles; short
                 // items then fill the units that are free early (20 sequences of up to 700 tokens behind 3000: 154 us in the call's
                 // order, 132 in this one; 100 of up to 60 tokens, where counting takes its share: 96 and 100).
-                const int32_t there = std::min(64, a.batch.seqs + 1 - base);
+                const int32_t there = std::min(64, a.batch.seqs + 2 - base);
                 int32_t rank = 0;
                 for (int i = 0; i < there; ++i) {
                     const int32_t other = __builtin_amdgcn_readlane(len, i);
@@ -173,7 +169,7 @@ __device__ __forceinline__ Item locate(const AttentionArgs &a, int32_t want, int
         passed += __builtin_amdgcn_readlane(upto, 63);
         tiles_passed += __builtin_amdgcn_readlane(tiles_upto, 63);
         base += 64;
-        if (base > a.batch.seqs) {
+        if (base > a.batch.seqs + 1) {
             it.tile_of_call = tiles_passed + (want - passed);
             return it;
         }
@@ -265,16 +261,13 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         token[n] = there ? it.begin + (int32_t)t : -1;
         last[n] = there ? it.len - it.count + (int32_t)t : -1;
     }
-    if (it.seq == a.batch.seqs) { // rows of no sequence
+    if (it.seq >= a.batch.seqs) { // rows of no sequence
         if (!a.zero_tail || (!SHARED && wave != 0)) return;
-        const int32_t front = rows_in_front(a);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            if (token[n] < 0) continue;
-            // below a.tokens: the number of these rows is, and is at most front + (a.tokens - it.begin)
-            const int32_t t = token[n] - it.begin, row = t < front ? t : it.begin + (t - front);
-            for (int d = quad * 8; d < a.dim; d += 32) store_words<16>(a.out + row * a.out_token + head[n] * a.out_head + d * 2, Words<16>{});
-        }
+        for (int n = 0; n < NB; ++n)
+            if (token[n] >= 0)
+                for (int d = quad * 8; d < a.dim; d += 32)
+                    store_words<16>(a.out + token[n] * a.out_token + head[n] * a.out_head + d * 2, Words<16>{});
         return;
     }
 
@@ -891,7 +884,7 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
     if (rows_all > 0x7fffff00) return TDE_ETOOBIG;
     if (rows_all <= (int64_t)seqs * 16) p->rows = 16;
     else p->rows = rows_all / 128 * kv_heads >= (p->wide_dim <= 128 ? 3 : 1) * cus ? 128 : 64;
-    const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence and one of the rows of none
+    const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence, one in front of them and one behind
     const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // rather
     p->min_chunk = 256;
     p->split = p->rows < 128 && likely * kv_heads < (p->rows == 16 ? 4 : 1) * cus && capacity > p->min_chunk;
