@@ -55,6 +55,15 @@ __device__ __forceinline__ float max_of_row(float x) {
     return __builtin_fmaxf(__builtin_bit_cast(float, h0), __builtin_bit_cast(float, h1));
 }
 
+// The exponent of a weight is x * scale_log2 - m * scale_log2, one instruction that has the second product rounded.  What the rounding
+// leaves is the same for all weights that refer to one maximum, and cancels, but it grows with the product: up to 2^-15 of an octave below 2^10
+// octaves (which is also how far two maxima's weights may be off when they meet), up to 2^7 octaves below 2^32, where a row's largest weight is
+// 0 or no number of T any more.  From 2^10 octaves on the distance from the maximum is taken first, which is exact next to it.
+constexpr float kFarOctaves = 1024.0f;
+
+// What maximum m takes off the maxima that are compared with it; nothing where no key has been seen, for all of them are -inf then.
+__device__ __forceinline__ float seen_or_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+
 // What a workgroup works on.  The items of a call: for every sequence its tiles of rows, for every tile its chunks of keys, in that
 // order; the rows of no sequence, behind the last one and in front of the first, are two more "sequences" without keys.
 struct Item {
@@ -415,10 +424,11 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         }
 
     f32x4 o[NB][D / 16], l[NB]; // l: sums of weights, each of the four elements the whole row's
-    float m[NB];
+    float m[NB], shift[NB], away[NB]; // the maximum; what is taken off exponents; off scores that are far from zero
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         m[n] = -__builtin_inff();
+        shift[n] = away[n] = 0.0f; // nothing seen yet: every weight is 0
         l[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) o[n][d] = f32x4{0, 0, 0, 0};
@@ -523,22 +533,35 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         if (__builtin_amdgcn_ballot_w64(grown) != 0) {
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                const float shift = top_score[n] == -__builtin_inff() ? 0.0f : top_score[n] * a.scale_log2;
-                const float alpha = __builtin_amdgcn_exp2f(m[n] * a.scale_log2 - shift);
+                const float top = seen_or_zero(top_score[n]), octaves = top * a.scale_log2;
+                const float alpha = __builtin_amdgcn_exp2f((m[n] - top) * a.scale_log2);
                 m[n] = top_score[n];
+                const bool near = __builtin_fabsf(octaves) < kFarOctaves;
+                shift[n] = near ? octaves : 0.0f;
+                away[n] = near ? 0.0f : top;
                 l[n] *= alpha;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) o[n][d] *= alpha;
             }
         }
+        bool far = false;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) far = far || away[n] != 0.0f;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(far) != 0, 0)) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int kb = 0; kb < KT / 16; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[n][kb][r] -= away[n];
+        }
         u32x4 p[NB][KT / 32];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            const float shift = m[n] == -__builtin_inff() ? 0.0f : m[n] * a.scale_log2; // nothing seen yet: every weight is 0
 #pragma unroll
             for (int kb = 0; kb < KT / 16; ++kb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[n][kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][r], a.scale_log2, -shift));
+                for (int r = 0; r < 4; ++r) s[n][kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][r], a.scale_log2, -shift[n]));
 #pragma unroll
             for (int ks = 0; ks < KT / 32; ++ks)
                 p[n][ks] = u32x4{T::narrow(s[n][2 * ks][0], s[n][2 * ks][1]), T::narrow(s[n][2 * ks][2], s[n][2 * ks][3]),
@@ -720,13 +743,13 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             float top_m = -__builtin_inff();
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) top_m = __builtin_fmaxf(top_m, ((float *)lds)[(w * 16 * NB + row) * (D + 4) + D]);
-            const float shift = top_m == -__builtin_inff() ? 0.0f : top_m * a.scale_log2;
+            const float top = seen_or_zero(top_m);
             f32x4 sum = {0, 0, 0, 0};
             float all = 0.0f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
                 const float *const part = (const float *)lds + (w * 16 * NB + row) * (D + 4);
-                const float weight = __builtin_amdgcn_exp2f(part[D] * a.scale_log2 - shift);
+                const float weight = __builtin_amdgcn_exp2f((part[D] - top) * a.scale_log2);
                 sum += *(const f32x4 *)(part + d) * weight;
                 all += part[D + 1] * weight;
             }
@@ -786,14 +809,14 @@ __global__ void __launch_bounds__(64 * RW * WAVES) attention_join_kernel(const A
         float top = best;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) top = __builtin_fmaxf(top, pm[i]);
-        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale_log2;
-        const float old = __builtin_amdgcn_exp2f(best * a.scale_log2 - shift);
+        const float from = seen_or_zero(top);
+        const float old = __builtin_amdgcn_exp2f((best - from) * a.scale_log2);
         all *= old;
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[e] *= old;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const float weight = __builtin_amdgcn_exp2f(pm[i] * a.scale_log2 - shift);
+            const float weight = __builtin_amdgcn_exp2f((pm[i] - from) * a.scale_log2);
             const bool counts = c0 + i * WAVES < chunks; // what a repeated chunk holds may not be finite
             all += counts ? pl[i] * weight : 0.0f;
 #pragma unroll
@@ -817,13 +840,13 @@ __global__ void __launch_bounds__(64 * RW * WAVES) attention_join_kernel(const A
         float top = -__builtin_inff();
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) top = __builtin_fmaxf(top, joined[wave + w][D]);
-        const float shift = top == -__builtin_inff() ? 0.0f : top * a.scale_log2;
+        const float from = seen_or_zero(top);
         all = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[e] = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            const float weight = __builtin_amdgcn_exp2f(joined[wave + w][D] * a.scale_log2 - shift);
+            const float weight = __builtin_amdgcn_exp2f((joined[wave + w][D] - from) * a.scale_log2);
             all += joined[wave + w][D + 1] * weight;
 #pragma unroll
             for (int e = 0; e < E; ++e) sum[e] += joined[wave + w][lane * E + e] * weight;
