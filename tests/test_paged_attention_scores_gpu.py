@@ -25,14 +25,14 @@ CALLS = {
 def softmax_of(batch, scores_of, values_of, heads, kv_heads, dim, dtype):
     """From scores [rows, keys] that are exact in doubles and in fp32.  A weight enters twice, in numerator and sum, each time off
 
-    - by half a step of T, an absolute one among T's subnormal numbers: 2^-25 of the largest weight in fp16; in bf16 what lies below fp32's 2^-126
-      may be gone;
+    - by half a step of T, an absolute one among T's subnormal numbers: 2^-36 of the largest weight in fp16, whose largest one is raised to 2^11 at
+      least; in bf16 what lies below fp32's 2^-126 may be gone;
     - by what its exponent is off.  A score d below the row's largest (by way of maxima that lag by up to 12): three roundings of d, the
-      scale's, the difference's, the product's.  Products of a maximum and the scale that are kept rounded, up to 1024 octaves: 2^-15 of an
-      octave, 2^9 * log 2 units of 2^-24, in each of two maxima that meet, twice (wavefronts, launches)."""
+      scale's, the difference's, the product's.  Products of a maximum and the scale that are kept rounded, up to 1024 octaves, and raised: 2^-15 of an
+      octave twice, 2 * 2^9 * log 2 units of 2^-24, in each of two maxima that meet, which they do twice (wavefronts, launches)."""
     out, bound = torch.zeros((batch.tokens, heads, dim), dtype=torch.float64), torch.zeros((batch.tokens, heads, dim), dtype=torch.float64)
     h, at = half_step(dtype), 0
-    lost = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+    lost = 2.0 ** -36 if dtype == torch.float16 else 2.0 ** -126
     for b, (new, length) in enumerate(zip(batch.new, batch.lens)):
         sees = torch.arange(length, device="cuda")[None] <= torch.arange(length - new, length, device="cuda")[:, None]
         for head in range(heads):
@@ -42,7 +42,7 @@ def softmax_of(batch, scores_of, values_of, heads, kv_heads, dim, dtype):
             o, beyond = w @ v, sees.double() @ v.abs()
             counts = sees.sum(-1, keepdim=True)
             distance = (s.amax(-1, keepdim=True) - s).clamp(max=2000.0)
-            wrong = w * (h + (3 * (distance + 12) + 4 * 355 + counts + 16) * U32)
+            wrong = w * (h + (3 * (distance + 12) + 8 * 355 + counts + 16) * U32)
             out[at:at + new, head] = o.cpu()
             bound[at:at + new, head] = ((wrong @ v.abs() + wrong.sum(-1, keepdim=True) * o.abs()) * 1.02 + (h * o.abs() + smallest(dtype)) * 1.02
                                         + lost * (beyond + counts * o.abs()) * w.amax(-1, keepdim=True)).cpu()
@@ -107,4 +107,30 @@ def test_scores_with_a_common_offset(tde, call, offset, dtype):
         return q[starts[b]:starts[b + 1], head] @ keys[b][:, head * kv_heads // heads].t().contiguous() * scale
 
     got = tde.paged_attention(q.to(dtype), k, v, *batch.on("cuda"), scale)
+    assert_close(got, *softmax_of(batch, scores, lambda b, h: values[b][:, h], heads, kv_heads, dim, dtype))
+
+
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("nats", [10.0, 17.375, 21.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_a_key_that_takes_nearly_all_weight(tde, call, nats, dtype):
+    """One key far above all others, whose value is zero: what is left is the sum of the others' small weights."""
+    new, lens, heads, kv_heads = CALLS[call]
+    new, lens = ([1, 1], [20000, 130]) if call == "decode" else (new, lens)
+    batch, dim = Batch(new, lens, page_size=16, seed=7), 64
+    q = torch.zeros((batch.tokens, heads, dim), dtype=torch.float64, device="cuda")
+    q[..., 0] = 1.0
+    keys = [whole((n, kv_heads, dim), -5, 5, 8 + b) for b, n in enumerate(lens)]
+    values = [1.0 + whole((n, kv_heads, dim), 0, 100, 1000 + b) / 128 for b, n in enumerate(lens)]
+    for b, x in enumerate(keys):
+        x[..., 0] = whole(x.shape[:2], -8, 8, 2000 + b) / 64
+        at = x.size(0) // 3 if b % 2 else 0
+        x[at, :, 0], values[b][at] = nats * 1.0, 0.0
+    starts = batch.starts.tolist()
+    k, v = caches(batch, kv_heads, dim, dtype, keys, values)
+
+    def scores(b, head):
+        return q[starts[b]:starts[b + 1], head] @ keys[b][:, head * kv_heads // heads].t().contiguous()
+
+    got = tde.paged_attention(q.to(dtype), k, v, *batch.on("cuda"), 1.0)
     assert_close(got, *softmax_of(batch, scores, lambda b, h: values[b][:, h], heads, kv_heads, dim, dtype))

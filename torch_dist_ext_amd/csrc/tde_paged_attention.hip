@@ -34,6 +34,7 @@ struct Mfma<Bf16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static constexpr uint32_t kExponent = 0x7f80u, kMantissa = 0x007fu;
+    static constexpr float kLag = 8.0f, kRaise = 0.0f; // see where weights are computed
 };
 template <>
 struct Mfma<F16> {
@@ -41,6 +42,7 @@ struct Mfma<F16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
     static constexpr uint32_t kExponent = 0x7c00u, kMantissa = 0x03ffu;
+    static constexpr float kLag = 4.0f, kRaise = 11.0f;
 };
 
 // Maximum over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48): swaps of rows of 16 lanes and of halves, of a value
@@ -516,8 +518,11 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         }
 
         // ---- softmax ----
-        // The maximum that weights refer to only moves once a score exceeds it by 8 octaves: weights stay below 2^8, the largest of a
-        // row at 1 at least, and sums are rarely rescaled.
+        // The maximum that weights refer to only moves once a score exceeds it by kLag octaves, so that sums are rarely rescaled.
+        // Weights and sums alike are raised by kRaise octaves: weights reach 2^(kRaise + kLag), the largest of a row 2^kRaise at least, and sums
+        // are fp32.  In bf16 neither matters.  Of fp16's 40 octaves 2^-24 .. 2^16 the raised ones leave weights of 2^-25 of the
+        // largest all their bits and lose those below 2^-36; unraised, 16 octaves would lie idle above and a row whose one key takes nearly
+        // all would lose what the others add up to (20000 keys at 2^-25 each: nothing of 6e-4).
         float top_score[NB];
         bool grown = false;
 #pragma unroll
@@ -528,7 +533,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
                 for (int r = 0; r < 4; ++r) t = __builtin_fmaxf(t, s[n][kb][r]);
             top_score[n] = __builtin_fmaxf(m[n], max_of_row(t));
-            grown = grown || (top_score[n] - m[n]) * a.scale_log2 > 8.0f;
+            grown = grown || (top_score[n] - m[n]) * a.scale_log2 > Mfma<T>::kLag;
         }
         if (__builtin_amdgcn_ballot_w64(grown) != 0) {
 #pragma unroll
@@ -537,7 +542,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
                 const float alpha = __builtin_amdgcn_exp2f((m[n] - top) * a.scale_log2);
                 m[n] = top_score[n];
                 const bool near = __builtin_fabsf(octaves) < kFarOctaves;
-                shift[n] = near ? octaves : 0.0f;
+                shift[n] = (near ? octaves : 0.0f) - Mfma<T>::kRaise;
                 away[n] = near ? 0.0f : top;
                 l[n] *= alpha;
 #pragma unroll
