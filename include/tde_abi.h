@@ -331,8 +331,8 @@ typedef struct tde_head_rows {
     int64_t cos_sin_rows, cos_sin_stride;
     const void *q_gamma, *k_gamma; /* [dim] of `dtype`, or null */
     tde_heads q, k, v;             /* inputs: tde_qk_norm_rope q, k; tde_append_kv k, v and, if q_heads > 0, q */
-    tde_heads q_out, k_out;        /* outputs, not overlapping the inputs: q_out; k_out of tde_qk_norm_rope */
-    tde_cache k_cache, v_cache;    /* tde_append_kv: kv_heads heads */
+    tde_heads q_out, k_out;        /* outputs: q_out; k_out of tde_qk_norm_rope; no byte twice, apart from each other and the inputs */
+    tde_cache k_cache, v_cache;    /* tde_append_kv: kv_heads heads; no byte twice, apart from each other and the inputs */
     tde_paged_batch batch;         /* tde_append_kv */
     int64_t reserved;              /* must be 0 */
 } tde_head_rows;
@@ -357,7 +357,7 @@ typedef struct tde_attention {
     int64_t tokens;
     float scale;              /* > 0, finite */
     int32_t zero_tail;        /* 0/1 */
-    tde_heads q, out;         /* out must not overlap q */
+    tde_heads q, out;         /* out: no byte twice, apart from q and the caches */
     tde_cache k_cache, v_cache; /* data and strides multiples of 16 bytes (TDE_EALIGN); page and slot strides
                                    below 2^32 bytes (TDE_ESHAPE) */
     tde_paged_batch batch;

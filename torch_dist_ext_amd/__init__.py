@@ -153,6 +153,7 @@ allreduce_rms = torch.ops.torch_dist_ext.allreduce_rms
 #   paged_attention(q, k_cache, v_cache, page_table, q_starts, kv_lens, scale=None) -> [tokens, heads, dim]
 #     causal attention of the new rows over their sequences' keys, bf16 or fp16; scale defaults to dim ** -0.5.  Rows in front of
 #     the first sequence and behind the last become zeros; paged_attention_out(..., out, scale=None) writes to `out` and leaves them as they are.
+# What a call writes (the caches of append_kv, `out`) must not overlap what it reads, nor itself.
 int8_linear = torch.ops.torch_dist_ext.int8_linear.default
 qk_norm_rope = torch.ops.torch_dist_ext.qk_norm_rope.default
 _append_kv = torch.ops.torch_dist_ext.append_kv.default

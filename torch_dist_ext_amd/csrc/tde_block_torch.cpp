@@ -4,6 +4,7 @@
 #include <cmath>
 #include <tuple>
 
+#include "tde_overlap.h"
 #include "tde_torch.h"
 
 namespace {
@@ -91,6 +92,30 @@ tde_cache cache_of(const Tensor &t, const Tensor &like, int64_t heads, int64_t d
     TORCH_CHECK(t.scalar_type() == like.scalar_type(), op, ": ", name, " dtype differs");
     TORCH_CHECK(t.size(3) <= 1 || t.stride(3) == 1, op, ": channels of ", name, " must be contiguous");
     return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+}
+
+// A tensor and the addresses that it lies between, which is all that most calls need to know of it.
+struct Spanned {
+    const Tensor &t;
+    const char *begin, *end;
+    Spanned(const Tensor &tensor, const void *data) : t(tensor), begin(static_cast<const char *>(data)), end(begin) {
+        int64_t last = 0;
+        for (size_t i = 0; i < t.sizes().size(); ++i) {
+            if (t.sizes()[i] == 0) return;
+            last += (t.sizes()[i] - 1) * t.strides()[i];
+        }
+        end += (last + 1) * (int64_t)t.element_size();
+    }
+    tde::Region region() const { return {begin, (int)t.dim(), t.sizes().data(), t.strides().data(), (int64_t)t.element_size()}; }
+};
+
+// What a call writes takes every byte once, and shares none with what it reads or writes besides: rows run in no order.
+void check_written(const Spanned &x, const char *op, const char *name) {
+    TORCH_CHECK(x.t.is_contiguous() || !tde::overlaps_itself(x.region()), op, ": elements of ", name, " overlap");
+}
+void check_apart(const Spanned &written, const Spanned &other, const char *op, const char *name, const char *other_name) {
+    TORCH_CHECK(written.end <= other.begin || other.end <= written.begin || !tde::overlap(written.region(), other.region()), op, ": ", name, " overlaps ",
+                other_name);
 }
 
 const int32_t *ints_of(const Tensor &t, const Tensor &like, int64_t size, const char *op, const char *name) {
@@ -205,6 +230,16 @@ Tensor run_append(const Tensor &k, const Tensor &v, const Tensor &k_cache, const
     TORCH_CHECK(v.sizes() == k.sizes(), op, ": k and v differ in shape");
     r.k_cache = cache_of(k_cache, k, r.kv_heads, r.dim, op, "k_cache");
     r.v_cache = cache_of(v_cache, k, r.kv_heads, r.dim, op, "v_cache");
+    const Spanned keys(k_cache, r.k_cache.data), values(v_cache, r.v_cache.data);
+    check_written(keys, op, "k_cache");
+    check_written(values, op, "v_cache");
+    check_apart(keys, values, op, "k_cache", "v_cache");
+    const auto check_input = [&](const Spanned &rows, const char *name) {
+        check_apart(keys, rows, op, "k_cache", name);
+        check_apart(values, rows, op, "v_cache", name);
+    };
+    check_input({k, r.k.data}, "k");
+    check_input({v, r.v.data}, "v");
     r.batch = batch_of(page_table, q_starts, kv_lens, k_cache, v_cache, k, op);
     r.k_gamma = gamma_of(k_gamma, k, r.dim, op, "k_gamma");
     rotation_of(r, cos_sin, positions, k, r.tokens, interleaved, op);
@@ -213,6 +248,7 @@ Tensor run_append(const Tensor &k, const Tensor &v, const Tensor &k_cache, const
     if (q != nullptr) {
         r.q = heads_of(*q, k, op, "q");
         TORCH_CHECK(q->size(0) == k.size(0) && q->size(2) == k.size(2), op, ": q and k differ in tokens or dim");
+        check_input({*q, r.q.data}, "q");
         r.q_heads = (int32_t)q->size(1);
         r.q_gamma = gamma_of(q_gamma, k, r.dim, op, "q_gamma");
         q_out = device.new_like(*q);
@@ -263,6 +299,13 @@ void run_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache
     TORCH_CHECK(dim >= 8 && dim <= 256 && dim % 8 == 0, op, ": heads of 8 to 256 channels in steps of 8 expected, not ", dim);
     t.k_cache = cache_of(k_cache, q, heads, dim, op, "k_cache");
     t.v_cache = cache_of(v_cache, q, heads, dim, op, "v_cache");
+    if (!zero_tail) { // the caller's output
+        const Spanned written(out, t.out.data);
+        check_written(written, op, "out");
+        check_apart(written, {q, t.q.data}, op, "out", "q");
+        check_apart(written, {k_cache, t.k_cache.data}, op, "out", "k_cache");
+        check_apart(written, {v_cache, t.v_cache.data}, op, "out", "v_cache");
+    }
     t.batch = batch_of(page_table, q_starts, kv_lens, k_cache, v_cache, q, op);
     t.dim = (int32_t)dim;
     t.q_heads = (int32_t)q.size(1);
