@@ -118,6 +118,11 @@ void check_apart(const Spanned &written, const Spanned &other, const char *op, c
                 other_name);
 }
 
+// Counts a change of the tensor, so that a backward pass that saved it before refuses to run on other values.
+void changed(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 const int32_t *ints_of(const Tensor &t, const Tensor &like, int64_t size, const char *op, const char *name) {
     check_on(t, like, op, name);
     TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.size(0) == size, op, ": ", name,
@@ -255,6 +260,8 @@ Tensor run_append(const Tensor &k, const Tensor &v, const Tensor &k_cache, const
         r.q_out = heads_of(q_out, k, op, "q_out");
     }
     check_status(tde_append_kv(&r, device.stream()), op);
+    changed(k_cache);
+    changed(v_cache);
     return q_out;
 }
 
@@ -323,6 +330,7 @@ void run_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache
         t.workspace = workspace.data_ptr();
     }
     check_status(tde_paged_attention(&t, device.stream()), op);
+    if (!zero_tail) changed(out);
 }
 
 void check_queries(const Tensor &q) {
