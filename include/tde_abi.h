@@ -46,7 +46,8 @@ typedef enum tde_status {
     TDE_EHIP = 9,       /* HIP runtime error; see tde_last_hip_error() */
     TDE_ERANK = 10,     /* rank outside [0,nranks) */
     TDE_ENOMEM = 11,    /* device allocation failed */
-    TDE_ETOOBIG = 12    /* tde_reduce_rms_static_stage: the rows do not fit the library's static stage */
+    TDE_ETOOBIG = 12    /* tde_reduce_rms_static_stage: the rows do not fit the library's static stage; the attention block's
+                           operators: more threads than one launch holds (2^32) */
 } tde_status;
 
 /* ---- enums ---------------------------------------------------------------------------------- */

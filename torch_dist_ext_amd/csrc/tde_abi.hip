@@ -690,7 +690,7 @@ const char *tde_status_string(int status) {
     case TDE_EHIP: return "HIP runtime error (see tde_last_hip_error)";
     case TDE_ERANK: return "rank outside [0, nranks)";
     case TDE_ENOMEM: return "device allocation failed";
-    case TDE_ETOOBIG: return "tokens*hidden*elem_size exceeds the library's static stage (TDE_STATIC_STAGE_BYTES)";
+    case TDE_ETOOBIG: return "tokens*hidden*elem_size exceeds the library's static stage (TDE_STATIC_STAGE_BYTES), or more work than one launch holds";
     }
     return "unknown status";
 }

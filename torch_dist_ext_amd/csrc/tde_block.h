@@ -16,6 +16,9 @@ int device_compute_units();   // of the current device; 256 where none can be as
 
 namespace block {
 
+// Whether a launch holds that many threads: the packet that starts it counts them in 32 bits.
+inline bool fits_launch(int64_t blocks, int threads) { return blocks <= (int64_t)0xffffffff / threads; }
+
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));

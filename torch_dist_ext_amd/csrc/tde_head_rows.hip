@@ -351,6 +351,7 @@ int plan_head_rows(int elem, int dim, int half, bool interleaved, int64_t tokens
     p->waves_per_token = (uint32_t)waves;
     if (waves != 0 && tokens > (int64_t)0x7ffffff0 / waves) return TDE_ETOOBIG;
     p->blocks = (uint32_t)((tokens * waves + 3) / 4);
+    if (!fits_launch(p->blocks, 256)) return TDE_ETOOBIG;
     return TDE_OK;
 }
 

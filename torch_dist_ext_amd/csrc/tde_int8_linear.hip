@@ -606,18 +606,20 @@ __global__ void __launch_bounds__(64 * WAVES) linear_loose_kernel(const LinearAr
 bool streams(const LinearArgs &a) { return a.n * a.k >= (int64_t)32 << 20; }
 
 template <class T, int M>
-void launch_dot(const LinearArgs &a, hipStream_t s) {
+int launch_dot(const LinearArgs &a, hipStream_t s) {
+    if (!fits_launch((a.n + (a.n >= 8192 ? 15 : 3)) / (a.n >= 8192 ? 16 : 4), 256)) return TDE_ETOOBIG;
     // four channels a wavefront share the codes' loads; one where that leaves few wavefronts
     if (a.n >= 8192 && streams(a)) linear_dot_kernel<T, M, 4, 2, true><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
     else if (a.n >= 8192) linear_dot_kernel<T, M, 4, 2, false><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
     else if (streams(a)) linear_dot_kernel<T, M, 1, 4, true><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
     else linear_dot_kernel<T, M, 1, 4, false><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
+    return TDE_OK;
 }
 
 template <class T, int BT, int BN, int WT, int WN, int STAGES>
 int launch_staged(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + BT - 1) / BT, channel_tiles = (a.n + BN - 1) / BN;
-    if (token_tiles * channel_tiles > 0x7fffffff / 8) return TDE_ETOOBIG;
+    if (!fits_launch(token_tiles * channel_tiles, (BT / WT) * (BN / WN) * 64)) return TDE_ETOOBIG;
     const TileOrder order{(uint32_t)(token_tiles * channel_tiles), (uint32_t)token_tiles, (uint32_t)channel_tiles};
     linear_staged_kernel<T, BT, BN, WT, WN, STAGES><<<order.tiles, (BT / WT) * (BN / WN) * 64, 0, s>>>(a, order);
     return TDE_OK;
@@ -626,7 +628,7 @@ int launch_staged(const LinearArgs &a, hipStream_t s) {
 template <class T, int MB, int NB, int WAVES, int STAGES>
 int launch_pieces(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + 16 * MB - 1) / (16 * MB), blocks = token_tiles * ((a.n + 16 * NB - 1) / (16 * NB));
-    if (blocks > 0x7fffffff) return TDE_ETOOBIG;
+    if (!fits_launch(blocks, 64 * WAVES)) return TDE_ETOOBIG;
     if (streams(a) && token_tiles == 1)
         linear_pieces_kernel<T, MB, NB, WAVES, STAGES, true><<<(uint32_t)blocks, 64 * WAVES, 0, s>>>(a, (int32_t)token_tiles);
     else linear_pieces_kernel<T, MB, NB, WAVES, STAGES, false><<<(uint32_t)blocks, 64 * WAVES, 0, s>>>(a, (int32_t)token_tiles);
@@ -636,7 +638,7 @@ int launch_pieces(const LinearArgs &a, hipStream_t s) {
 template <class T, int BT, int BN, int WT, int WN>
 int launch_tile(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + BT - 1) / BT, blocks = token_tiles * ((a.n + BN - 1) / BN);
-    if (blocks > 0x7fffffff) return TDE_ETOOBIG;
+    if (!fits_launch(blocks, (BT / WT) * (BN / WN) * 64)) return TDE_ETOOBIG;
     linear_tile_kernel<T, BT, BN, WT, WN><<<(uint32_t)blocks, (BT / WT) * (BN / WN) * 64, 0, s>>>(a, (int32_t)token_tiles);
     return TDE_OK;
 }
@@ -644,7 +646,7 @@ int launch_tile(const LinearArgs &a, hipStream_t s) {
 template <class T, int MB>
 int launch_loose(const LinearArgs &a, hipStream_t s) {
     const int64_t token_tiles = (a.tokens + 16 * MB - 1) / (16 * MB), blocks = token_tiles * ((a.n + 15) / 16);
-    if (blocks > 0x7fffffff) return TDE_ETOOBIG;
+    if (!fits_launch(blocks, 512)) return TDE_ETOOBIG;
     linear_loose_kernel<T, MB, 1, 8, 2><<<(uint32_t)blocks, 512, 0, s>>>(a, (int32_t)token_tiles);
     return TDE_OK;
 }
@@ -689,9 +691,9 @@ int launch_typed(const LinearArgs &a, hipStream_t s) {
     int st = TDE_OK;
     const bool words = a.k % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.codes) | reinterpret_cast<uintptr_t>(a.weight)) & 3u) == 0;
     if (a.tokens <= 4) {
-        if (a.tokens == 1) launch_dot<T, 1>(a, s);
-        else if (a.tokens == 2) launch_dot<T, 2>(a, s);
-        else launch_dot<T, 4>(a, s);
+        if (a.tokens == 1) st = launch_dot<T, 1>(a, s);
+        else if (a.tokens == 2) st = launch_dot<T, 2>(a, s);
+        else st = launch_dot<T, 4>(a, s);
     } else if (words && a.tokens <= 64) {
         // channels of a workgroup: two blocks of 16 where that leaves a workgroup for half of the units at least (16 x 5120 x 7168 9.0
         // us, with one block 12.0; 16 x 8192 x 1280 6.7 and 5.9)

@@ -920,7 +920,11 @@ int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs,
     p->tiles = tiles;
     p->items = tiles + (p->split ? p->target : 0);
     if (p->items > 0x7fffff00 / kv_heads || (p->split && tiles > 0x7fffff00 / kv_heads / p->rows)) return TDE_ETOOBIG;
-    p->join_waves = p->target / likely >= 32 ? 16 : 1; // of a row: where it may have many parts
+    // of a row: where it may have many parts, and a launch holds them for as many tiles as there may be
+    p->join_waves = p->target / likely >= 32 && fits_launch(tiles * kv_heads * p->rows, 1024) ? 16 : 1;
+    // eight wavefronts are the most that a tile has
+    if (!fits_launch(p->items * kv_heads, p->wide_dim == 256 && p->rows == 128 ? 512 : 256)) return TDE_ETOOBIG;
+    if (p->split && !fits_launch(tiles * kv_heads * (p->rows / 4), 256)) return TDE_ETOOBIG;
     if (p->split)
         p->workspace_bytes = p->tiles * (int64_t)sizeof(JoinItem) + p->items * kv_heads * p->rows * (int64_t)(p->wide_dim + 4) * 4;
     return TDE_OK;
