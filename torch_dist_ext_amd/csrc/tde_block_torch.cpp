@@ -75,13 +75,16 @@ Tensor int8_linear_meta(const Tensor &codes, const Tensor &, const Tensor &weigh
 
 // ---- heads and caches -----------------------------------------------------------------------------------------------
 
+// What separates the elements of a dimension: nothing where there is one at most, whatever stride the tensor names.
+int64_t stride_of(const Tensor &t, int64_t d) { return t.size(d) <= 1 ? 0 : t.stride(d); }
+
 // [rows, heads, dim] with neighbouring channels; any row and head strides.
 tde_heads heads_of(const Tensor &t, const Tensor &like, const char *op, const char *name) {
     check_on(t, like, op, name);
     TORCH_CHECK(t.dim() == 3, op, ": ", name, " must be [tokens, heads, dim]");
     TORCH_CHECK(t.scalar_type() == like.scalar_type(), op, ": ", name, " dtype differs");
     TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, op, ": channels of ", name, " must be contiguous");
-    return {t.data_ptr(), t.stride(0), t.stride(1)};
+    return {t.data_ptr(), stride_of(t, 0), stride_of(t, 1)};
 }
 
 // Keys and values: [pages, page_size, heads, dim], any strides but the channels'.
@@ -91,7 +94,7 @@ tde_cache cache_of(const Tensor &t, const Tensor &like, int64_t heads, int64_t d
                 heads, " heads of ", dim);
     TORCH_CHECK(t.scalar_type() == like.scalar_type(), op, ": ", name, " dtype differs");
     TORCH_CHECK(t.size(3) <= 1 || t.stride(3) == 1, op, ": channels of ", name, " must be contiguous");
-    return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+    return {t.data_ptr(), stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)};
 }
 
 // A tensor and the addresses that it lies between, which is all that most calls need to know of it.
@@ -141,7 +144,7 @@ tde_paged_batch batch_of(const Tensor &page_table, const Tensor &q_starts, const
     TORCH_CHECK(seqs <= limit && page_table.size(1) <= limit && k_cache.size(0) <= limit && k_cache.size(1) <= limit, op, ": too many pages");
     tde_paged_batch b{};
     b.page_table = page_table.data_ptr<int32_t>();
-    b.table_stride = page_table.stride(0);
+    b.table_stride = stride_of(page_table, 0);
     b.seqs = (int32_t)seqs;
     b.table_pages = (int32_t)page_table.size(1);
     b.cache_pages = (int32_t)k_cache.size(0);
