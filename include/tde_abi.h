@@ -351,12 +351,13 @@ int tde_append_kv(const tde_head_rows *rows, void *hip_stream);
    sequence's last key, or later rows of the call -- does not reach it, whatever it is.  A key without a page makes the rows that see
    it NaN.  Rows of a sequence without a position (see tde_paged_batch) become zeros; rows of no sequence become zeros if zero_tail, else
    they are left as they are. */
+#define TDE_MAX_SCALE 2e38f /* its product with the base-2 logarithm of e is a number */
 typedef struct tde_attention {
     int32_t dtype;            /* TDE_BF16, TDE_F16 */
     int32_t dim;              /* a multiple of 8, 8 .. 256 (TDE_ESHAPE, TDE_EHIDDEN) */
     int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads */
     int64_t tokens;
-    float scale;              /* > 0, finite */
+    float scale;              /* > 0, at most TDE_MAX_SCALE */
     int32_t zero_tail;        /* 0/1 */
     tde_heads q, out;         /* out: no byte twice, apart from q and the caches */
     tde_cache k_cache, v_cache; /* data and strides multiples of 16 bytes (TDE_EALIGN); page and slot strides

@@ -115,7 +115,7 @@ int check_attention(const tde_attention *t, AttentionPlan *plan) {
     if (t->tokens < 0 || t->tokens >= kMaxRows || t->dim < 1 || t->dim % 8 != 0) return TDE_ESHAPE;
     if (t->q_heads < 1 || t->kv_heads < 1 || t->q_heads % t->kv_heads != 0 || t->q_heads > (1 << 16)) return TDE_ESHAPE;
     if (t->dim > 256) return TDE_EHIDDEN;
-    if (!(t->scale > 0.0f) || !std::isfinite(t->scale) || (t->zero_tail != 0 && t->zero_tail != 1)) return TDE_EINVAL;
+    if (!(t->scale > 0.0f && t->scale <= TDE_MAX_SCALE) || (t->zero_tail != 0 && t->zero_tail != 1)) return TDE_EINVAL;
     if (!heads_ok(t->q) || !heads_ok(t->out) || !cache_ok(t->k_cache) || !cache_ok(t->v_cache)) return TDE_ESHAPE;
     for (const tde_cache *c : {&t->k_cache, &t->v_cache}) // in bytes they are 32-bit factors of the keys' offsets
         if (c->page_stride >= (int64_t)1 << 31 || c->slot_stride >= (int64_t)1 << 31) return TDE_ESHAPE;

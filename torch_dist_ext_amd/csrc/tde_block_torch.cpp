@@ -322,7 +322,7 @@ void run_attention(const Tensor &q, const Tensor &k_cache, const Tensor &v_cache
     t.kv_heads = (int32_t)heads;
     t.tokens = q.size(0);
     const double s = scale.value_or(1.0 / std::sqrt((double)dim));
-    TORCH_CHECK(std::isfinite((float)s) && (float)s > 0.0f, op, ": scale must be positive and finite");
+    TORCH_CHECK((float)s > 0.0f && (float)s <= TDE_MAX_SCALE, op, ": scale must be positive and at most ", TDE_MAX_SCALE);
     t.scale = (float)s;
     t.zero_tail = zero_tail;
     check_status(tde_paged_attention_workspace(&t, &t.workspace_bytes), op);
