@@ -27,3 +27,15 @@ def test_scales_on_tensors(cuda_device):
     assert torch.equal(out.view(64), cache.view(8, 64)[top])        # all weight on one key
     with pytest.raises(RuntimeError, match="scale"):
         tde.paged_attention(q, cache, cache, table, starts, lens, 2.4e38)
+
+
+@pytest.mark.gpu
+def test_head_counts(cuda_device):
+    """Heads are counted in 32 bits: a tensor expanded beyond them is not one of its first few."""
+    import torch_dist_ext_amd as tde
+    many = torch.zeros((1, 1, 1), dtype=torch.bfloat16, device="cuda").expand(1, (1 << 32) + 4, 1)
+    k = torch.zeros((1, 1, 1), dtype=torch.bfloat16, device="cuda")
+    k_cache, v_cache = (torch.zeros((2, 4, 1, 1), dtype=torch.bfloat16, device="cuda") for _ in (0, 1))
+    table, starts, lens = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0, 1]], [0, 1], [5]))
+    with pytest.raises(RuntimeError, match="heads"):
+        tde.append_kv(k, k, k_cache, v_cache, table, starts, lens, q=many)

@@ -82,6 +82,7 @@ int64_t stride_of(const Tensor &t, int64_t d) { return t.size(d) <= 1 ? 0 : t.st
 tde_heads heads_of(const Tensor &t, const Tensor &like, const char *op, const char *name) {
     check_on(t, like, op, name);
     TORCH_CHECK(t.dim() == 3, op, ": ", name, " must be [tokens, heads, dim]");
+    TORCH_CHECK(t.size(1) <= 1 << 16, op, ": at most ", 1 << 16, " heads expected in ", name, ", not ", t.size(1));
     TORCH_CHECK(t.scalar_type() == like.scalar_type(), op, ": ", name, " dtype differs");
     TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, op, ": channels of ", name, " must be contiguous");
     return {t.data_ptr(), stride_of(t, 0), stride_of(t, 1)};
