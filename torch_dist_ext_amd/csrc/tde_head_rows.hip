@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(256) head_rows_kernel(const HeadRowsArgs a) {
 }
 
 // Any head length and rotation: a wavefront for each row, one element a lane at a time; the partner is read again (from the cache
-// nearest to the unit).  Taken where no chunk of 8 bytes divides the head and the rotation's halves.
+// nearest to the unit).  Taken where no chunk of 8 bytes divides the head and the rotation's halves, and where a wavefront's lanes do not hold
+// a row with two chunks each: more than 512 channels in fp32, or in 2-byte types where only chunks of 8 bytes divide them.
 template <class T, bool INTERLEAVED, bool PAGED>
 __global__ void __launch_bounds__(256) head_elements_kernel(const HeadRowsArgs a) {
     const int lane = threadIdx.x & 63;
@@ -335,7 +336,9 @@ int plan_head_rows(int elem, int dim, int half, bool interleaved, int64_t tokens
         const int64_t at_once = 64 >> p->lanes_log2;
         const auto waves_of = [&](int rows) { return (heads_all + rows * at_once - 1) / (rows * at_once); };
         // Rows that share a lane's cosines and sines: as many as make the fewest wavefronts' work, counting those loads as two rows,
-        // once there is work for every unit at least four times over; before that one, and more wavefronts.
+        // once there is work for every unit at least four times over; before that one, and more wavefronts.  (8192 tokens x 40 heads of 128: by 5
+        // rows 35.0 us, 2 38.3, 3 38.0, 4 41.0; x 20 heads by 3 21.1, 2 23.5, 5 23.3.  4 is not built: where it would be taken, with 32 heads, it
+        // is 31.1, 5 32.4.)
         if (p->chunk_bytes == 16 && tokens * waves_of(5) >= 4096) {
             int64_t best = 0;
             for (int rows : {2, 3, 5}) {

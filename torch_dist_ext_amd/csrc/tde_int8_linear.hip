@@ -608,7 +608,9 @@ bool streams(const LinearArgs &a) { return a.n * a.k >= (int64_t)32 << 20; }
 template <class T, int M>
 int launch_dot(const LinearArgs &a, hipStream_t s) {
     if (!fits_launch((a.n + (a.n >= 8192 ? 15 : 3)) / (a.n >= 8192 ? 16 : 4), 256)) return TDE_ETOOBIG;
-    // four channels a wavefront share the codes' loads; one where that leaves few wavefronts
+    // Four channels a wavefront share the codes' loads; one where that leaves few wavefronts.  With rows of 8192 bytes, in us: four tokens x 8192
+    // channels 17.9 (one channel a wavefront 22.5), x 4096 13.5 (12.3), x 1280 8.9 (5.4); two x 8192 14.1 (16.2), x 4096 11.2 (9.2); one token has no
+    // codes to share: x 8192 12.5 (12.4), x 10240 17.0 (14.9), but 28672 channels of 2048 bytes 10.6 (12.0).
     if (a.n >= 8192 && streams(a)) linear_dot_kernel<T, M, 4, 2, true><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
     else if (a.n >= 8192) linear_dot_kernel<T, M, 4, 2, false><<<(uint32_t)((a.n + 15) / 16), 256, 0, s>>>(a);
     else if (streams(a)) linear_dot_kernel<T, M, 1, 4, true><<<(uint32_t)((a.n + 3) / 4), 256, 0, s>>>(a);
@@ -653,14 +655,14 @@ int launch_loose(const LinearArgs &a, hipStream_t s) {
 
 // ---- which kernel ----
 
-// From four tokens on every kernel works on tiles, and which one is best follows from how many rounds its tiles need on the units and
+// From 65 tokens on every kernel works on tiles, and which one is best follows from how many rounds its tiles need on the units and
 // what 128 bytes of the rows cost in a round (microseconds, measured with every unit busy) beside what a launch costs at all:
 //
 //   tokens x channels  a round's 128 bytes  launch   e.g. (us, against the next best)
 //   256 x 256          1.9                  5        8192 x 8192 x 8192 487 (256 x 128: 553)
 //   256 x 128          1.17                 4        2048 x 4096 x 4096 41 (128 x 128: 49)
 //   128 x 128          0.66                 4        512 x 8192 x 8192 46 (256 x 128: 61)
-//   64 x 128           0.55                 3.5      1257 x 5000 x 1100 21.9 (64 x 64: 25.1)
+//   64 x 128           0.55                 3.5      1257 x 5000 x 1100 22.8 (64 x 64: 26.0)
 //   64 x 64            0.37 one a unit, 0.62 two a unit at once
 //                                           3.5      128 x 5120 x 7168 18.3 (64 x 32: 22.2)
 //   64 x 32 in pieces  0.25, 0.11 where fewer than half of the units are busy

@@ -29,7 +29,6 @@ template <class T>
 struct Mfma;
 template <>
 struct Mfma<Bf16> {
-    typedef bf16x8 operand;
     static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -904,7 +903,10 @@ void launch_type(const AttentionArgs &a, const AttentionPlan &p, uint32_t blocks
 // 3000, 8 heads, 300 workgroups: 198 us, of 64 rows 235; 2048 tokens behind 2048, 128 workgroups: 191 and 164).
 //
 // Keys are split where a launch would not give every unit its workgroups (four of 16 rows each, one else), into about as many
-// items as that and twice as many of the larger tiles, and none of less than 256 keys (one decode row over 131072 keys 24 us).
+// items as that and twice as many of the larger tiles, and none of less than 256 keys (one decode row over 131072 keys 24 us).  Splitting
+// beyond that was measured with heads of 256 alone, one wavefront a SIMD (2048 tokens behind 2048 164 us, split 243).  The rule
+// sees rows, not lengths, those of no sequence included: one long sequence among many, or decode rows beside chunks that fill the
+// units, are walked by one workgroup a key head.
 int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
     *p = AttentionPlan{};
     p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
