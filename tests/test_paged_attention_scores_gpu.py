@@ -22,7 +22,7 @@ CALLS = {
 }
 
 
-def softmax_of(batch, scores_of, values_of, heads, kv_heads, dim, dtype):
+def softmax_of(batch, scores_of, values_of, heads, kv_heads, dim, dtype, weight_step=None):
     """From scores [rows, keys] that are exact in doubles and in fp32.  A weight enters twice, in numerator and sum, each time off
 
     - by half a step of T, an absolute one among T's subnormal numbers: 2^-36 of the largest weight in fp16, whose largest one is raised to 2^11 at
@@ -32,6 +32,7 @@ def softmax_of(batch, scores_of, values_of, heads, kv_heads, dim, dtype):
       octave twice, 2 * 2^9 * log 2 units of 2^-24, in each of two maxima that meet, which they do twice (wavefronts, launches)."""
     out, bound = torch.zeros((batch.tokens, heads, dim), dtype=torch.float64), torch.zeros((batch.tokens, heads, dim), dtype=torch.float64)
     h, at = half_step(dtype), 0
+    weight_step = h if weight_step is None else weight_step
     lost = 2.0 ** -36 if dtype == torch.float16 else 2.0 ** -126
     for b, (new, length) in enumerate(zip(batch.new, batch.lens)):
         sees = torch.arange(length, device="cuda")[None] <= torch.arange(length - new, length, device="cuda")[:, None]
@@ -42,7 +43,7 @@ def softmax_of(batch, scores_of, values_of, heads, kv_heads, dim, dtype):
             o, beyond = w @ v, sees.double() @ v.abs()
             counts = sees.sum(-1, keepdim=True)
             distance = (s.amax(-1, keepdim=True) - s).clamp(max=2000.0)
-            wrong = w * (h + (3 * (distance + 12) + 8 * 355 + counts + 16) * U32)
+            wrong = w * (weight_step + (3 * (distance + 12) + 8 * 355 + counts + 16) * U32)
             out[at:at + new, head] = o.cpu()
             bound[at:at + new, head] = ((wrong @ v.abs() + wrong.sum(-1, keepdim=True) * o.abs()) * 1.02 + (h * o.abs() + smallest(dtype)) * 1.02
                                         + lost * (beyond + counts * o.abs()) * w.amax(-1, keepdim=True)).cpu()
@@ -134,3 +135,24 @@ def test_a_key_that_takes_nearly_all_weight(tde, call, nats, dtype):
 
     got = tde.paged_attention(q.to(dtype), k, v, *batch.on("cuda"), 1.0)
     assert_close(got, *softmax_of(batch, scores, lambda b, h: values[b][:, h], heads, kv_heads, dim, dtype))
+
+
+@pytest.mark.parametrize("call", ["decode", "decode whole"])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_decode_rows_are_off_by_their_own_rounding(tde, call, dim, dtype):
+    """With 16 rows a tile weights are two numbers of T: half a step of half a step of a weight is lost."""
+    new, lens, heads, kv_heads = CALLS[call]
+    batch = Batch(new, lens, page_size=16, seed=11)
+    q = whole((batch.tokens, heads, dim), -3, 3, 12)
+    keys = [whole((n, kv_heads, dim), -3, 3, 13 + b) for b, n in enumerate(lens)]
+    values = [whole((n, kv_heads, dim), -200, 200, 1000 + b) / 64 for b, n in enumerate(lens)]
+    scale, starts = 2.0 ** -5, batch.starts.tolist()
+    k, v = caches(batch, kv_heads, dim, dtype, keys, values)
+
+    def scores(b, head):
+        return q[starts[b]:starts[b + 1], head] @ keys[b][:, head * kv_heads // heads].t().contiguous() * scale
+
+    got = tde.paged_attention(q.to(dtype), k, v, *batch.on("cuda"), scale)
+    values = [x.to(dtype).double() for x in values]
+    assert_close(got, *softmax_of(batch, scores, lambda b, h: values[b][:, h], heads, kv_heads, dim, dtype, half_step(dtype) ** 2))

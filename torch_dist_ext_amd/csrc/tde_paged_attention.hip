@@ -9,8 +9,10 @@
 // An instruction's result has its 16 columns -- the rows -- along the lanes, so a row's maximum, sum and rescaling factor are one value
 // a lane, and a lane's scores of two key blocks are, converted to T, its operand of the second product without any exchange: the
 // product's keys only need the same order on both sides, and V' is read from LDS with transposing loads in just that order.
-// The weights are rounded to T for the second product, whose operands are T, and their sum is that of the rounded ones: one more
-// product, with a row of ones.
+// The weights go into the second product, whose operands are T, rounded to T, and their sum is that of the rounded ones: one more product, with
+// a row of ones.  Where calls wait for the caches' bytes (16 rows a tile) what the rounding leaves goes in as a second operand: the
+// result is then off by its own rounding alone (error against doubles 0.0017 in place of 0.0022 in bf16, 64 rows over up to 8192 keys 195.1 us
+// and 194.7).  Chunks wait for their instructions, and stay with one: 4096 rows behind 4096 take 406 us, with two operands 540.
 //
 // Where the rows of a call fill few workgroups the keys are split as well (see locate) and a second launch joins the parts.
 #include "tde_paged_attention.h"
@@ -231,6 +233,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
     constexpr int AT_ONCE = 64 / CH;                  // rows of a load
     constexpr int LOADS = KT / AT_ONCE / LOADERS;     // a wavefront, of keys and of values
     constexpr int TILE = KT * D * 2;
+    constexpr bool REST = !SHARED; // weights as two numbers of T
     constexpr int BUFFERS = SHARED ? 2 : WAVES;
     constexpr int JOIN = SHARED ? 0 : WAVES * 16 * NB * (D + 4) * 4;
     constexpr int LDS = 2 * TILE * BUFFERS > JOIN ? 2 * TILE * BUFFERS : JOIN;
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[n][kb][r] -= away[n];
         }
-        u32x4 p[NB][KT / 32];
+        u32x4 p[NB][KT / 32], rest[NB][REST ? KT / 32 : 1];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -570,6 +573,17 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
             for (int ks = 0; ks < KT / 32; ++ks)
                 p[n][ks] = u32x4{T::narrow(s[n][2 * ks][0], s[n][2 * ks][1]), T::narrow(s[n][2 * ks][2], s[n][2 * ks][3]),
                                  T::narrow(s[n][2 * ks + 1][0], s[n][2 * ks + 1][1]), T::narrow(s[n][2 * ks + 1][2], s[n][2 * ks + 1][3])};
+            if constexpr (REST) {
+#pragma unroll
+                for (int ks = 0; ks < KT / 32; ++ks)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        float lo, hi;
+                        T::widen(p[n][ks][w], lo, hi);
+                        const f32x4 x = s[n][2 * ks + (w >> 1)];
+                        rest[n][ks][w] = T::narrow(x[(w & 1) * 2] - lo, x[(w & 1) * 2 + 1] - hi);
+                    }
+            }
         }
 
         __builtin_amdgcn_sched_barrier(0);
@@ -672,7 +686,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
         for (int ks = 0; ks < KT / 32; ++ks)
 #pragma unroll
-            for (int n = 0; n < NB; ++n) l[n] = Mfma<T>::mul(u32x4{ones, ones, ones, ones}, p[n][ks], l[n]);
+            for (int n = 0; n < NB; ++n) {
+                l[n] = Mfma<T>::mul(u32x4{ones, ones, ones, ones}, p[n][ks], l[n]);
+                if constexpr (REST) l[n] = Mfma<T>::mul(u32x4{ones, ones, ones, ones}, rest[n][ks], l[n]);
+            }
         {
             constexpr int U = 4, UNITS = KT / 32 * (D / 16 / U);
             u32x4 vf[2][U];
@@ -690,7 +707,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], p[n][ks], o[n][d + u]);
+                    for (int n = 0; n < NB; ++n) {
+                        o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], p[n][ks], o[n][d + u]);
+                        if constexpr (REST) o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], rest[n][ks], o[n][d + u]);
+                    }
             }
         }
 
