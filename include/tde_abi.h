@@ -348,8 +348,8 @@ int tde_append_kv(const tde_head_rows *rows, void *hip_stream);
 
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] over the keys j of the row's sequence up to its own position, for every query head;
    key head h serves query heads h * q_heads / kv_heads and the following.  Scores, softmax and sums in fp32.  Weights are held as two numbers
-   of `dtype` for the product with the values where sequences have 16 rows on average (of query heads that share a key head) at most,
-   else rounded to one, and summed so (fp16: to 2^-11 of a weight down to 2^-25 of the row's largest, to 2^-36 of that below).
+   of `dtype` for the product with the values in calls of at most 16 rows a sequence (tokens, those of no sequence included, times query
+   heads that share a key head), else rounded to one, and summed so (fp16: to 2^-11 of a weight down to 2^-25 of the row's largest, to 2^-36 of that below).
    What the caches hold in slots that a row does not see -- behind a sequence's last key, or later rows of the call -- does not reach it,
    whatever it is.  A key without a page makes the rows that see it NaN.  Rows of a sequence without a position (see tde_paged_batch)
    become zeros; rows of no sequence become zeros if zero_tail, else they are left as they are. */
