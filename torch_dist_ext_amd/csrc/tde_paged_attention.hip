@@ -10,9 +10,10 @@
 // a lane, and a lane's scores of two key blocks are, converted to T, its operand of the second product without any exchange: the
 // product's keys only need the same order on both sides, and V' is read from LDS with transposing loads in just that order.
 // The weights go into the second product, whose operands are T, rounded to T, and their sum is that of the rounded ones: one more product, with
-// a row of ones.  Where calls wait for the caches' bytes (16 rows a tile) what the rounding leaves goes in as a second operand: the
-// result is then off by its own rounding alone (error against doubles 0.0017 in place of 0.0022 in bf16, 64 rows over up to 8192 keys 195.1 us
-// and 194.7).  Chunks wait for their instructions, and stay with one: 4096 rows behind 4096 take 406 us, with two operands 540.
+// a row of ones.  Where calls wait for the caches' bytes (16 rows a tile) what the rounding leaves goes in as a second operand, into sums of
+// its own: the result is then off by its own rounding alone (error against doubles 0.0017 in place of 0.0022 in bf16; 64 rows over up to 8192
+// keys 195.9 us and 194.8, one over 131072 24.5 and 23.9).  Chunks wait for their instructions, and stay with one: 4096 rows behind 4096
+// take 406 us, with two operands 540.
 //
 // Where the rows of a call fill few workgroups the keys are split as well (see locate) and a second launch joins the parts.
 #include "tde_paged_attention.h"
@@ -36,6 +37,8 @@ struct Mfma<Bf16> {
     }
     static constexpr uint32_t kExponent = 0x7f80u, kMantissa = 0x007fu;
     static constexpr float kLag = 8.0f, kRaise = 0.0f; // see where weights are computed
+    // Two numbers within a step of x0 and x1, where another operand takes what is left.
+    static __device__ __forceinline__ uint32_t part(float x0, float x1) { return Bf16::narrow(x0, x1); }
 };
 template <>
 struct Mfma<F16> {
@@ -44,6 +47,9 @@ struct Mfma<F16> {
     }
     static constexpr uint32_t kExponent = 0x7c00u, kMantissa = 0x03ffu;
     static constexpr float kLag = 4.0f, kRaise = 11.0f;
+    static __device__ __forceinline__ uint32_t part(float x0, float x1) { // towards zero: one instruction for both, to nearest it is three
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    }
 };
 
 // Maximum over the four lanes that hold a row (lane, lane ^ 16, lane ^ 32, lane ^ 48): swaps of rows of 16 lanes and of halves, of a value
@@ -224,8 +230,9 @@ __device__ __forceinline__ void wait_for_loads() {
 
 // NB blocks of 16 rows a wavefront.  SHARED: the wavefronts have rows of their own and share tiles of keys, double-buffered in LDS;
 // otherwise all have the same rows and take the tiles in turn, each through LDS of its own, and are joined at the end.
+// (Heads of 64: four such workgroups a unit hide the loads, with the registers of three 8 rows over 16000 keys take 24.0 us in place of 20.2.)
 template <class T, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
-__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel(const AttentionArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED ? 4 : 2)) attention_kernel(const AttentionArgs a) {
     constexpr int KT = SHARED && D <= 128 ? 64 : 32; // keys a tile
     constexpr int CH = D / 8;                        // chunks of 16 bytes a row
     constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
@@ -428,6 +435,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         }
 
     f32x4 o[NB][D / 16], l[NB]; // l: sums of weights, each of the four elements the whole row's
+    f32x4 o_rest[NB][REST ? D / 16 : 1]; // apart: a rest of 0, or of the other sign, would make an infinite value's sum NaN
     float m[NB], shift[NB], away[NB]; // the maximum; what is taken off exponents; off scores that are far from zero
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -435,7 +443,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         shift[n] = away[n] = 0.0f; // nothing seen yet: every weight is 0
         l[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) o[n][d] = f32x4{0, 0, 0, 0};
+        for (int d = 0; d < D / 16; ++d) {
+            o[n][d] = f32x4{0, 0, 0, 0};
+            if constexpr (REST) o_rest[n][d] = f32x4{0, 0, 0, 0};
+        }
     }
 
     const auto sync = [] { // between what a tile's readers and writers do in LDS
@@ -548,7 +559,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
                 away[n] = near ? 0.0f : top;
                 l[n] *= alpha;
 #pragma unroll
-                for (int d = 0; d < D / 16; ++d) o[n][d] *= alpha;
+                for (int d = 0; d < D / 16; ++d) {
+                    o[n][d] *= alpha;
+                    if constexpr (REST) o_rest[n][d] *= alpha;
+                }
             }
         }
         bool far = false;
@@ -571,8 +585,13 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
                 for (int r = 0; r < 4; ++r) s[n][kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kb][r], a.scale_log2, -shift[n]));
 #pragma unroll
             for (int ks = 0; ks < KT / 32; ++ks)
-                p[n][ks] = u32x4{T::narrow(s[n][2 * ks][0], s[n][2 * ks][1]), T::narrow(s[n][2 * ks][2], s[n][2 * ks][3]),
-                                 T::narrow(s[n][2 * ks + 1][0], s[n][2 * ks + 1][1]), T::narrow(s[n][2 * ks + 1][2], s[n][2 * ks + 1][3])};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const f32x4 x = s[n][2 * ks + (w >> 1)];
+                    const float x0 = x[(w & 1) * 2], x1 = x[(w & 1) * 2 + 1];
+                    if constexpr (REST) p[n][ks][w] = Mfma<T>::part(x0, x1);
+                    else p[n][ks][w] = T::narrow(x0, x1);
+                }
             if constexpr (REST) {
 #pragma unroll
                 for (int ks = 0; ks < KT / 32; ++ks)
@@ -581,7 +600,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
                         float lo, hi;
                         T::widen(p[n][ks][w], lo, hi);
                         const f32x4 x = s[n][2 * ks + (w >> 1)];
-                        rest[n][ks][w] = T::narrow(x[(w & 1) * 2] - lo, x[(w & 1) * 2 + 1] - hi);
+                        rest[n][ks][w] = Mfma<T>::part(x[(w & 1) * 2] - lo, x[(w & 1) * 2 + 1] - hi);
                     }
             }
         }
@@ -649,8 +668,8 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
                         for (int hi = 0; hi < 32; hi += 16) {
                             const uint32_t h = (vf[w] >> hi) & 0xffffu;
-                            const float code = (h & M) != 0 ? 16384.0f : ((h & 0x8000u) != 0 ? 128.0f : 1.0f);
-                            marks |= (T::narrow1(code) & ((h & E) == E ? 0xffffu : 0u)) << hi;
+                            const uint32_t code = (h & M) != 0 ? T::narrow1(16384.0f) : ((h & 0x8000u) != 0 ? T::narrow1(128.0f) : T::narrow1(1.0f));
+                            marks |= ((h & E) == E ? code : 0u) << hi;
                         }
                         mark[w] = marks;
                     }
@@ -665,6 +684,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
                             add -= (f & (16384u - 128u)) != 0 ? __builtin_inff() : 0.0f;
                             o[n][d][r] += f >= 16384u ? __builtin_nanf("") : add;
                         }
+                        asm volatile("" : "+v"(o[n][d])); // now, not once all channels' marks have been found
                     }
                 }
             }
@@ -709,7 +729,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
                         o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], p[n][ks], o[n][d + u]);
-                        if constexpr (REST) o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], rest[n][ks], o[n][d + u]);
+                        if constexpr (REST) o_rest[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], rest[n][ks], o_rest[n][d + u]);
                     }
             }
         }
@@ -721,6 +741,15 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : 2) attention_kernel
         }
         key0 = (int32_t)std::min<int64_t>(next, 0x7fffffff);
         next += TILE_STEP;
+    }
+
+    if constexpr (REST) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[n][d][r] += __builtin_fabsf(o[n][d][r]) < __builtin_inff() ? o_rest[n][d][r] : 0.0f;
     }
 
     // ---- what is left ----
