@@ -373,6 +373,78 @@ typedef struct tde_attention {
 int tde_paged_attention_workspace(const tde_attention *attention, int64_t *bytes);
 int tde_paged_attention(const tde_attention *attention, void *hip_stream);
 
+/* ---- the attention block over a paged cache in 4 bits --------------------------------------------
+   A cache holds, for every head and slot, `dim` codes and a scale for each 32 of them.  A code is an e2m1 number: bit 3 the sign, 0 .. 7 for
+   0, 0.5, 1, 1.5, 2, 3, 4, 6; channel 2i lies in the low four bits of byte i, channel 2i + 1 in the high ones.  A scale is a byte e that
+   stands for 2^(e - 127); 255 makes its 32 channels NaN.  dim is a multiple of 32, 32 .. TDE_FP4_MAX_DIM.  In the structures' caches strides count
+   bytes: k_cache and v_cache are those of the codes (dim / 2 a head and slot), k_scales and v_scales those of the scales (dim / 32). */
+#define TDE_FP4_BLOCK 32
+#define TDE_FP4_MAX_DIM 256
+
+/* As tde_append_kv, keys and values rounded to 4 bits.  The scale's exponent is that of the block's largest magnitude, rounded to two
+   significant bits (from 1.75 of a power of two on it is the next one's), less 2, and lies between -125 and the largest whose 6 is a number of
+   `dtype` (125, fp16 13); a channel is the nearest code to its quotient, the even code of two as near, 6 at most.  A block with an infinity or a NaN
+   becomes NaN (scale 255, codes 0).  Keys are normed and rotated in 64 bits, so that only a channel's exact value decides; queries as by tde_append_kv.
+   Codes and scales need no alignment; no byte of the four tensors twice, apart from each other and the inputs. */
+typedef struct tde_append_fp4 {
+    tde_head_rows rows;
+    tde_cache k_scales, v_scales;
+    int64_t reserved; /* must be 0 */
+} tde_append_fp4;
+int tde_append_kv_fp4(const tde_append_fp4 *append, void *hip_stream);
+
+/* As tde_paged_attention; keys and values enter as numbers of `dtype`: exact in bf16 (down to 2^-133), to 2^-25 below 2^-14 in fp16 and infinite beyond
+   65504.  Codes: data and strides multiples of 16 bytes (TDE_EALIGN); scales need no alignment; page and slot strides below 2^31 bytes (TDE_ESHAPE).
+   The workspace is tde_paged_attention_fp4_workspace bytes. */
+typedef struct tde_attention_fp4 {
+    tde_attention attention;
+    tde_cache k_scales, v_scales;
+    int64_t reserved; /* must be 0 */
+} tde_attention_fp4;
+int tde_paged_attention_fp4_workspace(const tde_attention_fp4 *attention, int64_t *bytes);
+int tde_paged_attention_fp4(const tde_attention_fp4 *attention, void *hip_stream);
+
+/* out[i][j][k][d] = T(code * scale), rounded to nearest: rows of `dim` channels in up to three dimensions.  code_strides and scale_strides in bytes, from
+   one row to the next in each dimension; out is contiguous and takes its element's alignment.  The number of rows is below 2^31. */
+typedef struct tde_unpack_fp4_rows {
+    int64_t sizes[3];
+    int64_t code_strides[3], scale_strides[3];
+    int32_t dim;
+    int32_t out_dtype;  /* TDE_BF16, TDE_F16, TDE_F32 */
+    const uint8_t *codes, *scales;
+    void *out;          /* must not overlap an input */
+    int64_t reserved;   /* must be 0 */
+} tde_unpack_fp4_rows;
+int tde_unpack_fp4(const tde_unpack_fp4_rows *rows, void *hip_stream);
+
+/* The pages of a step, for any paged cache: lengths, page tables and slot maps from what each sequence keeps and adds, in device memory alone.
+     1. Sequence b shrinks to keep_lens[b] tokens (to none below 0; not at all where keep_lens is null or more than it has).  Pages without tokens go back
+        on the stack free_pages[0 .. *free_count), the last sequence's first and of a sequence the last one first; what finds no room in
+        free_capacity entries is dropped.
+     2. Sequences grow by new_tokens[b] (none below 0), in order, with pages from the top of the stack.  One grows if its page table's row holds it, if the
+        rows of all up to it that theirs hold are at most `tokens`, and if the pages that these need are at most those on the stack or it needs
+        none; else it keeps what it has and adds no rows.
+   kv_lens, page_table, free_pages and *free_count become those of the step.  q_starts[seqs + 1] are the sums of the rows that were added;
+   positions[tokens] and slots[tokens] their places: in the sequence, and page * page_size + slot; -1 behind the last row.
+   What the arrays hold is not checked on the host and cannot lead a kernel out of bounds: lengths beyond a table's row count as many pages as the row has,
+   and numbers that are no pages stay what they are.  seqs * table_pages < 2^31 (TDE_ETOOBIG).  Page and length arrays share no bytes. */
+typedef struct tde_page_update {
+    int32_t *page_table;       /* [seqs, table_pages] */
+    int32_t *kv_lens;          /* [seqs] */
+    const int32_t *new_tokens; /* [seqs] */
+    const int32_t *keep_lens;  /* [seqs] or null */
+    int32_t *free_pages;       /* [free_capacity] */
+    int32_t *free_count;       /* [1]; counts below 0 and beyond free_capacity are taken as these */
+    int32_t *q_starts;         /* [seqs + 1] */
+    int32_t *positions;        /* [tokens] */
+    int64_t *slots;            /* [tokens] */
+    int64_t table_stride;      /* elements from one row of page_table to the next */
+    int64_t tokens;
+    int32_t seqs, table_pages, free_capacity, page_size;
+    int64_t reserved;          /* must be 0 */
+} tde_page_update;
+int tde_update_pages(const tde_page_update *update, void *hip_stream);
+
 /* ---- emulated peer workspace ----------------------------------------------------------------
    One allocation per emulated rank plays the role of that rank's IPC-mapped comm buffer
    (CommWorkspace, src/ops/all_reduce_fusion.cpp:63-96).  Each slot is 2*slot_bytes large: the

@@ -169,3 +169,47 @@ def append_kv(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos_sin=Non
     if q_gamma is not None:
         raise RuntimeError("append_kv: q_gamma without q")
     return _append_kv(k, v, k_cache, v_cache, page_table, q_starts, kv_lens, cos_sin, positions, k_gamma, eps, interleaved)
+
+
+# The same block over a paged cache in 4 bits: e2m1 codes, two a byte (the even channel's in the low bits), and a byte e for 32 channels that stands
+# for 2^(e - 127).  Codes are uint8 [pages, page_size, kv_heads, dim / 2], scales uint8 [pages, page_size, kv_heads, dim / 32]; dim is 32 to
+# 256 in steps of 32.
+#
+#   fp4_cache(pages, page_size, kv_heads, dim, device="cuda") -> (k_cache, k_scales, v_cache, v_scales)
+#     empty ones, a page's heads one after the other, which is the order that reads fastest.
+#   update_pages(page_table, kv_lens, new_tokens, free_pages, free_count, page_size, tokens, keep_lens=None) -> (q_starts, positions, slots)
+#     a step's page tables and slot maps, for any paged cache: sequences shrink to keep_lens, their pages go back on the stack
+#     free_pages[:free_count], then sequences grow by new_tokens in order, as far as pages, their row of page_table and `tokens` rows reach.
+#     page_table, kv_lens, free_pages and free_count (all int32) change; q_starts[b + 1] - q_starts[b] is what sequence b was given.
+#     positions and slots (page * page_size + slot, int64) have a value for each of `tokens` rows, -1 behind the last.
+#   append_kv_fp4(k, v, k_cache, k_scales, v_cache, v_scales, page_table, q_starts, kv_lens, cos_sin=None, positions=None, q=None, q_gamma=None,
+#                 k_gamma=None, eps=1e-6, interleaved=False) -> q_out or None
+#     as append_kv, keys and values rounded to 4 bits.
+#   paged_attention_fp4(q, k_cache, k_scales, v_cache, v_scales, page_table, q_starts, kv_lens, scale=None) -> [tokens, heads, dim]
+#     as paged_attention; paged_attention_fp4_out(..., out, scale=None) writes to `out` and leaves rows of no sequence as they are.
+#   unpack_fp4(codes, scales, out_dtype=bf16) -> [..., dim]
+#     what codes and scales stand for, in bf16, fp16 or fp32.
+# What a call writes must not overlap what it reads, nor itself.
+_append_kv_fp4 = torch.ops.torch_dist_ext.append_kv_fp4.default
+_append_kv_fp4_queries = torch.ops.torch_dist_ext.append_kv_fp4.queries
+paged_attention_fp4 = torch.ops.torch_dist_ext.paged_attention_fp4.default
+paged_attention_fp4_out = torch.ops.torch_dist_ext.paged_attention_fp4_out.default
+unpack_fp4 = torch.ops.torch_dist_ext.unpack_fp4.default
+update_pages = torch.ops.torch_dist_ext.update_pages.default
+
+
+def fp4_cache(pages, page_size, kv_heads, dim, device="cuda"):
+    if dim % _capi.FP4_BLOCK or not _capi.FP4_BLOCK <= dim <= _capi.FP4_MAX_DIM:
+        raise RuntimeError("fp4_cache: heads of %d to %d channels in steps of %d expected, not %d" % (_capi.FP4_BLOCK, _capi.FP4_MAX_DIM, _capi.FP4_BLOCK, dim))
+    return tuple(torch.zeros((pages, kv_heads, page_size, width), dtype=torch.uint8, device=device).transpose(1, 2)
+                 for width in (dim // 2, dim // _capi.FP4_BLOCK) * 2)
+
+
+def append_kv_fp4(k, v, k_cache, k_scales, v_cache, v_scales, page_table, q_starts, kv_lens, cos_sin=None, positions=None, q=None, q_gamma=None,
+                  k_gamma=None, eps=1e-6, interleaved=False):
+    if q is not None:
+        return _append_kv_fp4_queries(k, v, k_cache, k_scales, v_cache, v_scales, page_table, q_starts, kv_lens, q, cos_sin, positions, q_gamma, k_gamma, eps,
+                                      interleaved)
+    if q_gamma is not None:
+        raise RuntimeError("append_kv_fp4: q_gamma without q")
+    return _append_kv_fp4(k, v, k_cache, k_scales, v_cache, v_scales, page_table, q_starts, kv_lens, cos_sin, positions, k_gamma, eps, interleaved)

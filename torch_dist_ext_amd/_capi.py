@@ -26,6 +26,7 @@ EXPORTS = (
     "tde_workspace_create", "tde_workspace_destroy", "tde_workspace_slot", "tde_workspace_stage",
     "tde_workspace_slot_bytes", "tde_workspace_nranks", "tde_workspace_fill_table",
     "tde_int8_linear", "tde_qk_norm_rope", "tde_append_kv", "tde_paged_attention", "tde_paged_attention_workspace",
+    "tde_append_kv_fp4", "tde_paged_attention_fp4", "tde_paged_attention_fp4_workspace", "tde_unpack_fp4", "tde_update_pages",
 )
 
 
@@ -117,6 +118,33 @@ class Attention(ctypes.Structure):
     ]
 
 
+FP4_BLOCK, FP4_MAX_DIM = 32, 256
+
+
+class AppendFp4(ctypes.Structure):
+    _fields_ = [("rows", HeadRows), ("k_scales", Cache), ("v_scales", Cache), ("reserved", ctypes.c_int64)]
+
+
+class AttentionFp4(ctypes.Structure):
+    _fields_ = [("attention", Attention), ("k_scales", Cache), ("v_scales", Cache), ("reserved", ctypes.c_int64)]
+
+
+class UnpackFp4Rows(ctypes.Structure):
+    _fields_ = [
+        ("sizes", ctypes.c_int64 * 3), ("code_strides", ctypes.c_int64 * 3), ("scale_strides", ctypes.c_int64 * 3), ("dim", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32), ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("out", ctypes.c_void_p), ("reserved", ctypes.c_int64),
+    ]
+
+
+class PageUpdate(ctypes.Structure):
+    _fields_ = [
+        ("page_table", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("new_tokens", ctypes.c_void_p), ("keep_lens", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p), ("free_count", ctypes.c_void_p), ("q_starts", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("tokens", ctypes.c_int64), ("seqs", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32), ("free_capacity", ctypes.c_int32), ("page_size", ctypes.c_int32), ("reserved", ctypes.c_int64),
+    ]
+
+
 class TdeError(RuntimeError):
     def __init__(self, status, text):
         super().__init__("tde status %d: %s" % (status, text))
@@ -175,11 +203,14 @@ def load():
     lib.tde_workspace_fill_table.restype = ctypes.c_int
     lib.tde_workspace_fill_table.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p), ctypes.c_int32]
     for fn, struct in ((lib.tde_int8_linear, Int8Product), (lib.tde_qk_norm_rope, HeadRows), (lib.tde_append_kv, HeadRows),
-                       (lib.tde_paged_attention, Attention)):
+                       (lib.tde_paged_attention, Attention), (lib.tde_append_kv_fp4, AppendFp4), (lib.tde_paged_attention_fp4, AttentionFp4),
+                       (lib.tde_unpack_fp4, UnpackFp4Rows), (lib.tde_update_pages, PageUpdate)):
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
     lib.tde_paged_attention_workspace.restype = ctypes.c_int
     lib.tde_paged_attention_workspace.argtypes = [ctypes.POINTER(Attention), ctypes.POINTER(ctypes.c_int64)]
+    lib.tde_paged_attention_fp4_workspace.restype = ctypes.c_int
+    lib.tde_paged_attention_fp4_workspace.argtypes = [ctypes.POINTER(AttentionFp4), ctypes.POINTER(ctypes.c_int64)]
     _lib = lib
     return lib
 

@@ -160,6 +160,15 @@ __device__ __forceinline__ float sum_over_lanes(float x, int log2) {
     return x;
 }
 
+// The running kernel's only argument, loaded again where it is used: for kernels whose arguments would otherwise take the scalar registers (or spill) from
+// their beginning to their end.
+template <class Args>
+__device__ __forceinline__ const Args &arguments_again() {
+    const auto *p = (const __attribute__((address_space(4))) Args *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Args *)p;
+}
+
 // n / d for n < 2^31 and 1 <= d < 2^31.  With r = floor(2^32 / d), n * r / 2^32 is below n / d by less than n / 2^32 < 1/2, so its
 // floor is the quotient or one less, and one comparison tells which.
 struct Divisor32 {

@@ -3,8 +3,10 @@
 #include <cmath>
 
 #include "tde_abi.h"
+#include "tde_fp4_rows.h"
 #include "tde_head_rows.h"
 #include "tde_int8_linear.h"
+#include "tde_page_update.h"
 #include "tde_paged_attention.h"
 
 using namespace tde::block;
@@ -39,7 +41,9 @@ PagedBatch device_batch(const tde_paged_batch &b) {
     return d;
 }
 
-int head_rows(const tde_head_rows *r, bool paged, void *hip_stream) {
+// Checks a call and fills in its arguments; `nothing`: there is nothing to do.  cache_bytes: of an element of the caches.
+int head_rows_args(const tde_head_rows *r, bool paged, int64_t cache_bytes, HeadRowsArgs &a, bool &nothing) {
+    nothing = false;
     if (r == nullptr || r->reserved != 0) return TDE_EINVAL;
     if (r->dtype != TDE_BF16 && r->dtype != TDE_F16 && r->dtype != TDE_F32) return TDE_EDTYPE;
     if (r->dim < 1 || r->tokens < 0 || r->tokens >= kMaxRows || r->q_heads < 0 || r->kv_heads < 0) return TDE_ESHAPE;
@@ -57,7 +61,10 @@ int head_rows(const tde_head_rows *r, bool paged, void *hip_stream) {
         const int st = check_batch(r->batch);
         if (st != TDE_OK) return st;
     }
-    if (r->tokens == 0 || r->q_heads + r->kv_heads == 0) return TDE_OK;
+    if (r->tokens == 0 || r->q_heads + r->kv_heads == 0) {
+        nothing = true;
+        return TDE_OK;
+    }
     if (r->rot_dim > 0 && (r->cos_sin == nullptr || (!paged && r->positions == nullptr))) return TDE_EINVAL;
     if (r->q_heads > 0 && (!r->q.data || !r->q_out.data)) return TDE_EINVAL;
     if (r->kv_heads > 0) {
@@ -66,7 +73,6 @@ int head_rows(const tde_head_rows *r, bool paged, void *hip_stream) {
     }
 
     const int64_t e = elem_bytes(r->dtype);
-    HeadRowsArgs a{};
     const tde_heads *in[] = {&r->q, &r->k, &r->v};
     for (int i = 0; i < 3; ++i) {
         a.in[i] = static_cast<const char *>(in[i]->data);
@@ -83,9 +89,9 @@ int head_rows(const tde_head_rows *r, bool paged, void *hip_stream) {
         const tde_cache *caches[] = {&r->k_cache, &r->v_cache};
         for (int i = 0; i < 2; ++i) {
             a.out[1 + i] = static_cast<char *>(caches[i]->data);
-            a.out_page[1 + i] = caches[i]->page_stride * e;
-            a.out_token[1 + i] = caches[i]->slot_stride * e;
-            a.out_head[1 + i] = caches[i]->head_stride * e;
+            a.out_page[1 + i] = caches[i]->page_stride * cache_bytes;
+            a.out_token[1 + i] = caches[i]->slot_stride * cache_bytes;
+            a.out_head[1 + i] = caches[i]->head_stride * cache_bytes;
         }
         a.batch = device_batch(r->batch);
     } else {
@@ -106,10 +112,19 @@ int head_rows(const tde_head_rows *r, bool paged, void *hip_stream) {
     a.eps = r->eps;
     a.interleaved = r->interleaved != 0;
     a.paged = paged;
-    return launch_head_rows(a, r->dtype, static_cast<hipStream_t>(hip_stream));
+    return TDE_OK;
 }
 
-int check_attention(const tde_attention *t, AttentionPlan *plan) {
+int head_rows(const tde_head_rows *r, bool paged, void *hip_stream) {
+    HeadRowsArgs a{};
+    bool nothing;
+    const int st = head_rows_args(r, paged, r != nullptr ? elem_bytes(r->dtype) : 0, a, nothing);
+    return st != TDE_OK || nothing ? st : launch_head_rows(a, r->dtype, static_cast<hipStream_t>(hip_stream));
+}
+
+bool fp4_dim_ok(int dim) { return dim >= TDE_FP4_BLOCK && dim % TDE_FP4_BLOCK == 0; }
+
+int check_attention(const tde_attention *t, bool fp4, AttentionPlan *plan) {
     if (t == nullptr || t->reserved != 0) return TDE_EINVAL;
     if (t->dtype != TDE_BF16 && t->dtype != TDE_F16) return TDE_EDTYPE;
     if (t->tokens < 0 || t->tokens >= kMaxRows || t->dim < 1 || t->dim % 8 != 0) return TDE_ESHAPE;
@@ -121,11 +136,58 @@ int check_attention(const tde_attention *t, AttentionPlan *plan) {
         if (c->page_stride >= (int64_t)1 << 31 || c->slot_stride >= (int64_t)1 << 31) return TDE_ESHAPE;
     const int st = check_batch(t->batch);
     if (st != TDE_OK) return st;
-    return plan_attention(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch.seqs, (int64_t)t->batch.table_pages * t->batch.page_size, plan);
+    const int64_t capacity = (int64_t)t->batch.table_pages * t->batch.page_size;
+    return (fp4 ? plan_attention_fp4 : plan_attention)(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch.seqs, capacity, plan);
 }
 
-bool lines_of_16(const tde_cache &c) {
-    return (reinterpret_cast<uintptr_t>(c.data) & 15u) == 0 && c.page_stride % 8 == 0 && c.slot_stride % 8 == 0 && c.head_stride % 8 == 0;
+int check_attention_fp4(const tde_attention_fp4 *t, AttentionPlan *plan) {
+    if (t == nullptr || t->reserved != 0) return TDE_EINVAL;
+    const int st = check_attention(&t->attention, true, plan);
+    if (st != TDE_OK) return st;
+    if (!fp4_dim_ok(t->attention.dim)) return TDE_ESHAPE;
+    for (const tde_cache *c : {&t->k_scales, &t->v_scales})
+        if (!cache_ok(*c) || c->page_stride >= (int64_t)1 << 31 || c->slot_stride >= (int64_t)1 << 31) return TDE_ESHAPE;
+    return TDE_OK;
+}
+
+// Whether a cache's rows begin on 16 bytes; `unit`: bytes of an element.
+bool lines_of_16(const tde_cache &c, int64_t unit) {
+    const int64_t per = 16 / unit;
+    return (reinterpret_cast<uintptr_t>(c.data) & 15u) == 0 && c.page_stride % per == 0 && c.slot_stride % per == 0 && c.head_stride % per == 0;
+}
+
+// Of a call that has rows, whose plan is made; unit: bytes of an element of the caches.
+int attention_args(const tde_attention *t, const AttentionPlan &plan, int64_t unit, AttentionArgs &a) {
+    if (!t->q.data || !t->out.data) return TDE_EINVAL;
+    if (t->batch.cache_pages > 0 && (!t->k_cache.data || !t->v_cache.data)) return TDE_EINVAL;
+    if (!lines_of_16(t->k_cache, unit) || !lines_of_16(t->v_cache, unit)) return TDE_EALIGN;
+    if (plan.workspace_bytes > 0) {
+        if (t->workspace == nullptr || t->workspace_bytes < plan.workspace_bytes) return TDE_EINVAL;
+        if ((reinterpret_cast<uintptr_t>(t->workspace) & 15u) != 0) return TDE_EALIGN;
+    }
+    a.q = static_cast<const char *>(t->q.data);
+    a.k = static_cast<const char *>(t->k_cache.data);
+    a.v = static_cast<const char *>(t->v_cache.data);
+    a.out = static_cast<char *>(t->out.data);
+    a.q_token = t->q.row_stride * 2;
+    a.q_head = t->q.head_stride * 2;
+    a.out_token = t->out.row_stride * 2;
+    a.out_head = t->out.head_stride * 2;
+    a.k_page = (uint32_t)(t->k_cache.page_stride * unit);
+    a.k_slot = (uint32_t)(t->k_cache.slot_stride * unit);
+    a.k_head = t->k_cache.head_stride * unit;
+    a.v_page = (uint32_t)(t->v_cache.page_stride * unit);
+    a.v_slot = (uint32_t)(t->v_cache.slot_stride * unit);
+    a.v_head = t->v_cache.head_stride * unit;
+    a.batch = device_batch(t->batch);
+    a.group = Divisor32((uint32_t)(t->q_heads / t->kv_heads));
+    a.kv_heads = Divisor32((uint32_t)t->kv_heads);
+    a.tokens = t->tokens;
+    a.dim = t->dim;
+    a.scale_log2 = t->scale * 1.4426950408889634f;
+    a.partial = static_cast<float *>(t->workspace);
+    a.zero_tail = t->zero_tail != 0;
+    return TDE_OK;
 }
 
 } // namespace
@@ -150,7 +212,7 @@ int tde_append_kv(const tde_head_rows *rows, void *hip_stream) { return head_row
 int tde_paged_attention_workspace(const tde_attention *t, int64_t *bytes) {
     if (bytes == nullptr) return TDE_EINVAL;
     AttentionPlan plan;
-    const int st = check_attention(t, &plan);
+    const int st = check_attention(t, false, &plan);
     if (st != TDE_OK) return st;
     *bytes = t->tokens == 0 ? 0 : plan.workspace_bytes;
     return TDE_OK;
@@ -158,40 +220,120 @@ int tde_paged_attention_workspace(const tde_attention *t, int64_t *bytes) {
 
 int tde_paged_attention(const tde_attention *t, void *hip_stream) {
     AttentionPlan plan;
-    const int st = check_attention(t, &plan);
-    if (st != TDE_OK) return st;
-    if (t->tokens == 0) return TDE_OK;
-    if (!t->q.data || !t->out.data) return TDE_EINVAL;
-    if (t->batch.cache_pages > 0 && (!t->k_cache.data || !t->v_cache.data)) return TDE_EINVAL;
-    if (!lines_of_16(t->k_cache) || !lines_of_16(t->v_cache)) return TDE_EALIGN;
-    if (plan.workspace_bytes > 0) {
-        if (t->workspace == nullptr || t->workspace_bytes < plan.workspace_bytes) return TDE_EINVAL;
-        if ((reinterpret_cast<uintptr_t>(t->workspace) & 15u) != 0) return TDE_EALIGN;
-    }
     AttentionArgs a{};
-    a.q = static_cast<const char *>(t->q.data);
-    a.k = static_cast<const char *>(t->k_cache.data);
-    a.v = static_cast<const char *>(t->v_cache.data);
-    a.out = static_cast<char *>(t->out.data);
-    a.q_token = t->q.row_stride * 2;
-    a.q_head = t->q.head_stride * 2;
-    a.out_token = t->out.row_stride * 2;
-    a.out_head = t->out.head_stride * 2;
-    a.k_page = (uint32_t)(t->k_cache.page_stride * 2);
-    a.k_slot = (uint32_t)(t->k_cache.slot_stride * 2);
-    a.k_head = t->k_cache.head_stride * 2;
-    a.v_page = (uint32_t)(t->v_cache.page_stride * 2);
-    a.v_slot = (uint32_t)(t->v_cache.slot_stride * 2);
-    a.v_head = t->v_cache.head_stride * 2;
-    a.batch = device_batch(t->batch);
-    a.group = Divisor32((uint32_t)(t->q_heads / t->kv_heads));
-    a.kv_heads = Divisor32((uint32_t)t->kv_heads);
-    a.tokens = t->tokens;
-    a.dim = t->dim;
-    a.scale_log2 = t->scale * 1.4426950408889634f;
-    a.partial = static_cast<float *>(t->workspace);
-    a.zero_tail = t->zero_tail != 0;
-    return launch_attention(a, plan, t->dtype, static_cast<hipStream_t>(hip_stream));
+    int st = check_attention(t, false, &plan);
+    if (st != TDE_OK || t->tokens == 0) return st;
+    st = attention_args(t, plan, 2, a);
+    return st != TDE_OK ? st : launch_attention(a, plan, t->dtype, static_cast<hipStream_t>(hip_stream));
+}
+
+int tde_append_kv_fp4(const tde_append_fp4 *t, void *hip_stream) {
+    if (t == nullptr || t->reserved != 0) return TDE_EINVAL;
+    HeadRowsFp4Args a{};
+    bool nothing;
+    const int st = head_rows_args(&t->rows, true, 1, a, nothing);
+    if (st != TDE_OK) return st;
+    if (!fp4_dim_ok(t->rows.dim)) return TDE_ESHAPE;
+    if (t->rows.dim > TDE_FP4_MAX_DIM) return TDE_EHIDDEN;
+    const tde_cache *scales[] = {&t->k_scales, &t->v_scales};
+    for (int i = 0; i < 2; ++i) {
+        if (!cache_ok(*scales[i])) return TDE_ESHAPE;
+        a.scales[i] = static_cast<char *>(scales[i]->data);
+        a.scale_page[i] = scales[i]->page_stride;
+        a.scale_slot[i] = scales[i]->slot_stride;
+        a.scale_head[i] = scales[i]->head_stride;
+    }
+    if (nothing) return TDE_OK;
+    if (t->rows.kv_heads > 0 && t->rows.batch.cache_pages > 0 && (!t->k_scales.data || !t->v_scales.data)) return TDE_EINVAL;
+    a.most_exponent = t->rows.dtype == TDE_F16 ? 13 : 125;
+    return launch_head_rows_fp4(a, t->rows.dtype, static_cast<hipStream_t>(hip_stream));
+}
+
+int tde_paged_attention_fp4_workspace(const tde_attention_fp4 *t, int64_t *bytes) {
+    if (bytes == nullptr) return TDE_EINVAL;
+    AttentionPlan plan;
+    const int st = check_attention_fp4(t, &plan);
+    if (st != TDE_OK) return st;
+    *bytes = t->attention.tokens == 0 ? 0 : plan.workspace_bytes;
+    return TDE_OK;
+}
+
+int tde_paged_attention_fp4(const tde_attention_fp4 *t, void *hip_stream) {
+    AttentionPlan plan;
+    AttentionFp4Args a{};
+    int st = check_attention_fp4(t, &plan);
+    if (st != TDE_OK || t->attention.tokens == 0) return st;
+    st = attention_args(&t->attention, plan, 1, a);
+    if (st != TDE_OK) return st;
+    if (t->attention.batch.cache_pages > 0 && (!t->k_scales.data || !t->v_scales.data)) return TDE_EINVAL;
+    a.k_scales = static_cast<const char *>(t->k_scales.data);
+    a.v_scales = static_cast<const char *>(t->v_scales.data);
+    a.k_scale_page = (uint32_t)t->k_scales.page_stride;
+    a.k_scale_slot = (uint32_t)t->k_scales.slot_stride;
+    a.k_scale_head = t->k_scales.head_stride;
+    a.v_scale_page = (uint32_t)t->v_scales.page_stride;
+    a.v_scale_slot = (uint32_t)t->v_scales.slot_stride;
+    a.v_scale_head = t->v_scales.head_stride;
+    return launch_attention_fp4(a, plan, t->attention.dtype, static_cast<hipStream_t>(hip_stream));
+}
+
+int tde_unpack_fp4(const tde_unpack_fp4_rows *r, void *hip_stream) {
+    if (r == nullptr || r->reserved != 0) return TDE_EINVAL;
+    if (r->out_dtype != TDE_BF16 && r->out_dtype != TDE_F16 && r->out_dtype != TDE_F32) return TDE_EDTYPE;
+    if (!fp4_dim_ok(r->dim)) return TDE_ESHAPE;
+    if (r->dim > TDE_FP4_MAX_DIM) return TDE_EHIDDEN;
+    int64_t rows = 1;
+    UnpackArgs a{};
+    for (int i = 0; i < 3; ++i) {
+        if (r->sizes[i] < 0 || !stride_ok(r->code_strides[i]) || !stride_ok(r->scale_strides[i])) return TDE_ESHAPE;
+        a.code_stride[i] = r->code_strides[i];
+        a.scale_stride[i] = r->scale_strides[i];
+    }
+    for (int i = 0; i < 3; ++i) // none where any size is 0, whatever the others are
+        if (r->sizes[i] == 0) return TDE_OK;
+    for (int i = 0; i < 3; ++i) {
+        if (r->sizes[i] >= kMaxRows / rows) return TDE_ETOOBIG;
+        rows *= r->sizes[i];
+    }
+    const int64_t pieces = rows * (r->dim / 8);
+    if (pieces >= kMaxRows) return TDE_ETOOBIG;
+    if (!r->codes || !r->scales || !r->out) return TDE_EINVAL;
+    a.codes = reinterpret_cast<const char *>(r->codes);
+    a.scales = reinterpret_cast<const char *>(r->scales);
+    a.out = static_cast<char *>(r->out);
+    a.pieces = Divisor32((uint32_t)(r->dim / 8));
+    a.inner = Divisor32((uint32_t)r->sizes[2]);
+    a.middle = Divisor32((uint32_t)r->sizes[1]);
+    a.total = (uint32_t)pieces;
+    return launch_unpack_fp4(a, r->out_dtype, static_cast<hipStream_t>(hip_stream));
+}
+
+int tde_update_pages(const tde_page_update *u, void *hip_stream) {
+    if (u == nullptr || u->reserved != 0) return TDE_EINVAL;
+    if (u->seqs < 0 || u->seqs > (1 << 24) || u->table_pages < 0 || u->free_capacity < 0 || u->page_size < 1 || u->tokens < 0 || u->tokens >= kMaxRows - 256 ||
+        !stride_ok(u->table_stride))
+        return TDE_ESHAPE;
+    if ((int64_t)u->seqs * u->table_pages >= kMaxRows) return TDE_ETOOBIG;
+    if (!u->free_count || !u->q_starts || (u->seqs > 0 && (!u->kv_lens || !u->new_tokens)) || (u->seqs > 0 && u->table_pages > 0 && !u->page_table) ||
+        (u->free_capacity > 0 && !u->free_pages) || (u->tokens > 0 && (!u->positions || !u->slots)))
+        return TDE_EINVAL;
+    PageUpdateArgs a{};
+    a.table = u->page_table;
+    a.lens = u->kv_lens;
+    a.added = u->new_tokens;
+    a.kept = u->keep_lens;
+    a.stack = u->free_pages;
+    a.count = u->free_count;
+    a.starts = u->q_starts;
+    a.positions = u->positions;
+    a.slots = u->slots;
+    a.table_stride = u->table_stride;
+    a.tokens = (int32_t)u->tokens;
+    a.seqs = u->seqs;
+    a.width = u->table_pages;
+    a.capacity = u->free_capacity;
+    a.page = Divisor32((uint32_t)u->page_size);
+    return launch_page_update(a, static_cast<hipStream_t>(hip_stream));
 }
 
 } // extern "C"

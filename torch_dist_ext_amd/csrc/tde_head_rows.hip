@@ -14,49 +14,12 @@
 namespace tde {
 namespace block {
 
-// The token's place: its sequence's cache position and the slot's page.  position < 0: the row belongs to no sequence's range (it
-// lies in front of the first one or behind the last, or its sequence is shorter than its new tokens).
-struct Place {
-    int64_t position;
-    int32_t page, slot; // page < 0: not in the cache
-};
-
-__device__ __forceinline__ Place place_of(const PagedBatch &b, int64_t token, int lane) {
-    Place p{-1, -1, 0};
-    const int seq = __builtin_amdgcn_readfirstlane(sequence_of(b, token, lane));
-    if (seq >= b.seqs) return p;
-    const int64_t begin = b.starts[seq], end = b.starts[seq + 1], len = b.lens[seq];
-    if (token < begin) return p;
-    p.position = len - (end - begin) + (token - begin);
-    if (p.position < 0) return p;
-    if (p.position > 0x7fffffff) return p; // only where starts do not ascend
-    const uint32_t at = b.page.quotient((uint32_t)p.position);
-    p.slot = (int32_t)((uint32_t)p.position - at * b.page.d);
-    p.page = page_number(b, b.table + seq * b.table_stride, at);
-    return p;
-}
-
-__device__ __forceinline__ int64_t explicit_position(const HeadRowsArgs &a, int64_t token) {
-    return a.positions_wide ? ((const int64_t *)a.positions)[token] : (int64_t)((const int32_t *)a.positions)[token];
-}
-
 // Address of head `h` of class `cls` (0 query, 1 key, 2 value) in the outputs; null where the row is not stored.
 template <bool PAGED>
 __device__ __forceinline__ char *destination(const HeadRowsArgs &a, const Place &place, int64_t token, int cls, int h) {
     if (!PAGED || cls == 0) return a.out[cls] + token * a.out_token[cls] + h * a.out_head[cls];
     if (place.page < 0) return nullptr;
     return a.out[cls] + place.page * a.out_page[cls] + place.slot * a.out_token[cls] + h * a.out_head[cls];
-}
-
-// VE floats of the table; NaN where the position is not in it.
-template <int N>
-__device__ __forceinline__ void load_floats(const float *p, bool known, float (&x)[N]) {
-    Words<N * 4> w;
-#pragma unroll
-    for (int i = 0; i < N; ++i) w.w[i] = 0x7fc00000u;
-    if (known) w = load_words<N * 4>(p);
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __builtin_bit_cast(float, w.w[i]);
 }
 
 // A lane has two chunks of VE channels of a row: chunk p and its partner in the other half of the rotation, or, behind the rotated

@@ -33,6 +33,23 @@ struct AttentionArgs {
     bool zero_tail;        // rows of no sequence become zeros
 };
 
+// The same over caches in 4 bits: k and v are codes.
+struct AttentionFp4Args : AttentionArgs {
+    const char *k_scales, *v_scales;
+    int64_t k_scale_head, v_scale_head;
+    uint32_t k_scale_page, k_scale_slot, v_scale_page, v_scale_slot;
+};
+
+// What caches hold: numbers of the queries' type, or e2m1 codes with a scale for 32 channels.
+struct Held16 {
+    using Args = AttentionArgs;
+    static constexpr bool kFp4 = false;
+};
+struct HeldFp4 {
+    using Args = AttentionFp4Args;
+    static constexpr bool kFp4 = true;
+};
+
 struct AttentionPlan {
     int wide_dim;   // 64, 128, 256: what the head is padded to in registers and LDS
     int rows;       // rows (token x query head of a group) of a tile
@@ -45,7 +62,10 @@ struct AttentionPlan {
 };
 
 int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p);
+int plan_attention_rows(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, int least_rows, AttentionPlan *p);
+int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p);
 int launch_attention(AttentionArgs &a, const AttentionPlan &p, int dtype, hipStream_t s);
+int launch_attention_fp4(AttentionFp4Args &a, const AttentionPlan &p, int dtype, hipStream_t s);
 
 } // namespace block
 } // namespace tde
