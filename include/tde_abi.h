@@ -393,8 +393,8 @@ typedef struct tde_append_fp4 {
 } tde_append_fp4;
 int tde_append_kv_fp4(const tde_append_fp4 *append, void *hip_stream);
 
-/* As tde_paged_attention; keys and values enter as numbers of `dtype`: exact in bf16 (down to 2^-133), to 2^-25 below 2^-14 in fp16 and infinite beyond
-   65504.  Codes: data and strides multiples of 16 bytes (TDE_EALIGN); scales need no alignment; page and slot strides below 2^31 bytes (TDE_ESHAPE).
+/* As tde_paged_attention; keys and values enter as numbers of `dtype`: exact in bf16 (down to 2^-133); in fp16 to 2^-25 below 2^-14, and blocks
+   whose 6 it does not hold (scales from 141 on) are NaN.  Codes: data and strides multiples of 16 bytes (TDE_EALIGN); scales need no alignment; page and slot strides below 2^31 bytes (TDE_ESHAPE).
    The workspace is tde_paged_attention_fp4_workspace bytes. */
 typedef struct tde_attention_fp4 {
     tde_attention attention;

@@ -110,17 +110,18 @@ def test_every_scale_byte(tde, dtype, new):
     run(tde, batch, 4, 2, 64, dtype, seed=6, scale=0.02, parts=parts)
 
 
-def test_values_beyond_fp16_are_infinite(tde):
-    """What fp16 does not hold is an infinity for the rows that see it, and for no others."""
+@pytest.mark.parametrize("which", [1, 3], ids=["keys", "values"])
+def test_blocks_beyond_fp16_are_nan(tde, which):
+    """Blocks whose 6 fp16 does not hold are NaN for the rows that see them, and the largest that it holds are numbers."""
     for new in ([3], [90]):
         batch = Batch(new=new, lens=[150], page_size=16, seed=4)
         parts = held(batch, 1, 64, 7)
         j = 150 - new[0] + 1                                                       # the second new row's key
-        page, slot = batch.page_of(0, j), j % 16
-        parts[3][page, slot, 0, 1] = 127 + 14
-        parts[2][page, slot, 0, 16:] = 0x77                                         # 6 * 2^14
-        parts[2][page, slot, 0, 16] = 0xf1                                          # 0.5 * 2^14, -6 * 2^14
+        parts[which][batch.page_of(0, j), j % 16, 0, 1] = 127 + 14
+        parts[3][batch.page_of(0, 5), 5, 0, 0] = 127 + 13
         run(tde, batch, 2, 1, 64, torch.float16, seed=8, parts=parts)
+        parts[which][batch.page_of(0, j), j % 16, 0, 1] = 127 + 13
+        run(tde, batch, 2, 1, 64, torch.float16, seed=8, parts=parts, scale=1e-5)
 
 
 @pytest.mark.parametrize("new,lens", [([2, 1, 3], [90, 2000, 40]), ([70, 150, 3], [90, 200, 40])], ids=["decode", "chunks"])

@@ -137,7 +137,8 @@ int check_attention(const tde_attention *t, bool fp4, AttentionPlan *plan) {
     const int st = check_batch(t->batch);
     if (st != TDE_OK) return st;
     const int64_t capacity = (int64_t)t->batch.table_pages * t->batch.page_size;
-    return (fp4 ? plan_attention_fp4 : plan_attention)(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch.seqs, capacity, plan);
+    return fp4 ? plan_attention_fp4(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch, plan)
+               : plan_attention(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch.seqs, capacity, plan);
 }
 
 int check_attention_fp4(const tde_attention_fp4 *t, AttentionPlan *plan) {

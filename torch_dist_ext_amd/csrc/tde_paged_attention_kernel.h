@@ -59,10 +59,16 @@ struct Mfma<F16> {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
     }
     template <int BYTE>
-    static __device__ __forceinline__ uint32_t from_fp4(uint32_t codes, float scale) { // beyond 65504 infinite
+    static __device__ __forceinline__ uint32_t from_fp4(uint32_t codes, float scale) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, BYTE));
     }
 };
+// What a scale's byte counts as where codes become numbers of T: blocks whose 6 is no number of fp16 are NaN there.
+template <class T>
+__device__ __forceinline__ uint32_t read_scale(uint32_t e) {
+    return __is_same(T, F16) && e > 127 + 13 ? 255 : e;
+}
+
 __device__ __forceinline__ uint32_t load_byte(const char *p) { return *(const __attribute__((address_space(1))) uint8_t *)p; }
 // Eight codes as numbers of T; `scale` is a scale's byte.
 template <class T>
@@ -476,8 +482,8 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
             if (piece_row >= KT) return;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                *(u32x4 *)(lds + to + k_place(piece_row, piece * 4, j)) = from_fp4<T>(codes.k[j], codes.k_scale);
-                *(u32x4 *)(lds + to + TILE + v_place(piece_row, piece * 4, j)) = from_fp4<T>(codes.v[j], codes.v_scale);
+                *(u32x4 *)(lds + to + k_place(piece_row, piece * 4, j)) = from_fp4<T>(codes.k[j], read_scale<T>(codes.k_scale));
+                *(u32x4 *)(lds + to + TILE + v_place(piece_row, piece * 4, j)) = from_fp4<T>(codes.v[j], read_scale<T>(codes.v_scale));
             }
         }
     };
@@ -1038,9 +1044,8 @@ void launch_type(const typename C::Args &a, const AttentionPlan &p, uint32_t blo
     else launch_dim<T, C, 256>(a, p, blocks, s);
 }
 
-// The sizes of a plan, and its launch.
-template <class C>
-int launch_planned(typename C::Args &a, const AttentionPlan &p, int dtype, hipStream_t s) {
+// A plan's sizes into the arguments; returns the number of workgroups.
+[[maybe_unused]] uint32_t set_sizes(AttentionArgs &a, const AttentionPlan &p) {
     a.items = (int32_t)p.items;
     a.tiles = (int32_t)p.tiles;
     a.target = p.target;
@@ -1048,7 +1053,12 @@ int launch_planned(typename C::Args &a, const AttentionPlan &p, int dtype, hipSt
     a.capacity = (int32_t)std::min<int64_t>((int64_t)a.batch.table_pages * a.batch.page.d, 0x7fffff00);
     // the joins' items behind the partial results, which want 16-byte boundaries
     a.joins = reinterpret_cast<JoinItem *>(a.partial + p.items * a.kv_heads.d * p.rows * (p.wide_dim + 4));
-    const uint32_t blocks = (uint32_t)(p.items * a.kv_heads.d);
+    return (uint32_t)(p.items * a.kv_heads.d);
+}
+
+template <class C>
+int launch_planned(typename C::Args &a, const AttentionPlan &p, int dtype, hipStream_t s) {
+    const uint32_t blocks = set_sizes(a, p);
     if (dtype == TDE_BF16) launch_type<Bf16, C>(a, p, blocks, s);
     else launch_type<F16, C>(a, p, blocks, s);
     const hipError_t e = hipGetLastError();
