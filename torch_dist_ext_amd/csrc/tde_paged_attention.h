@@ -38,6 +38,9 @@ struct AttentionFp4Args : AttentionArgs {
     const char *k_scales, *v_scales;
     int64_t k_scale_head, v_scale_head;
     uint32_t k_scale_page, k_scale_slot, v_scale_page, v_scale_slot;
+    Divisor32 runners; // decode: workgroups that share out the keys of a key head
+    bool whole_tiles;  // decode: a tile each
+    int32_t most_each; // decode: units of a runner
 };
 
 // What caches hold: numbers of the queries' type, or e2m1 codes with a scale for 32 channels.
@@ -58,6 +61,8 @@ struct AttentionPlan {
     int64_t target;
     int32_t min_chunk;
     int join_waves; // wavefronts that join a row
+    int64_t runners, most_each; // caches in 4 bits, tiles of 16 rows
+    bool whole_tiles;
     int64_t workspace_bytes;
 };
 
