@@ -142,6 +142,18 @@ def test_blocks_that_are_nan(tde, new, lens, dim):
         run(tde, batch, 4, 2, dim, torch.float16, seed=11, parts=parts)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_behind_the_last_key_of_one_token(tde, dim):
+    """A tile of 64 rows that all see the same keys, in a page whose other slots are NaN."""
+    batch = Batch(new=[1, 1], lens=[67, 200], page_size=16, seed=6)
+    parts = held(batch, 1, dim, 15)
+    for b, length in enumerate(batch.lens):
+        parts[1][batch.page_of(b, length - 1), length % 16:] = 255
+        parts[3][batch.page_of(b, length - 1), length % 16:] = 255
+    run(tde, batch, 64, 1, dim, torch.bfloat16, seed=16, parts=parts)
+    run(tde, batch, 64, 1, dim, torch.float16, seed=16, parts=parts)
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 1, 70, 9]], ids=["decode", "chunks"])
 def test_pages_that_are_none(tde, new):
     batch = Batch(new=new, lens=[100, 700, 90, 64], page_size=16, seed=6)
@@ -231,6 +243,19 @@ def test_strided_rows_and_shared_caches(tde):
     rows[..., :32], rows[..., 35:37] = here[0], here[1]
     again = tde.paged_attention_fp4(q.cuda()[:, 2:6], rows[..., :32], rows[..., 35:37], rows[..., :32], rows[..., 35:37], *batch.on("cuda"))
     assert torch.equal(again, got)
+
+
+def test_starts_that_do_not_ascend(tde):
+    """What the rows get is unspecified; nothing outside the call's rows is touched, and the call ends."""
+    batch = Batch(new=[1] * 40, lens=[300] * 40, page_size=16, seed=12)
+    parts = on_gpu(held(batch, 2, 64, 3))
+    table, _, lens = batch.on("cuda")
+    q = randn((40, 4, 64), torch.bfloat16, 4).cuda()
+    for starts in ([0, 40] * 20 + [0], list(range(40, -1, -1)), [0] + [1 << 30, -5] * 20, [7] * 41):
+        whole = torch.full((60, 4, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+        tde.paged_attention_fp4_out(q, *parts, table, torch.tensor(starts, dtype=torch.int32, device="cuda"), lens, whole[10:50])
+        torch.cuda.synchronize()
+        assert bool((whole[:10] == 3).all()) and bool((whole[50:] == 3).all())
 
 
 def test_far_pages(tde):

@@ -437,54 +437,108 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
         lost = __builtin_amdgcn_ballot_w64(where.k == kNoPage);
         return false;
     };
-    // A cache in 4 bits goes by way of registers: a lane takes 32 channels of a key and of its value, which are numbers of T once they are in LDS.  The
-    // next tile's codes are on their way while a tile is worked on.
+    // A cache in 4 bits goes by way of registers: a lane takes 32 channels of a key and of its value, or of one of the two where lanes are enough for both, which are
+    // numbers of T once they are in LDS.  The next tile's codes are on their way while a tile is worked on.
     static_assert(!FP4 || SHARED, "wavefronts with keys of their own take codes another way");
-    constexpr int PIECES = D / 32; // of a row
-    static_assert(!FP4 || KT * PIECES <= 64 * WAVES, "one piece a lane");
+    constexpr int PIECES = D / 32;                                  // of a row
+    constexpr bool HALVES = FP4 && KT * PIECES * 2 <= 64 * WAVES;   // keys are the first half of the wavefronts', values the second's
+    static_assert(!FP4 || KT * PIECES == 64 * WAVES / (HALVES ? 2 : 1), "one piece a lane");
     struct Codes {
-        u32x4 k, v;
+        u32x4 k, v; // HALVES: k alone
         uint32_t k_scale, v_scale;
     };
-    [[maybe_unused]] Codes codes;
-    const int piece_row = (int)threadIdx.x / PIECES, piece = (int)threadIdx.x % PIECES; // lanes behind the tile's rows have none
-    [[maybe_unused]] const char *k_piece = nullptr, *v_piece = nullptr, *k_scale_piece = nullptr, *v_scale_piece = nullptr;
-    if constexpr (FP4) { // addresses of the lane, which leave scalar registers free
-        k_piece = k_base + piece * 16;
-        v_piece = v_base + piece * 16;
-        k_scale_piece = a.k_scales + kv_head * a.k_scale_head + piece;
-        v_scale_piece = a.v_scales + kv_head * a.v_scale_head + piece;
-        asm volatile("" : "+v"(k_piece), "+v"(v_piece), "+v"(k_scale_piece), "+v"(v_scale_piece));
-    }
+    [[maybe_unused]] Codes codes{};
+    [[maybe_unused]] const bool takes_values = HALVES && wave >= WAVES / 2;
+    constexpr int WAVE_ROWS = 64 / PIECES;
+    const int piece_row0 = (HALVES ? wave % (WAVES / 2) : wave) * WAVE_ROWS, piece_row = piece_row0 + lane / PIECES, piece = lane % PIECES;
+    [[maybe_unused]] const bool piece_there = piece * 32 < a.dim;
+    // What a wavefront loads from: keys' codes or, with HALVES, its own kind's; values' codes; their scales.
+    struct Held {
+        const char *codes, *scales;
+        uint32_t page, slot, scale_page, scale_slot;
+    };
+    const auto held = [&]([[maybe_unused]] bool values) -> Held {
+        if constexpr (FP4) {
+            return values ? Held{v_base, a.v_scales + kv_head * a.v_scale_head, a.v_page, a.v_slot, a.v_scale_page, a.v_scale_slot}
+                          : Held{k_base, a.k_scales + kv_head * a.k_scale_head, a.k_page, a.k_slot, a.k_scale_page, a.k_scale_slot};
+        }
+        return {};
+    };
+    // Where 16 keys lie in one page, and lanes' offsets hold 32 bits, a wavefront's rows (8, 16 or twice 16) have scalar addresses.
+    [[maybe_unused]] const bool scalar_rows = FP4 && a.batch.page.d % 16 == 0 && (a.k_slot | a.v_slot) < 1u << 27 && a.batch.cache_pages > 0;
     const auto fetch = [&]([[maybe_unused]] int32_t key0, [[maybe_unused]] uint64_t &lost) { // look_up has been called for the tile
         if constexpr (FP4) {
-            const int64_t key = (int64_t)key0 + lane;
-            const bool there = (KT == 64 || lane < KT) && key < until;
-            const uint32_t at = a.batch.page.quotient((uint32_t)(there ? key : key0));
-            const int32_t entry = __shfl(entries, (int)(at - (uint32_t)window));
-            const int32_t page = there ? entry : -1;
-            lost = __builtin_amdgcn_ballot_w64(there && page < 0);
-            const uint32_t of_page = (uint32_t)__shfl(page, piece_row & (KT - 1)), of_at = (uint32_t)__shfl((int)at, piece_row & (KT - 1));
-            const uint32_t slot = (uint32_t)key0 + piece_row - of_at * a.batch.page.d;
-            codes = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}, 0, 0}; // zeros where there is no key: no weight would keep what lies there from the sums
-            if (piece_row < KT && (int32_t)of_page >= 0 && piece * 32 < a.dim) {
-                const Words<16> k = load_words<16>(k_piece + (uint64_t)of_page * a.k_page + (uint64_t)slot * a.k_slot);
-                const Words<16> v = load_words<16>(v_piece + (uint64_t)of_page * a.v_page + (uint64_t)slot * a.v_slot);
-                codes.k = u32x4{k.w[0], k.w[1], k.w[2], k.w[3]};
-                codes.v = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
-                codes.k_scale = load_byte(k_scale_piece + (uint64_t)of_page * a.k_scale_page + (uint64_t)slot * a.k_scale_slot);
-                codes.v_scale = load_byte(v_scale_piece + (uint64_t)of_page * a.v_scale_page + (uint64_t)slot * a.v_scale_slot);
+            const uint32_t first = a.batch.page.quotient((uint32_t)key0) - (uint32_t)window;
+            const uint32_t end = a.batch.page.quotient((uint32_t)key0 + KT - 1) - (uint32_t)window;
+            uint32_t of_page = 0, of_slot = 0; // of the lane's row
+            bool there = true;
+            lost = 0;
+            const bool all_there = scalar_rows && end < 64 && (missing >> first << first << (63 - end)) == 0;
+            if (!all_there) {
+                const int64_t key = (int64_t)key0 + lane;
+                const bool key_there = (KT == 64 || lane < KT) && key < until;
+                const uint32_t at = a.batch.page.quotient((uint32_t)(key_there ? key : key0));
+                const int32_t entry = __shfl(entries, (int)(at - (uint32_t)window));
+                const int32_t page = key_there ? entry : -1;
+                lost = __builtin_amdgcn_ballot_w64(key_there && page < 0);
+                of_page = (uint32_t)__shfl(page, piece_row);
+                of_slot = (uint32_t)key0 + piece_row - (uint32_t)__shfl((int)at, piece_row) * a.batch.page.d;
+                there = (int32_t)of_page >= 0;
+                codes = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}, 0, 0}; // zeros where there is no key: no weight would keep what lies there from the sums
+            }
+            const auto one = [&](const Held &h, u32x4 &to, uint32_t &to_scale) {
+                const char *from, *scale_from;
+                if (all_there) {
+                    // keys behind the last one may be there, whatever they hold: their weights are 0, and where they are not finite they are taken out as
+                    // values are that not all rows see
+                    const auto at_key = [&](uint32_t key, const char *&codes_at, const char *&scales_at) {
+                        const uint32_t page = a.batch.page.quotient(key), slot = key - page * a.batch.page.d;
+                        const uint32_t number = (uint32_t)__builtin_amdgcn_readlane(entries, (int)(page - (uint32_t)window));
+                        codes_at = h.codes + ((uint64_t)number * h.page + (uint64_t)slot * h.slot);
+                        scales_at = h.scales + ((uint64_t)number * h.scale_page + (uint64_t)slot * h.scale_slot);
+                    };
+                    at_key((uint32_t)key0 + piece_row0, from, scale_from);
+                    if constexpr (WAVE_ROWS > 16) {
+                        const char *second, *scale_second;
+                        at_key((uint32_t)key0 + piece_row0 + 16, second, scale_second);
+                        from = lane < 32 ? from : second;
+                        scale_from = lane < 32 ? scale_from : scale_second;
+                    }
+                    const uint32_t row = (uint32_t)(lane / PIECES) & 15u;
+                    from += row * h.slot + (piece_there ? piece : 0) * 16;
+                    scale_from += row * h.scale_slot + (piece_there ? piece : 0);
+                } else {
+                    from = h.codes + ((uint64_t)of_page * h.page + (uint64_t)of_slot * h.slot + piece * 16);
+                    scale_from = h.scales + ((uint64_t)of_page * h.scale_page + (uint64_t)of_slot * h.scale_slot + piece);
+                }
+                if (all_there || (there && piece_there)) {
+                    const Words<16> w = load_words<16>(from);
+                    to = u32x4{w.w[0], w.w[1], w.w[2], w.w[3]};
+                    to_scale = load_byte(scale_from);
+                }
+            };
+            if constexpr (HALVES) {
+                one(held(takes_values), codes.k, codes.k_scale);
+            } else {
+                one(held(false), codes.k, codes.k_scale);
+                one(held(true), codes.v, codes.v_scale);
             }
         }
     };
-    const auto put = [&]([[maybe_unused]] uint32_t to) {
+    // Part `i` of PARTS of the codes that were fetched into LDS as numbers.
+    constexpr int PARTS = HALVES ? 4 : 8;
+    // When: while the matrix units work on the tile's scores, if registers allow for it (4096 rows behind 4096 in heads of 128: 436 us, ahead of them 449).  Heads of 64
+    // keep four workgroups a unit without it (24 sequences of up to 512 rows 65 us, with it three and 74).
+    [[maybe_unused]] constexpr bool WITH_SCORES = D > 64;
+    const auto put = [&]([[maybe_unused]] uint32_t to, [[maybe_unused]] int i) {
         if constexpr (FP4) {
-            if (piece_row >= KT) return;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                *(u32x4 *)(lds + to + k_place(piece_row, piece * 4, j)) = from_fp4<T>(codes.k[j], read_scale<T>(codes.k_scale));
-                *(u32x4 *)(lds + to + TILE + v_place(piece_row, piece * 4, j)) = from_fp4<T>(codes.v[j], read_scale<T>(codes.v_scale));
-            }
+            const bool second = !HALVES && i >= 4;
+            const u32x4 from = second ? codes.v : codes.k;
+            const uint32_t scale = second ? codes.v_scale : codes.k_scale;
+            const bool values = HALVES ? takes_values : second;
+            const int at = values ? TILE + v_place(piece_row, piece * 4, i & 3) : k_place(piece_row, piece * 4, i & 3);
+            // channels that the head does not have are zeros
+            *(u32x4 *)(lds + to + at) = from_fp4<T>(piece_there ? from[i & 3] : 0, piece_there ? read_scale<T>(scale) : 0);
         }
     };
     constexpr std::true_type kYes{};
@@ -501,7 +555,8 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
         look_up(first_key);
         if constexpr (FP4) {
             fetch(first_key, lost_next);
-            put(buf);
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) put(buf, i);
             if ((int64_t)first_key + TILE_STEP < until) {
                 look_up(first_key + TILE_STEP);
                 fetch(first_key + TILE_STEP, lost_fetched);
@@ -554,9 +609,10 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
         const uint64_t lost = lost_next; // keys without a page
         if constexpr (FP4) {
             sync();
-            if (more) {
-                put(buf ^ (2 * TILE));
-                lost_next = lost_fetched;
+            lost_next = lost_fetched;
+            if (!WITH_SCORES && more) {
+#pragma unroll
+                for (int i = 0; i < PARTS; ++i) put(buf ^ (2 * TILE), i);
                 if (next + TILE_STEP < until) {
                     look_up((int32_t)next + TILE_STEP);
                     fetch((int32_t)next + TILE_STEP, lost_fetched);
@@ -602,10 +658,21 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
 #pragma unroll
                     for (int u = 0; u < U; ++u) s[n][kb] = Mfma<T>::mul(kf[unit & 1][u], q[n][st + u], s[n][kb]);
                 }
+                // the next tile's numbers, which the products leave time for (behind the last tile old ones, which nothing reads)
+                if constexpr (FP4 && WITH_SCORES) {
+#pragma unroll
+                    for (int i = unit * PARTS / UNITS; i < (unit + 1) * PARTS / UNITS; ++i) put(buf ^ (2 * TILE), i);
+                }
+            }
+        }
+        if constexpr (FP4 && WITH_SCORES) {
+            if (next + TILE_STEP < until) {
+                look_up((int32_t)next + TILE_STEP);
+                fetch((int32_t)next + TILE_STEP, lost_fetched);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (lost != 0) {
+        if (FP4 ? __builtin_expect(lost != 0, 0) : lost != 0) {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -716,7 +783,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
         }
         // whether values that not all rows see hold an infinity or a NaN
         bool poisoned = false;
-        if (std::min<int64_t>((int64_t)key0 + KT, until) > lowest) {
+        if ((FP4 ? (int64_t)key0 + KT : std::min<int64_t>((int64_t)key0 + KT, until)) > lowest) { // (of 4 bits, what lies behind the last key is there)
             // an exponent of ones plus one at its lowest bit carries out of its field; the field's neighbours are masked off before
             constexpr uint32_t E = Mfma<T>::kExponent, LOW = E & (~E + 1u);
             uint32_t carried = 0;
