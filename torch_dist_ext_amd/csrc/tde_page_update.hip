@@ -1,17 +1,23 @@
 // A step's lengths, page tables and slot maps: sequences shrink, their pages go back on the stack, sequences grow with pages from it.
 //
 // All of it is sums over the sequences in order: a page that goes back or comes has a number among the call's, and with it its place on the stack; a row has
-// its number among the rows.  One workgroup does it, a sequence a thread, THREADS of them at a time, with sums over the threads; pages and rows, of
-// which a sequence has any number, are then shared out evenly, and each looks up whose it is in the sums.  A workgroup sees what it has written behind a
-// barrier, so nothing has to wait for another launch; only the maps of many rows are a launch of their own, over all units.
+// its number among the rows.  One workgroup does it, a sequence a thread, with sums over the threads; pages and rows, of which a sequence has any number,
+// are then shared out evenly, and each looks up whose it is in the sums.  A workgroup sees what it has written behind a barrier, so nothing has to wait
+// for another launch; only the maps of many rows are a launch of their own, over all units.
 //
-// Bound by latency: a chain of a load, four sums over the workgroup, a load from the stack, one from the table.
+// Bound by latency: loads of the lengths, a sum over the workgroup (a second one if something is missing), a load from the stack, one from the table.  64
+// sequences of 4 rows take 4.2 us in a captured graph, where an empty kernel takes 1.6.
 #include "tde_page_update.h"
+
+#include <type_traits>
 
 namespace tde {
 namespace block {
 
 namespace {
+
+template <int N>
+using Is = std::integral_constant<int, N>;
 
 __device__ __forceinline__ uint32_t add_up_to(uint32_t x, uint32_t y, uint32_t most) { return min(x + y, most); } // x, y <= most < 2^31 + 1
 
@@ -50,7 +56,7 @@ __device__ __forceinline__ Sums sums_over_threads(uint32_t x0, uint32_t x1, uint
 }
 
 // The first of n ascending sums that exceeds e, which the last one does.
-__device__ __forceinline__ int owner_of(const uint32_t *sums, int n, uint32_t e) {
+__device__ __forceinline__ int owner_of(const uint32_t *sums, int n, uint32_t e) { // n >= 1
     int low = 0;
     while (n > 1) {
         const int half = n >> 1;
@@ -80,8 +86,10 @@ __device__ __forceinline__ Lengths lengths_of(const PageUpdateArgs &a, int seq) 
 
 } // namespace
 
-template <int THREADS, bool MAPS>
-__global__ void __launch_bounds__(THREADS) page_update_kernel(const PageUpdateArgs a) {
+// Any number of sequences, THREADS at a time.
+template <bool MAPS>
+__global__ void __launch_bounds__(1024) page_update_kernel(const PageUpdateArgs a) {
+    constexpr int THREADS = 1024;
     __shared__ uint32_t parts[THREADS / 64][2], pages_upto[THREADS], rows_upto[THREADS], first_page[THREADS], keep_of[THREADS];
     constexpr uint32_t kAny = 0x80000000u;
     const int tid = threadIdx.x;
@@ -169,6 +177,102 @@ __global__ void __launch_bounds__(THREADS) page_update_kernel(const PageUpdateAr
         }
 }
 
+// The same for no more sequences than threads: one sum over them says what goes back, what is asked for and, unless something is missing, what is given.
+template <int THREADS, bool MAPS>
+__global__ void __launch_bounds__(THREADS) page_update_once_kernel(const PageUpdateArgs a) {
+    constexpr int WAVES = THREADS / 64;
+    constexpr uint32_t kAny = 0x7fffffffu;
+    __shared__ uint32_t parts[2][WAVES][3], back_upto[THREADS], pages_upto[THREADS], rows_upto[THREADS], first_page[THREADS], keep_of[THREADS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool there_is = tid < a.seqs;
+    const Lengths l = there_is ? lengths_of(a, tid) : Lengths{};
+    const uint32_t more = there_is ? (uint32_t)max(a.added[tid], 0) : 0;
+    const uint32_t before = (uint32_t)min(max(*a.count, 0), a.capacity);
+    const uint32_t then = l.keep + more; // below 2^32
+    const uint32_t need_pages = then <= kAny ? pages_of(a, then) : kAny;
+    const bool fits = need_pages <= (uint32_t)a.width;
+    const uint32_t need = fits && more != 0 ? need_pages - l.kept_pages : 0;
+
+    // Sums over the threads up to each one and of all, no more than kAny.
+    struct Three {
+        uint32_t v[3];
+    };
+    const auto sums = [&](Three &upto, Three &all, uint32_t(&of_waves)[WAVES][3]) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const auto add = [&](auto control, auto rows) {
+                upto.v[k] = add_up_to(upto.v[k], (uint32_t)__builtin_amdgcn_update_dpp(0, (int)upto.v[k], decltype(control)::value, decltype(rows)::value, 0xf, false), kAny);
+            };
+            // from 1, 2, 4, 8 lanes below, of rows of 16; a row's last lane to the next row, the second one's to the upper half
+            add(Is<0x111>{}, Is<0xf>{}), add(Is<0x112>{}, Is<0xf>{}), add(Is<0x114>{}, Is<0xf>{}), add(Is<0x118>{}, Is<0xf>{});
+            add(Is<0x142>{}, Is<0xa>{}), add(Is<0x143>{}, Is<0xc>{});
+            if (lane == 63) of_waves[wave][k] = upto.v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            uint32_t below = 0, sum = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                below = w == wave ? sum : below;
+                sum = add_up_to(sum, of_waves[w][k], kAny);
+            }
+            upto.v[k] = add_up_to(upto.v[k], below, kAny);
+            all.v[k] = sum;
+        }
+    };
+    Three upto{{l.had_pages - l.kept_pages, need, fits ? more : 0}}, all;
+    sums(upto, all, parts[0]);
+    const uint32_t returned = all.v[0], back = upto.v[0], there = min(before + returned, (uint32_t)a.capacity);
+    bool served = fits;
+    if (all.v[1] > there || all.v[2] > (uint32_t)a.tokens) { // some wait
+        served = fits && (need == 0 || upto.v[1] <= there) && upto.v[2] <= (uint32_t)a.tokens;
+        upto = Three{{0, served ? need : 0, served ? more : 0}};
+        sums(upto, all, parts[1]);
+    }
+    back_upto[tid] = back;
+    pages_upto[tid] = upto.v[1];
+    rows_upto[tid] = upto.v[2];
+    first_page[tid] = l.kept_pages;
+    keep_of[tid] = l.keep;
+    if (there_is) {
+        a.lens[tid] = (int32_t)(l.keep + (served ? more : 0));
+        a.starts[tid + 1] = (int32_t)upto.v[2];
+    }
+    const uint32_t taken = all.v[1], rows = all.v[2];
+    if (tid == 0) {
+        a.starts[0] = 0;
+        *a.count = (int32_t)(there - taken);
+    }
+    __syncthreads();
+    for (uint32_t e = tid; e < returned; e += THREADS) {
+        const int at = owner_of(back_upto, a.seqs, e);
+        const uint32_t page = first_page[at] + (e - (at == 0 ? 0 : back_upto[at - 1])), place = before + returned - 1 - e;
+        if (place < (uint32_t)a.capacity) a.stack[place] = a.table[at * a.table_stride + page];
+    }
+    __syncthreads();
+    for (uint32_t e = tid; e < taken; e += THREADS) {
+        const int at = owner_of(pages_upto, a.seqs, e);
+        const uint32_t page = first_page[at] + (e - (at == 0 ? 0 : pages_upto[at - 1]));
+        a.table[at * a.table_stride + page] = a.stack[there - 1 - e];
+    }
+    if constexpr (MAPS) {
+        __syncthreads();
+        for (uint32_t t = tid; t < (uint32_t)a.tokens; t += THREADS) {
+            int32_t position = -1;
+            int64_t slot = -1;
+            if (t < rows) {
+                const int at = owner_of(rows_upto, a.seqs, t);
+                const uint32_t p = keep_of[at] + (t - (at == 0 ? 0 : rows_upto[at - 1])), page = a.page.quotient(p);
+                position = (int32_t)p;
+                slot = (int64_t)a.table[at * a.table_stride + page] * a.page.d + (p - page * a.page.d);
+            }
+            a.positions[t] = position;
+            a.slots[t] = slot;
+        }
+    }
+}
+
 // Positions and slots of many rows, after the tables: a row a thread.
 __global__ void __launch_bounds__(256) page_maps_kernel(const PageUpdateArgs a) {
     const uint32_t t = blockIdx.x * 256 + threadIdx.x;
@@ -195,10 +299,14 @@ __global__ void __launch_bounds__(256) page_maps_kernel(const PageUpdateArgs a) 
 }
 
 int launch_page_update(const PageUpdateArgs &a, hipStream_t s) {
+    // Threads: 64 sequences with 4 rows each take 4.2 us with 256 and 5.3 with 1024; 200 with 16 take 9.0 and 6.6.  Maps in a launch of their own: 64
+    // sequences with 128 rows take 8.1 us, 7.8 without; 16 with 1024 take 7.4, 8.7 without.
     const bool maps = a.tokens > 4096;
-    if (maps) page_update_kernel<1024, false><<<1, 1024, 0, s>>>(a);
-    else if (a.seqs > 256 || a.tokens > 1024) page_update_kernel<1024, true><<<1, 1024, 0, s>>>(a);
-    else page_update_kernel<256, true><<<1, 256, 0, s>>>(a);
+    if (a.seqs <= 256 && a.tokens <= 512) page_update_once_kernel<256, true><<<1, 256, 0, s>>>(a);
+    else if (a.seqs <= 1024 && !maps) page_update_once_kernel<1024, true><<<1, 1024, 0, s>>>(a);
+    else if (a.seqs <= 1024) page_update_once_kernel<1024, false><<<1, 1024, 0, s>>>(a);
+    else if (!maps) page_update_kernel<true><<<1, 1024, 0, s>>>(a);
+    else page_update_kernel<false><<<1, 1024, 0, s>>>(a);
     if (maps) page_maps_kernel<<<((uint32_t)a.tokens + 255) / 256, 256, 0, s>>>(a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? TDE_OK : hip_failed(e);
