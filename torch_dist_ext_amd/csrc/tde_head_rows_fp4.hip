@@ -11,7 +11,9 @@
 // what is left is cut to 32 bits with its last bit set where anything was cut off: no border of codes, which have three significant bits, lies between.  The
 // hardware's conversion then rounds once.
 //
-// Bound by memory: a row is read once, 16 bytes a lane, with its partner in the rotation, which comes from the nearest cache.
+// A row is read once, 16 bytes a lane, with its partner in the rotation, which comes from the nearest cache.  8192 tokens of 32 + 2 * 8 heads of 128
+// fp16 channels, a half of them rotated, take 42 us, 4.2 TB/s: vector instructions take 27 us of it and the wait for a token's sequence, place and
+// cosines the rest; queries written past the caches and rows of one kind to a wavefront's instruction brought it there from 60.
 #include "tde_block.h"
 #include "tde_head_rows.h"
 
@@ -20,7 +22,8 @@ namespace block {
 
 namespace {
 
-__device__ __forceinline__ double sum_over_lanes(double x, int log2) {
+template <class A>
+__device__ __forceinline__ A sum_over_lanes(A x, int log2) {
     for (int m = 0; m < log2; ++m) x += __shfl_xor(x, 1 << m);
     return x;
 }
@@ -37,14 +40,16 @@ __device__ __forceinline__ float cut(double x) {
 __device__ __forceinline__ float multiply_add(float x, float y, float z) { return __builtin_fmaf(x, y, z); }
 __device__ __forceinline__ double multiply_add(double x, double y, double z) { return __builtin_fma(x, y, z); }
 
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
 // Norm and rotation of a lane's eight channels x; y are their partners in the rotation, c and s (with the sign that the channel takes it) theirs.
 template <class A>
 struct Channels {
     A x[8], y[8];
 };
-template <class A>
+template <bool WHOLE, class A>
 __device__ __forceinline__ void norm_and_turn(Channels<A> &v, bool normed, const float (&gx)[8], const float (&gy)[8], int dim, float eps, int lanes_log2,
-                                              uint32_t turned, const float (&c)[8], const float (&s)[8]) {
+                                              uint32_t turned, f32x8 c, f32x8 s) {
     if (normed) {
         A sq = 0;
 #pragma unroll
@@ -59,14 +64,15 @@ __device__ __forceinline__ void norm_and_turn(Channels<A> &v, bool normed, const
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if ((turned >> i) & 1) v.x[i] = multiply_add(v.x[i], (A)c[i], v.y[i] * (A)s[i]);
+        if (WHOLE ? turned != 0 : ((turned >> i) & 1) != 0) v.x[i] = multiply_add(v.x[i], (A)c[i], v.y[i] * (A)s[i]);
 }
 
 } // namespace
 
-// A lane has eight channels, four neighbouring lanes a block; rows of a token share a wavefront.
+// A lane has eight channels of R rows of one token, which share their cosines, sines, gammas and place; four neighbouring lanes have a block.  As many
+// rows as a wavefront has at once are of one kind: queries, keys or values, so that nothing but the row's head differs between lanes.
 // WHOLE: chunks of eight channels lie in one half of the rotation, or behind it.
-template <class T, bool INTERLEAVED, bool WHOLE>
+template <class T, bool INTERLEAVED, bool WHOLE, int R>
 __global__ void __launch_bounds__(256) head_rows_fp4_kernel(const HeadRowsFp4Args a) {
     constexpr int BYTES = 8 * T::kBytes;
     const int lane = threadIdx.x & 63;
@@ -74,123 +80,171 @@ __global__ void __launch_bounds__(256) head_rows_fp4_kernel(const HeadRowsFp4Arg
     const uint32_t row = a.waves_per_token.quotient(wave);
     const int64_t token = row;
     if (token >= a.tokens) return;
-    const int part = (int)(wave - row * a.waves_per_token.d);
+    const int round = (int)(wave - row * a.waves_per_token.d) * R;
     const int place = lane & ((1 << a.lanes_log2) - 1), d0 = place * 8;
     const bool has = d0 < a.dim;
-    int h = part * (64 >> a.lanes_log2) + (lane >> a.lanes_log2);
-    const bool there = h < a.heads[0] + a.heads[1] + a.heads[2];
-    const int cls = h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2);
-    h -= cls == 0 ? 0 : (cls == 1 ? a.heads[0] : a.heads[0] + a.heads[1]);
-    const char *src = cls == 0 ? a.in[0] : (cls == 1 ? a.in[1] : a.in[2]);
-    src += token * (cls == 0 ? a.in_token[0] : (cls == 1 ? a.in_token[1] : a.in_token[2]));
-    src += h * (cls == 0 ? a.in_head[0] : (cls == 1 ? a.in_head[1] : a.in_head[2]));
-
-    // Partners.  Not interleaved: the same channels of the rotation's other half, which are one chunk where halves are whole ones.
     const int rot = 2 * a.half;
-    const bool apart = !INTERLEAVED && cls != 2 && there && has && d0 < rot;
+    // Partners.  Not interleaved: the same channels of the rotation's other half, which are one chunk where halves are whole ones.
+    const bool turned_apart = !INTERLEAVED && WHOLE && d0 < rot;
     const int to_partner = d0 < a.half ? a.half : -a.half;
-    Words<BYTES> own{}, other{};
-    if (there && has) own = load_words<BYTES>(src + d0 * T::kBytes);
-    if (WHOLE && apart) other = load_words<BYTES>(src + (d0 + to_partner) * T::kBytes);
+
+    Words<BYTES> own[R], other[R];
+    const char *source[R];
+    int cls[R], head[R]; // query, key, value; -1: no row
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int of_q = a.rounds[0], of_k = a.rounds[1];
+        cls[r] = round + r < of_q ? 0 : (round + r < of_q + of_k ? 1 : 2);
+        const int h = ((round + r - (cls[r] == 0 ? 0 : (cls[r] == 1 ? of_q : of_q + of_k))) << (6 - a.lanes_log2)) + (lane >> a.lanes_log2);
+        const bool there = h < (cls[r] == 0 ? a.heads[0] : (cls[r] == 1 ? a.heads[1] : a.heads[2])) && has;
+        head[r] = there ? h : -1;
+        const auto &late = arguments_again<HeadRowsFp4Args>();
+        source[r] = late.in[cls[r]] + token * late.in_token[cls[r]] + h * late.in_head[cls[r]];
+        own[r] = Words<BYTES>{};
+        if (there) own[r] = load_words<BYTES, (R > 1)>(source[r] + d0 * T::kBytes);
+        if constexpr (!INTERLEAVED && WHOLE) {
+            other[r] = Words<BYTES>{};
+            if (there && turned_apart && cls[r] != 2) other[r] = load_words<BYTES>(source[r] + (d0 + to_partner) * T::kBytes);
+        }
+    }
 
     const Place where = place_of(a.batch, token, lane);
     const int64_t position = a.positions != nullptr ? explicit_position(a, token) : where.position;
     const bool known = position >= 0 && position < a.table_rows;
     const float *const row_of = a.cos_sin + (known ? position : 0) * a.table_stride;
-    const char *const gamma = cls == 2 ? nullptr : (cls == 0 ? a.gamma[0] : a.gamma[1]);
 
-    float x[8], y[8], gx[8] = {}, gy[8] = {}, c[8] = {}, s[8] = {};
-    widen_all<T, 8>(own, x);
-    widen_all<T, 8>(other, y);
+    // Cosines and sines (with the sign that the channel takes them) of the lane's channels.
+    f32x8 c = {}, s = {};
     uint32_t turned = 0; // channels that are rotated, a bit each
-    if (there && has && cls != 2) {
-        if (gamma != nullptr) widen_all<T, 8>(load_words<BYTES>(gamma + d0 * T::kBytes), gx);
-        if constexpr (!WHOLE) { // channel by channel
+    if constexpr (!WHOLE) {
+        for (int i = 0; i < 8; ++i) {
+            const int d = d0 + i;
+            if (d >= rot) break;
+            const bool first = INTERLEAVED ? (d & 1) == 0 : d < a.half;
+            const int j = INTERLEAVED ? d >> 1 : (first ? d : d - a.half);
+            const float sine = known ? row_of[a.half + j] : __builtin_nanf("");
+            c[i] = known ? row_of[j] : __builtin_nanf("");
+            s[i] = first ? -sine : sine;
+            turned |= 1u << i;
+        }
+    } else if (d0 < rot) {
+        turned = 0xff;
+        if constexpr (INTERLEAVED) {
+            float cosines[4], sines[4];
+            load_floats(row_of + d0 / 2, known, cosines);
+            load_floats(row_of + a.half + d0 / 2, known, sines);
+#pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int d = d0 + i;
-                if (d >= rot) break;
-                const bool first = INTERLEAVED ? (d & 1) == 0 : d < a.half;
-                const int j = INTERLEAVED ? d >> 1 : (first ? d : d - a.half), partner = INTERLEAVED ? d ^ 1 : (first ? d + a.half : d - a.half);
-                const float sine = known ? row_of[a.half + j] : __builtin_nanf("");
-                y[i] = load_element<T>(src + partner * T::kBytes);
-                if (gamma != nullptr) gy[i] = load_element<T>(gamma + partner * T::kBytes);
-                c[i] = known ? row_of[j] : __builtin_nanf("");
-                s[i] = first ? -sine : sine;
-                turned |= 1u << i;
+                c[i] = cosines[i >> 1];
+                s[i] = (i & 1) == 0 ? -sines[i >> 1] : sines[i >> 1];
             }
-        } else if (d0 < rot) {
-            turned = 0xff;
+        } else {
+            const int j = d0 < a.half ? d0 : d0 - a.half;
+            float cosines[8], sines[8];
+            load_floats(row_of + j, known, cosines);
+            load_floats(row_of + a.half + j, known, sines);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = cosines[i];
+                s[i] = d0 < a.half ? -sines[i] : sines[i];
+            }
+        }
+    }
+    const auto gammas_at = [&](const char *from, int d, bool wanted) {
+        Words<BYTES> w{};
+        if (from != nullptr && has && wanted) w = load_words<BYTES>(from + d * T::kBytes);
+        return w;
+    };
+    constexpr int K = R > 1 ? 1 : 0; // gammas of queries and of keys, or of the only row
+    Words<BYTES> gamma[K + 1], other_gamma[K + 1];
+#pragma unroll
+    for (int i = 0; i <= K; ++i) {
+        const char *const of = R > 1 ? a.gamma[i] : (cls[0] == 0 ? a.gamma[0] : (cls[0] == 1 ? a.gamma[1] : nullptr));
+        gamma[i] = gammas_at(of, d0, true);
+        other_gamma[i] = gammas_at(of, d0 + to_partner, turned_apart);
+    }
+
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float x[8];
+        widen_all<T, 8>(own[r], x);
+        const auto norm_and_turn_row = [&](auto &v, const char *from, const Words<BYTES> &own_gamma, const Words<BYTES> &other_gamma) {
+            float y[8] = {}, gx[8], gy[8];
+            if constexpr (!INTERLEAVED && WHOLE) widen_all<T, 8>(other[r], y);
+            widen_all<T, 8>(own_gamma, gx);
+            widen_all<T, 8>(other_gamma, gy);
             if constexpr (INTERLEAVED) {
-                float cosines[4], sines[4];
-                load_floats(row_of + d0 / 2, known, cosines);
-                load_floats(row_of + a.half + d0 / 2, known, sines);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     y[i] = x[i ^ 1];
                     gy[i] = gx[i ^ 1];
-                    c[i] = cosines[i >> 1];
-                    s[i] = (i & 1) == 0 ? -sines[i >> 1] : sines[i >> 1];
                 }
-            } else {
-                if (gamma != nullptr) widen_all<T, 8>(load_words<BYTES>(gamma + (d0 + to_partner) * T::kBytes), gy);
-                const int j = d0 < a.half ? d0 : d0 - a.half;
-                load_floats(row_of + j, known, c);
-                load_floats(row_of + a.half + j, known, s);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s[i] = d0 < a.half ? -s[i] : s[i];
+            } else if constexpr (!WHOLE) { // one by one
+                if (head[r] >= 0)
+                    for (int i = 0; i < 8; ++i) {
+                        if (((turned >> i) & 1) == 0) break;
+                        const int partner = d0 + i < a.half ? d0 + i + a.half : d0 + i - a.half;
+                        y[i] = load_element<T>(source[r] + partner * T::kBytes);
+                        if (from != nullptr) gy[i] = load_element<T>(from + partner * T::kBytes);
+                    }
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v.x[i] = x[i];
+                v.y[i] = y[i];
+            }
+            norm_and_turn<WHOLE>(v, from != nullptr, gx, gy, a.dim, a.eps, a.lanes_log2, turned, c, s);
+        };
+        if (cls[r] == 0) {
+            Channels<float> v;
+            norm_and_turn_row(v, a.gamma[0], gamma[0], other_gamma[0]);
+            if (head[r] >= 0) {
+                Words<BYTES> out = narrow_all<T, 8>(v.x);
+                if (where.position < 0) out = Words<BYTES>{};
+                store_words<BYTES, (R > 1)>(a.out[0] + token * a.out_token[0] + head[r] * a.out_head[0] + d0 * T::kBytes, out);
+            }
+            continue;
         }
-    }
-
-    if (cls == 0) {
-        Channels<float> v;
+        if (cls[r] == 1) {
+            if constexpr (R > 1 && !INTERLEAVED) { // as 64-bit numbers these are made anew for each row: kept, they would take the registers of more wavefronts
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v.x[i] = x[i];
-            v.y[i] = y[i];
+                for (int i = 0; i < 8; ++i) {
+                    float cosine = c[i], sine = s[i];
+                    asm volatile("" : "+v"(cosine), "+v"(sine));
+                    c[i] = cosine;
+                    s[i] = sine;
+                }
+#pragma unroll
+                for (int i = 0; i < BYTES / 4; ++i) asm volatile("" : "+v"(gamma[K].w[i]), "+v"(other_gamma[K].w[i]));
+            }
+            Channels<double> v;
+            norm_and_turn_row(v, a.gamma[1], gamma[K], other_gamma[K]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = cut(v.x[i]);
         }
-        norm_and_turn(v, gamma != nullptr, gx, gy, a.dim, a.eps, a.lanes_log2, turned, c, s);
-        if (!there || !has) return;
-        Words<BYTES> out = narrow_all<T, 8>(v.x);
-        if (where.position < 0) out = Words<BYTES>{};
-        store_words<BYTES>(a.out[0] + token * a.out_token[0] + h * a.out_head[0] + d0 * T::kBytes, out);
-        return;
-    }
-    if (cls == 1) {
-        Channels<double> v;
+        uint32_t largest = 0; // magnitudes compare as whole numbers, infinities and NaN above all
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v.x[i] = x[i];
-            v.y[i] = y[i];
+        for (int i = 0; i < 8; ++i) largest = max(largest, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+        largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0xB1, 0xf, 0xf, false));
+        largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0x4E, 0xf, 0xf, false));
+        const bool finite = largest < 0x7f800000u;
+        const int exponent = (int)((largest + 0x00200000u) >> 23) - 2;
+        const uint32_t scale = finite ? (uint32_t)min(max(exponent, 2), a.most_exponent + 127) : 255u;
+        const float unit = __builtin_bit_cast(float, scale << 23);
+        uint32_t codes = 0;
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], unit, 0);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], unit, 1);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], unit, 2);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], unit, 3);
+        if (head[r] < 0 || where.page < 0) continue;
+        const auto &late = arguments_again<HeadRowsFp4Args>();
+        char *const to = late.out[cls[r]] + where.page * late.out_page[cls[r]] + where.slot * late.out_token[cls[r]] + head[r] * late.out_head[cls[r]];
+        store_words<4>(to + d0 / 2, Words<4>{{finite ? codes : 0u}});
+        if ((place & 3) == 0) {
+            const int i = cls[r] - 1;
+            char *const scale_to = late.scales[i] + where.page * late.scale_page[i] + where.slot * late.scale_slot[i] + head[r] * late.scale_head[i];
+            *(__attribute__((address_space(1))) uint8_t *)(scale_to + place / 4) = (uint8_t)scale;
         }
-        norm_and_turn(v, gamma != nullptr, gx, gy, a.dim, a.eps, a.lanes_log2, turned, c, s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = cut(v.x[i]);
-    }
-    uint32_t largest = 0; // magnitudes compare as whole numbers, infinities and NaN above all
-#pragma unroll
-    for (int i = 0; i < 8; ++i) largest = max(largest, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
-    largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0xB1, 0xf, 0xf, false));
-    largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0x4E, 0xf, 0xf, false));
-    const bool finite = largest < 0x7f800000u;
-    const int exponent = (int)((largest + 0x00200000u) >> 23) - 2;
-    const uint32_t scale = finite ? (uint32_t)min(max(exponent, 2), a.most_exponent + 127) : 255u;
-    const float unit = __builtin_bit_cast(float, scale << 23);
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], unit, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], unit, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], unit, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], unit, 3);
-    if (!there || !has || where.page < 0) return;
-    const auto &late = arguments_again<HeadRowsFp4Args>();
-    const int i = cls - 1;
-    char *const to = (i == 0 ? late.out[1] : late.out[2]) + where.page * (i == 0 ? late.out_page[1] : late.out_page[2]) +
-                     where.slot * (i == 0 ? late.out_token[1] : late.out_token[2]) + h * (i == 0 ? late.out_head[1] : late.out_head[2]);
-    store_words<4>(to + d0 / 2, Words<4>{{finite ? codes : 0u}});
-    if ((place & 3) == 0) {
-        char *const scale_to = (i == 0 ? late.scales[0] : late.scales[1]) + where.page * (i == 0 ? late.scale_page[0] : late.scale_page[1]) +
-                               where.slot * (i == 0 ? late.scale_slot[0] : late.scale_slot[1]) + h * (i == 0 ? late.scale_head[0] : late.scale_head[1]);
-        *(__attribute__((address_space(1))) uint8_t *)(scale_to + place / 4) = (uint8_t)scale;
     }
 }
 
@@ -199,18 +253,28 @@ int launch_head_rows_fp4(HeadRowsFp4Args &a, int dtype, hipStream_t s) {
     if (a.tokens == 0 || heads_all == 0) return TDE_OK;
     a.lanes_log2 = 2;
     while ((8 << a.lanes_log2) < a.dim) ++a.lanes_log2;
-    const int64_t at_once = 64 >> a.lanes_log2, waves = (heads_all + at_once - 1) / at_once;
+    for (int i = 0; i < 3; ++i) a.rounds[i] = (a.heads[i] + (64 >> a.lanes_log2) - 1) >> (6 - a.lanes_log2);
+    const int64_t rounds = (int64_t)a.rounds[0] + a.rounds[1] + a.rounds[2];
+    const auto waves_of = [&](int rows) { return (rounds + rows - 1) / rows; };
+    const bool whole = (a.interleaved ? 2 * a.half : a.half) % 8 == 0;
+    // Rows of a lane.  2048 tokens of 32 + 2 * 8 heads of 128 bf16 channels, and the caches' unpacking behind them, take 29 us with four and 32 with one,
+    // four times as many 75 and 108; fp32 rows of as many bytes take 81 with four, which cost it registers, and 75 with one; few rows are for all units.
+    const int rows = whole && dtype != TDE_F32 && a.tokens * waves_of(4) >= 1024 ? 4 : 1;
+    const int64_t waves = waves_of(rows);
     if (a.tokens > (int64_t)0x7ffffff0 / waves) return TDE_ETOOBIG;
     const uint32_t blocks = (uint32_t)((a.tokens * waves + 3) / 4);
     if (!fits_launch(blocks, 256)) return TDE_ETOOBIG;
     a.waves_per_token = Divisor32((uint32_t)waves);
-    const bool whole = (a.interleaved ? 2 * a.half : a.half) % 8 == 0;
     const auto launch = [&](auto type) {
         using T = decltype(type);
-        if (a.interleaved && whole) head_rows_fp4_kernel<T, true, true><<<blocks, 256, 0, s>>>(a);
-        else if (a.interleaved) head_rows_fp4_kernel<T, true, false><<<blocks, 256, 0, s>>>(a);
-        else if (whole) head_rows_fp4_kernel<T, false, true><<<blocks, 256, 0, s>>>(a);
-        else head_rows_fp4_kernel<T, false, false><<<blocks, 256, 0, s>>>(a);
+        if (!whole && a.interleaved) head_rows_fp4_kernel<T, true, false, 1><<<blocks, 256, 0, s>>>(a);
+        else if (!whole) head_rows_fp4_kernel<T, false, false, 1><<<blocks, 256, 0, s>>>(a);
+        else if (rows == 1 && a.interleaved) head_rows_fp4_kernel<T, true, true, 1><<<blocks, 256, 0, s>>>(a);
+        else if (rows == 1) head_rows_fp4_kernel<T, false, true, 1><<<blocks, 256, 0, s>>>(a);
+        else if constexpr (T::kBytes == 2) {
+            if (a.interleaved) head_rows_fp4_kernel<T, true, true, 4><<<blocks, 256, 0, s>>>(a);
+            else head_rows_fp4_kernel<T, false, true, 4><<<blocks, 256, 0, s>>>(a);
+        }
     };
     if (dtype == TDE_BF16) launch(Bf16{});
     else if (dtype == TDE_F16) launch(F16{});
