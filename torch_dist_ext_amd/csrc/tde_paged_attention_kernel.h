@@ -263,9 +263,13 @@ __device__ __forceinline__ void wait_for_loads() {
 
 // NB blocks of 16 rows a wavefront.  SHARED: the wavefronts have rows of their own and share tiles of keys, double-buffered in LDS;
 // otherwise all have the same rows and take the tiles in turn, each through LDS of its own, and are joined at the end.
-// (Heads of 64: four such workgroups a unit hide the loads, with the registers of three 8 rows over 16000 keys take 24.0 us in place of 20.2.)
+// (Heads of 64: four workgroups a unit hide the loads, with the registers of three 8 rows over 16000 keys take 24.0 us in place of 20.2, and 24 sequences
+// of up to 512 rows over a cache in 4 bits 78 in place of 61.)
 template <class T, class C, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
-__global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED ? 4 : 2)) attention_kernel(const typename C::Args a) {
+constexpr int workgroups_a_unit = D == 256 ? 1 : (D == 64 && (!SHARED || (C::kFp4 && NB == 1 && !SPLIT)) ? 4 : 2);
+
+template <class T, class C, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
+__global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit<T, C, D, NB, WAVES, SHARED, SPLIT>) attention_kernel(const typename C::Args a) {
     constexpr bool FP4 = C::kFp4;
     constexpr int KT = SHARED && D <= 128 ? 64 : 32; // keys a tile
     constexpr int CH = D / 8;                        // chunks of 16 bytes a row
@@ -464,6 +468,11 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
         }
         return {};
     };
+    [[maybe_unused]] Held mine{};
+    if constexpr (HALVES) { // kept: loaded anew for each tile they are waited for (24 sequences of up to 512 rows: 64 us, and 61)
+        mine = held(takes_values);
+        asm volatile("" : "+s"(mine.codes), "+s"(mine.scales), "+s"(mine.page), "+s"(mine.slot), "+s"(mine.scale_page), "+s"(mine.scale_slot));
+    }
     // Where 16 keys lie in one page, and lanes' offsets hold 32 bits, a wavefront's rows (8, 16 or twice 16) have scalar addresses.
     [[maybe_unused]] const bool scalar_rows = FP4 && a.batch.page.d % 16 == 0 && (a.k_slot | a.v_slot) < 1u << 27 && a.batch.cache_pages > 0;
     const auto fetch = [&]([[maybe_unused]] int32_t key0, [[maybe_unused]] uint64_t &lost) { // look_up has been called for the tile
@@ -518,7 +527,7 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
                 }
             };
             if constexpr (HALVES) {
-                one(held(takes_values), codes.k, codes.k_scale);
+                one(mine, codes.k, codes.k_scale);
             } else {
                 one(held(false), codes.k, codes.k_scale);
                 one(held(true), codes.v, codes.v_scale);
@@ -527,9 +536,8 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
     };
     // Part `i` of PARTS of the codes that were fetched into LDS as numbers.
     constexpr int PARTS = HALVES ? 4 : 8;
-    // When: while the matrix units work on the tile's scores, if registers allow for it (4096 rows behind 4096 in heads of 128: 436 us, ahead of them 449).  Heads of 64
-    // keep four workgroups a unit without it (24 sequences of up to 512 rows 65 us, with it three and 74).
-    [[maybe_unused]] constexpr bool WITH_SCORES = D > 64;
+    // When: while the matrix units work on the tile's scores (4096 rows behind 4096 in heads of 128: 433 us, ahead of them 449; 24 sequences of up to 512
+    // rows in heads of 64 60.5 and 61).
     const auto put = [&]([[maybe_unused]] uint32_t to, [[maybe_unused]] int i) {
         if constexpr (FP4) {
             const bool second = !HALVES && i >= 4;
@@ -610,14 +618,6 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
         if constexpr (FP4) {
             sync();
             lost_next = lost_fetched;
-            if (!WITH_SCORES && more) {
-#pragma unroll
-                for (int i = 0; i < PARTS; ++i) put(buf ^ (2 * TILE), i);
-                if (next + TILE_STEP < until) {
-                    look_up((int32_t)next + TILE_STEP);
-                    fetch((int32_t)next + TILE_STEP, lost_fetched);
-                }
-            }
         } else if constexpr (SHARED) {
             wait_for_loads<0>();
             sync();
@@ -659,13 +659,13 @@ __global__ void __launch_bounds__(64 * WAVES, D == 256 ? 1 : (D == 64 && !SHARED
                     for (int u = 0; u < U; ++u) s[n][kb] = Mfma<T>::mul(kf[unit & 1][u], q[n][st + u], s[n][kb]);
                 }
                 // the next tile's numbers, which the products leave time for (behind the last tile old ones, which nothing reads)
-                if constexpr (FP4 && WITH_SCORES) {
+                if constexpr (FP4) {
 #pragma unroll
                     for (int i = unit * PARTS / UNITS; i < (unit + 1) * PARTS / UNITS; ++i) put(buf ^ (2 * TILE), i);
                 }
             }
         }
-        if constexpr (FP4 && WITH_SCORES) {
+        if constexpr (FP4) {
             if (next + TILE_STEP < until) {
                 look_up((int32_t)next + TILE_STEP);
                 fetch((int32_t)next + TILE_STEP, lost_fetched);
