@@ -265,11 +265,12 @@ __device__ __forceinline__ void wait_for_loads() {
 // otherwise all have the same rows and take the tiles in turn, each through LDS of its own, and are joined at the end.
 // (Heads of 64: four workgroups a unit hide the loads, with the registers of three 8 rows over 16000 keys take 24.0 us in place of 20.2, and 24 sequences
 // of up to 512 rows over a cache in 4 bits 78 in place of 61.)
-template <class T, class C, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
-constexpr int workgroups_a_unit = D == 256 ? 1 : (D == 64 && (!SHARED || (C::kFp4 && NB == 1 && !SPLIT)) ? 4 : 2);
+constexpr int workgroups_a_unit(bool fp4, int dim, int nb, bool shared, bool split) {
+    return dim == 256 ? 1 : (dim == 64 && (!shared || (fp4 && nb == 1 && !split)) ? 4 : 2);
+}
 
 template <class T, class C, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
-__global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit<T, C, D, NB, WAVES, SHARED, SPLIT>) attention_kernel(const typename C::Args a) {
+__global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, SHARED, SPLIT)) attention_kernel(const typename C::Args a) {
     constexpr bool FP4 = C::kFp4;
     constexpr int KT = SHARED && D <= 128 ? 64 : 32; // keys a tile
     constexpr int CH = D / 8;                        // chunks of 16 bytes a row
