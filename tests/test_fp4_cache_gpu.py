@@ -228,6 +228,15 @@ def test_many_sequences_and_rows(tde):
     run(tde, Batch([700, 900], [700, 1500], 64, seed=3), 4, 2, 64, torch.bfloat16, 64, False, True)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("heads,kv_heads,dim,rot,interleaved,norm,queries", [
+    (8, 2, 128, 64, True, False, True), (15, 5, 96, 96, False, True, True), (7, 1, 256, 128, True, True, True), (3, 3, 64, 0, False, True, True),
+    (1, 9, 32, 16, False, True, False), (33, 1, 64, 64, False, False, True), (2, 1, 96, 2, False, True, True)])
+def test_many_rows(tde, heads, kv_heads, dim, rot, interleaved, norm, queries, dtype):
+    run(tde, Batch([700, 1, 350], [700, 90, 500], 24, seed=4, pad=6), heads, kv_heads, dim, dtype, rot, interleaved, norm, seed=dim, queries=queries,
+        heads_first=True)
+
+
 def test_rows_of_one_projection_into_one_tensor(tde):
     """q, k and v as columns of one tensor, codes and scales as ranges of one allocation whose rows begin anywhere."""
     batch = Batch([3, 8], [9, 8], 4, seed=9)
