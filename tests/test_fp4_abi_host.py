@@ -78,6 +78,29 @@ def test_attention_refuses():
         assert lib.tde_paged_attention_fp4(ctypes.byref(attention_fp4(**split, **kw)), None) == status, kw
 
 
+def test_launches_that_do_not_fit():
+    """Calls of more threads than one launch holds (2^32), or of more tiles than are counted, are refused before anything runs, or planned another way."""
+    lib, n = _capi.load(), ctypes.c_int64()
+    for kw in (dict(tokens=1 << 26, q_heads=1, kv_heads=0, dim=32, rot_dim=0), dict(tokens=1 << 23, q_heads=64, kv_heads=8, dim=256, rot_dim=0),
+               dict(tokens=1 << 30, q_heads=8, kv_heads=8, dim=256, rot_dim=0)):
+        assert lib.tde_append_kv_fp4(ctypes.byref(append(**kw)), None) == _capi.ETOOBIG, kw
+    for kw in (dict(tokens=1 << 24, batch=batch(seqs=1 << 24)), dict(tokens=1 << 30, q_heads=1, kv_heads=1, dim=256, batch=batch(seqs=1 << 24)),
+               dict(tokens=1 << 24, q_heads=1, kv_heads=1, batch=batch(seqs=1 << 24))):
+        kw = dict(kw, workspace=SOMEWHERE, workspace_bytes=1 << 62)
+        assert lib.tde_paged_attention_fp4_workspace(ctypes.byref(attention_fp4(**kw)), ctypes.byref(n)) == _capi.ETOOBIG, kw
+        assert lib.tde_paged_attention_fp4(ctypes.byref(attention_fp4(**kw)), None) == _capi.ETOOBIG, kw
+    for kw in (dict(tokens=1 << 20, batch=batch(seqs=1 << 20)), dict(tokens=1, q_heads=64, kv_heads=64, batch=batch(seqs=1 << 15, table_pages=4096)),
+               dict(tokens=1, q_heads=1, kv_heads=1, batch=batch(seqs=1, table_pages=(1 << 31) // 128)), dict(tokens=1 << 23, q_heads=64, kv_heads=8, batch=batch(seqs=1))):
+        assert lib.tde_paged_attention_fp4_workspace(ctypes.byref(attention_fp4(**kw)), ctypes.byref(n)) == _capi.OK, kw
+
+
+def test_scales_of_scores():
+    """A scale whose product with log2(e) is no fp32 number would make every weight NaN."""
+    lib, n = _capi.load(), ctypes.c_int64()
+    for scale, status in ((2e38, _capi.OK), (2.4e38, _capi.EINVAL), (float("inf"), _capi.EINVAL), (1e-45, _capi.OK), (1e-46, _capi.EINVAL), (float("nan"), _capi.EINVAL)):
+        assert lib.tde_paged_attention_fp4_workspace(ctypes.byref(attention_fp4(scale=scale)), ctypes.byref(n)) == status, scale
+
+
 def unpack(sizes=(2, 3, 4), code_strides=(768, 256, 64), scale_strides=(48, 16, 4), **kw):
     base = dict(dim=128, out_dtype=_capi.BF16, codes=SOMEWHERE, scales=SOMEWHERE, out=SOMEWHERE)
     base.update(kw)
