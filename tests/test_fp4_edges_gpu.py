@@ -3,7 +3,7 @@ front, other streams, autograd and compiled graphs."""
 import pytest
 import torch
 
-from block_reference import Batch, assert_close, attention
+from block_reference import Batch, assert_close, attention, attention_at_once
 from fp4_reference import as_read, decode, encode
 from test_block_single_strides_gpu import ODD, with_stride
 from test_fp4_cache_gpu import caches, cos_sin
@@ -32,6 +32,22 @@ def test_tiles_alone_fill_the_device(tde, dim, seqs, page):
     batch = Batch([1] * seqs, [n + 1 for n in lens], page, seed=dim + 1)
     batch.table[9, 0] = -1
     run(tde, batch, 8, 8, dim, torch.float16, seed=dim + 1, heads_first=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("dim,page", [(96, 24), (128, 16), (128, 64)])
+@pytest.mark.parametrize("new,lens", [([1650, 0, 130], [2000, 5, 130]), ([2300, 900, 1500], [2300, 1000, 3000])], ids=["256 rows", "128 rows"])
+def test_largest_tiles(tde, new, lens, dim, page, dtype):
+    """64 heads that share 8; a block of values that is NaN, a page that is none, garbage behind the last keys."""
+    batch = Batch(new, lens, page, seed=2, pad=5)
+    parts = held(batch, 8, dim, 3)
+    parts[3][batch.page_of(0, 300), 300 % page, :, 1] = 255
+    parts[3][batch.page_of(2, lens[2] - 20), 5, 3, 0] = 255
+    for b in (0, 2):
+        for i in (1, 3):
+            parts[i][batch.page_of(b, lens[b] - 1), lens[b] % page or page:] = 255
+    batch.table[2, (lens[2] - 1) // page] = -1                                    # (the last: the oracle wants a key in every sequence)
+    run(tde, batch, 64, 8, dim, dtype, seed=4, parts=parts, reference=attention_at_once)
 
 
 def test_more_heads_than_the_device_holds_workgroups(tde):

@@ -792,17 +792,34 @@ void launch_decode_type(const AttentionFp4Args &a, const AttentionPlan &p, hipSt
 
 // Which kernel.  Calls whose sequences have no more than 16 rows on average go to the decode kernel, which takes pages of whole 8 keys, and a table and caches that
 // have any; the others to tiles of 64 or 128 rows, as plan_attention says.
+namespace {
+
+// Tiles that share keys.  Heads of 65 to 128 take 256 rows where those are two workgroups a unit at most (128 rows, two workgroups at once, make numbers of all
+// codes twice): 4096 rows behind 4096 405 us and 433, 2 x 2048 behind 2048 218 and 246, 3100 rows by themselves 107 and 107.  Beyond, a unit that gets one
+// tile more than others costs what that saves: 5000 rows behind 2000 434 and 416, 8192 by themselves 558 and 572.
+int plan_tiles(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
+    const int status = plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 64, p);
+    if (status != TDE_OK || p->rows != 128 || p->wide_dim != 128) return status;
+    const int64_t rows_all = tokens * (q_heads / kv_heads);
+    if ((rows_all / 256 + seqs / 4) * kv_heads > 2 * (int64_t)device_compute_units()) return status;
+    p->rows = 256;
+    p->tiles = p->items = rows_all / 256 + seqs + 2; // no more than of 128 rows, but their workgroups have twice the threads
+    return fits_launch(p->items * kv_heads, 512) ? TDE_OK : TDE_ETOOBIG;
+}
+
+} // namespace
+
 int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const tde_paged_batch &b, AttentionPlan *p) {
     const int64_t rows_all = tokens * (q_heads / kv_heads), capacity = (int64_t)b.table_pages * b.page_size;
     if (b.page_size % 8 != 0 || b.table_pages == 0 || b.cache_pages == 0 || rows_all > (int64_t)b.seqs * 16)
-        return plan_attention_rows(dim, tokens, q_heads, kv_heads, b.seqs, capacity, 64, p);
+        return plan_tiles(dim, tokens, q_heads, kv_heads, b.seqs, capacity, p);
     *p = AttentionPlan{};
     p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
     p->rows = 16;
     // As many runners as the device holds workgroups, by their registers; every die the same number.
     const int64_t tiles = rows_all / 16 + b.seqs + 2;
     const int64_t most = std::max<int64_t>(kDecodeWaves, (capacity + kUnit) / kUnit); // units of a tile
-    if (tiles > 0x7fffff00 / most) return plan_attention_rows(dim, tokens, q_heads, kv_heads, b.seqs, capacity, 64, p); // units are counted in 32 bits
+    if (tiles > 0x7fffff00 / most) return plan_tiles(dim, tokens, q_heads, kv_heads, b.seqs, capacity, p); // units are counted in 32 bits
     const int64_t at_once = std::max<int64_t>(1, std::min<int64_t>((int64_t)resident_workgroups(p->wide_dim, b.page_size % 16 == 0 ? 16 : 8) * device_compute_units() / kv_heads, kMostRunners));
     const int64_t likely = std::max<int64_t>(1, std::min<int64_t>(b.seqs, tokens)); // tiles
     // Where tiles alone fill the device more than twice each is a runner's, and nothing is cut.

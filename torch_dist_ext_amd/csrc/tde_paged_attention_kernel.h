@@ -1101,6 +1101,12 @@ void launch_dim(const typename C::Args &a, const AttentionPlan &p, uint32_t bloc
     if constexpr (!C::kFp4) {
         if (p.rows == 16) return launch_one<T, C, D, 1, ALONE, false>(a, p, blocks, s);
     }
+    if constexpr (C::kFp4 && D == 128) {
+        if (p.rows == 256) {
+            attention_kernel<T, C, D, 2, 8, true, false><<<blocks, 512, 0, s>>>(a);
+            return;
+        }
+    }
     if (p.rows == 64) launch_one<T, C, D, 1, 4, true>(a, p, blocks, s);
     else attention_kernel<T, C, D, D <= 128 ? 2 : 1, D <= 128 ? 4 : 8, true, false><<<blocks, D <= 128 ? 256 : 512, 0, s>>>(a); // 128, never split
 }
