@@ -36,17 +36,19 @@ def test_tiles_alone_fill_the_device(tde, dim, seqs, page):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("dim,page", [(96, 24), (128, 16), (128, 64)])
-@pytest.mark.parametrize("new,lens", [([1650, 0, 130], [2000, 5, 130]), ([2300, 900, 1500], [2300, 1000, 3000])], ids=["256 rows", "128 rows"])
+@pytest.mark.parametrize("new,lens", [([1650, 0, 130], [2000, 5, 130]), ([2300, 900, 1500], [2300, 1000, 3000]), ([1950, 100], [2200, 130])],
+                         ids=["few", "many", "long"])
 def test_largest_tiles(tde, new, lens, dim, page, dtype):
     """64 heads that share 8; a block of values that is NaN, a page that is none, garbage behind the last keys."""
     batch = Batch(new, lens, page, seed=2, pad=5)
     parts = held(batch, 8, dim, 3)
     parts[3][batch.page_of(0, 300), 300 % page, :, 1] = 255
-    parts[3][batch.page_of(2, lens[2] - 20), 5, 3, 0] = 255
-    for b in (0, 2):
+    last = len(new) - 1
+    parts[3][batch.page_of(last, lens[last] - 20), 5, 3, 0] = 255
+    for b in (0, last):
         for i in (1, 3):
             parts[i][batch.page_of(b, lens[b] - 1), lens[b] % page or page:] = 255
-    batch.table[2, (lens[2] - 1) // page] = -1                                    # (the last: the oracle wants a key in every sequence)
+    batch.table[last, (lens[last] - 1) // page] = -1                                 # (the last: the oracle wants a key in every sequence)
     run(tde, batch, 64, 8, dim, dtype, seed=4, parts=parts, reference=attention_at_once)
 
 

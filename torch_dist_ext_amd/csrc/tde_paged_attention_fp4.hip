@@ -794,14 +794,15 @@ void launch_decode_type(const AttentionFp4Args &a, const AttentionPlan &p, hipSt
 // have any; the others to tiles of 64 or 128 rows, as plan_attention says.
 namespace {
 
-// Tiles that share keys.  Heads of 65 to 128 take 256 rows where those are two workgroups a unit at most (128 rows, two workgroups at once, make numbers of all
-// codes twice): 4096 rows behind 4096 405 us and 433, 2 x 2048 behind 2048 218 and 246, 3100 rows by themselves 107 and 107.  Beyond, a unit that gets one
-// tile more than others costs what that saves: 5000 rows behind 2000 434 and 416, 8192 by themselves 558 and 572.
+// Tiles that share keys.  Heads of 65 to 128 take 256 rows where those are two workgroups a unit at most and sequences are long (128 rows, two workgroups
+// at once, make numbers of all codes twice): 4096 rows behind 4096 396 us and 427, 3700 behind 8000 604 and 660, 2 x 2048 behind 2048 218 and 246, 3100 by
+// themselves 107 and 107.  Elsewhere a unit that gets one tile more than others costs what that saves: 5000 rows behind 2000 434 and 416, 8192 by themselves 558
+// and 572, 20 sequences of up to 700 behind 3000 131 and 121.
 int plan_tiles(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
     const int status = plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 64, p);
     if (status != TDE_OK || p->rows != 128 || p->wide_dim != 128) return status;
     const int64_t rows_all = tokens * (q_heads / kv_heads);
-    if ((rows_all / 256 + seqs / 4) * kv_heads > 2 * (int64_t)device_compute_units()) return status;
+    if (rows_all < (int64_t)seqs * 8192 || rows_all / 256 * kv_heads > 2 * (int64_t)device_compute_units()) return status;
     p->rows = 256;
     p->tiles = p->items = rows_all / 256 + seqs + 2; // no more than of 128 rows, but their workgroups have twice the threads
     return fits_launch(p->items * kv_heads, 512) ? TDE_OK : TDE_ETOOBIG;

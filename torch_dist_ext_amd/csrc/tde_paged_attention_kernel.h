@@ -342,6 +342,9 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
     const int32_t *const table = a.batch.table + it.seq * a.batch.table_stride;
     const char *const k_base = a.k + kv_head * a.k_head, *const v_base = a.v + kv_head * a.v_head;
     constexpr int TILE_STEP = SHARED ? KT : KT * WAVES;
+    // Keys up to two tiles behind the last one: there are 2^31 - 255 at most, so 32 bits hold them, which scalar instructions compare.
+    using Key = std::conditional_t<FP4, int32_t, int64_t>;
+    static_assert(!FP4 || TILE_STEP <= 64, "");
     const int32_t first_key = from + (SHARED ? 0 : wave * KT);
     // Lane l holds the table's entry window + l: 64 pages, and a tile needs no more.  Nothing else in the loop is loaded by way of
     // registers: the compiler would wait for it, and with it for every load to LDS that was issued before.
@@ -349,7 +352,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
     uint64_t missing = 0; // entries that are no page
     const auto look_up = [&](int32_t key0) { // before offsets_of(key0)
         const uint32_t first = a.batch.page.quotient((uint32_t)key0);
-        const uint32_t end = a.batch.page.quotient((uint32_t)std::min<int64_t>((int64_t)key0 + KT, until) - 1);
+        const uint32_t end = a.batch.page.quotient((uint32_t)std::min<Key>((Key)key0 + KT, until) - 1);
         if (end - (uint32_t)window < 64) return;
         window = (int32_t)first;
         entries = page_number(a.batch, table, first + lane);
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
             fetch(first_key, lost_next);
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) put(buf, i);
-            if ((int64_t)first_key + TILE_STEP < until) {
+            if ((Key)first_key + TILE_STEP < until) {
                 look_up(first_key + TILE_STEP);
                 fetch(first_key + TILE_STEP, lost_fetched);
             }
@@ -612,7 +615,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
             __builtin_amdgcn_wave_barrier();
         }
     };
-    int64_t next = (int64_t)first_key + TILE_STEP;
+    Key next = (Key)first_key + TILE_STEP;
     for (int32_t key0 = first_key; key0 < until;) {
         const bool more = next < until;
         const uint64_t lost = lost_next; // keys without a page
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
                     for (int r = 0; r < 4; ++r)
                         if ((lost >> (quad * 4) >> (kb * 16 + r)) & 1) s[n][kb][r] = __builtin_nanf("");
         }
-        if ((int64_t)key0 + KT > std::min(lowest, until)) {
+        if ((Key)key0 + KT > std::min(lowest, until)) {
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 const int32_t see = std::min(last[n], until - 1) - key0 - quad * 4;
@@ -784,7 +787,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
         }
         // whether values that not all rows see hold an infinity or a NaN
         bool poisoned = false;
-        if ((FP4 ? (int64_t)key0 + KT : std::min<int64_t>((int64_t)key0 + KT, until)) > lowest) { // (of 4 bits, what lies behind the last key is there)
+        if ((FP4 ? (Key)key0 + KT : std::min<Key>((Key)key0 + KT, until)) > lowest) { // (of 4 bits, what lies behind the last key is there)
             // an exponent of ones plus one at its lowest bit carries out of its field; the field's neighbours are masked off before
             constexpr uint32_t E = Mfma<T>::kExponent, LOW = E & (~E + 1u);
             uint32_t carried = 0;
@@ -909,7 +912,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             values_exact = load((int32_t)next, buf, lost_next, kNo, kYes);
         }
-        key0 = (int32_t)std::min<int64_t>(next, 0x7fffffff);
+        key0 = (int32_t)std::min<Key>(next, 0x7fffffff);
         next += TILE_STEP;
     }
 
