@@ -81,7 +81,7 @@ def test_attention_refuses():
 def test_launches_that_do_not_fit():
     """Calls of more threads than one launch holds (2^32), or of more tiles than are counted, are refused before anything runs, or planned another way."""
     lib, n = _capi.load(), ctypes.c_int64()
-    for kw in (dict(tokens=1 << 26, q_heads=1, kv_heads=0, dim=32, rot_dim=0), dict(tokens=1 << 23, q_heads=64, kv_heads=8, dim=256, rot_dim=0),
+    for kw in (dict(tokens=1 << 26, q_heads=1, kv_heads=0, dim=32, rot_dim=0), dict(tokens=1 << 23, q_heads=64, kv_heads=8, dim=256, rot_dim=0, dtype=_capi.F32),
                dict(tokens=1 << 30, q_heads=8, kv_heads=8, dim=256, rot_dim=0)):
         assert lib.tde_append_kv_fp4(ctypes.byref(append(**kw)), None) == _capi.ETOOBIG, kw
     for kw in (dict(tokens=1 << 24, batch=batch(seqs=1 << 24)), dict(tokens=1 << 30, q_heads=1, kv_heads=1, dim=256, batch=batch(seqs=1 << 24)),

@@ -76,6 +76,7 @@ struct HeadRowsFp4Args : HeadRowsArgs {
     int64_t scale_page[2], scale_slot[2], scale_head[2];
     int32_t most_exponent;
     int32_t rounds[3]; // as many rows as a wavefront has at once
+    int32_t turns;     // times that a wavefront takes rows
 };
 
 int plan_head_rows(int elem, int dim, int half, bool interleaved, int64_t tokens, int64_t heads_all, HeadRowsPlan *p);

@@ -12,10 +12,12 @@
 // hardware's conversion then rounds once.
 //
 // A row is read once, 16 bytes a lane, with its partner in the rotation, which comes from the nearest cache.  8192 tokens of 32 + 2 * 8 heads of 128
-// fp16 channels, a half of them rotated, take 42 us, 4.2 TB/s: vector instructions take 27 us of it and the wait for a token's sequence, place and
-// cosines the rest; queries written past the caches and rows of one kind to a wavefront's instruction brought it there from 60.
+// fp16 channels, a half of them rotated, take 38 us, 4.6 TB/s: vector instructions take 21 us of it, and the waits for rows, a token's sequence and place the
+// rest.  Rows of one kind to an instruction, queries written past the caches and doubles of one channel at a time brought it there from 60.
 #include "tde_block.h"
 #include "tde_head_rows.h"
+
+#include <type_traits>
 
 namespace tde {
 namespace block {
@@ -37,34 +39,83 @@ __device__ __forceinline__ float cut(double x) {
     return __builtin_bit_cast(float, bits);
 }
 
-__device__ __forceinline__ float multiply_add(float x, float y, float z) { return __builtin_fmaf(x, y, z); }
-__device__ __forceinline__ double multiply_add(double x, double y, double z) { return __builtin_fma(x, y, z); }
-
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
+// x as if it were new here, behind what was new before: what follows from it is not computed any earlier.
+__device__ __forceinline__ float in_turn(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // Norm and rotation of a lane's eight channels x; y are their partners in the rotation, c and s (with the sign that the channel takes it) theirs.
-template <class A>
-struct Channels {
-    A x[8], y[8];
-};
-template <bool WHOLE, class A>
-__device__ __forceinline__ void norm_and_turn(Channels<A> &v, bool normed, const float (&gx)[8], const float (&gy)[8], int dim, float eps, int lanes_log2,
-                                              uint32_t turned, f32x8 c, f32x8 s) {
+template <bool WHOLE>
+__device__ __forceinline__ void norm_and_turn(float (&x)[8], const float (&y)[8], bool normed, const float (&gx)[8], const float (&gy)[8], int dim, float eps,
+                                              int lanes_log2, uint32_t turned, f32x8 c, f32x8 s) {
+    float scale = 1.0f;
     if (normed) {
-        A sq = 0;
+        float sq = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq += v.x[i] * v.x[i];
-        sq = sum_over_lanes(sq, lanes_log2);
-        const A scale = (A)1 / (sizeof(A) == 8 ? (A)__builtin_sqrt((double)(sq / (A)dim + (A)eps)) : (A)__builtin_sqrtf((float)(sq / (A)dim + (A)eps)));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v.x[i] = v.x[i] * scale * (A)gx[i];
-            v.y[i] = v.y[i] * scale * (A)gy[i];
-        }
+        for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
+        scale = 1.0f / __builtin_sqrtf(sum_over_lanes(sq, lanes_log2) / (float)dim + eps);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (WHOLE ? turned != 0 : ((turned >> i) & 1) != 0) v.x[i] = multiply_add(v.x[i], (A)c[i], v.y[i] * (A)s[i]);
+    for (int i = 0; i < 8; ++i) {
+        float other = y[i];
+        if (normed) {
+            x[i] = x[i] * scale * gx[i];
+            other = other * scale * gy[i];
+        }
+        // (partners are taken from y: x's own are those of other channels)
+        if (WHOLE ? turned != 0 : ((turned >> i) & 1) != 0) x[i] = __builtin_fmaf(x[i], c[i], other * s[i]);
+    }
+}
+// The same in doubles, cut: one channel after the other, as all at once they would take the registers of twice as many wavefronts.
+template <bool WHOLE>
+__device__ __forceinline__ void norm_and_turn_exactly(float (&x)[8], const float (&y)[8], bool normed, const float (&gx)[8], const float (&gy)[8], int dim, float eps,
+                                                      int lanes_log2, uint32_t turned, f32x8 c, f32x8 s) {
+    double scale = 1.0;
+    if (normed) {
+        double sq = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double own = in_turn(x[i]);
+            sq += own * own;
+        }
+        scale = 1.0 / __builtin_sqrt(sum_over_lanes(sq, lanes_log2) / (double)dim + (double)eps);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        double own = in_turn(x[i]), other = in_turn(y[i]);
+        if (normed) {
+            own = own * scale * (double)in_turn(gx[i]);
+            other = other * scale * (double)in_turn(gy[i]);
+        }
+        if (WHOLE ? turned != 0 : ((turned >> i) & 1) != 0) own = __builtin_fma(own, (double)in_turn(c[i]), other * (double)in_turn(s[i]));
+        x[i] = in_turn(cut(own));
+    }
+}
+
+// place_of, whose chain of loads is one shorter where a lane has a sequence of its own.
+__device__ __forceinline__ Place place_at_once(const PagedBatch &b, int64_t token, int lane) {
+    if (b.seqs > 64) return place_of(b, token, lane);
+    const int mine = min(lane, b.seqs - 1);
+    int32_t begin = 0, end = 0, len = 0;
+    if (mine >= 0) {
+        begin = b.starts[mine];
+        end = b.starts[mine + 1];
+        len = b.lens[mine];
+    }
+    Place p{-1, -1, 0};
+    const int seq = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < b.seqs && end <= token));
+    if (seq >= b.seqs) return p;
+    const int64_t first = __builtin_amdgcn_readlane(begin, seq);
+    if (token < first) return p;
+    p.position = (int64_t)__builtin_amdgcn_readlane(len, seq) - (__builtin_amdgcn_readlane(end, seq) - first) + (token - first);
+    if (p.position < 0 || p.position > 0x7fffffff) return p; // the latter only where starts do not ascend
+    const uint32_t at = b.page.quotient((uint32_t)p.position);
+    p.slot = (int32_t)((uint32_t)p.position - at * b.page.d);
+    p.page = page_number(b, b.table + seq * b.table_stride, at);
+    return p;
 }
 
 } // namespace
@@ -80,7 +131,7 @@ __global__ void __launch_bounds__(256) head_rows_fp4_kernel(const HeadRowsFp4Arg
     const uint32_t row = a.waves_per_token.quotient(wave);
     const int64_t token = row;
     if (token >= a.tokens) return;
-    const int round = (int)(wave - row * a.waves_per_token.d) * R;
+    int round = (int)(wave - row * a.waves_per_token.d) * (R > 1 ? R * a.turns : 1);
     const int place = lane & ((1 << a.lanes_log2) - 1), d0 = place * 8;
     const bool has = d0 < a.dim;
     const int rot = 2 * a.half;
@@ -91,24 +142,27 @@ __global__ void __launch_bounds__(256) head_rows_fp4_kernel(const HeadRowsFp4Arg
     Words<BYTES> own[R], other[R];
     const char *source[R];
     int cls[R], head[R]; // query, key, value; -1: no row
+    const auto load = [&] { // the rows from `round` on
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int of_q = a.rounds[0], of_k = a.rounds[1];
-        cls[r] = round + r < of_q ? 0 : (round + r < of_q + of_k ? 1 : 2);
-        const int h = ((round + r - (cls[r] == 0 ? 0 : (cls[r] == 1 ? of_q : of_q + of_k))) << (6 - a.lanes_log2)) + (lane >> a.lanes_log2);
-        const bool there = h < (cls[r] == 0 ? a.heads[0] : (cls[r] == 1 ? a.heads[1] : a.heads[2])) && has;
-        head[r] = there ? h : -1;
-        const auto &late = arguments_again<HeadRowsFp4Args>();
-        source[r] = late.in[cls[r]] + token * late.in_token[cls[r]] + h * late.in_head[cls[r]];
-        own[r] = Words<BYTES>{};
-        if (there) own[r] = load_words<BYTES, (R > 1)>(source[r] + d0 * T::kBytes);
-        if constexpr (!INTERLEAVED && WHOLE) {
-            other[r] = Words<BYTES>{};
-            if (there && turned_apart && cls[r] != 2) other[r] = load_words<BYTES>(source[r] + (d0 + to_partner) * T::kBytes);
+        for (int r = 0; r < R; ++r) {
+            const int of_q = a.rounds[0], of_k = a.rounds[1];
+            cls[r] = round + r < of_q ? 0 : (round + r < of_q + of_k ? 1 : 2);
+            const int h = ((round + r - (cls[r] == 0 ? 0 : (cls[r] == 1 ? of_q : of_q + of_k))) << (6 - a.lanes_log2)) + (lane >> a.lanes_log2);
+            const bool there = h < (cls[r] == 0 ? a.heads[0] : (cls[r] == 1 ? a.heads[1] : a.heads[2])) && has;
+            head[r] = there ? h : -1;
+            const auto &late = arguments_again<HeadRowsFp4Args>();
+            source[r] = late.in[cls[r]] + token * late.in_token[cls[r]] + h * late.in_head[cls[r]];
+            own[r] = Words<BYTES>{};
+            if (there) own[r] = load_words<BYTES, (R > 1)>(source[r] + d0 * T::kBytes);
+            if constexpr (!INTERLEAVED && WHOLE) {
+                other[r] = Words<BYTES>{};
+                if (there && turned_apart && cls[r] != 2) other[r] = load_words<BYTES>(source[r] + (d0 + to_partner) * T::kBytes);
+            }
         }
-    }
+    };
+    load();
 
-    const Place where = place_of(a.batch, token, lane);
+    const Place where = place_at_once(a.batch, token, lane);
     const int64_t position = a.positions != nullptr ? explicit_position(a, token) : where.position;
     const bool known = position >= 0 && position < a.table_rows;
     const float *const row_of = a.cos_sin + (known ? position : 0) * a.table_stride;
@@ -164,87 +218,71 @@ __global__ void __launch_bounds__(256) head_rows_fp4_kernel(const HeadRowsFp4Arg
         other_gamma[i] = gammas_at(of, d0 + to_partner, turned_apart);
     }
 
+    for (int turn = 0;;) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        float x[8];
-        widen_all<T, 8>(own[r], x);
-        const auto norm_and_turn_row = [&](auto &v, const char *from, const Words<BYTES> &own_gamma, const Words<BYTES> &other_gamma) {
-            float y[8] = {}, gx[8], gy[8];
-            if constexpr (!INTERLEAVED && WHOLE) widen_all<T, 8>(other[r], y);
-            widen_all<T, 8>(own_gamma, gx);
-            widen_all<T, 8>(other_gamma, gy);
-            if constexpr (INTERLEAVED) {
+        for (int r = 0; r < R; ++r) {
+            float x[8];
+            widen_all<T, 8>(own[r], x);
+            const auto norm_and_turn_row = [&](auto exactly, const char *from, const Words<BYTES> &own_gamma, const Words<BYTES> &other_gamma) {
+                float y[8] = {}, gx[8], gy[8];
+                if constexpr (!INTERLEAVED && WHOLE) widen_all<T, 8>(other[r], y);
+                widen_all<T, 8>(own_gamma, gx);
+                widen_all<T, 8>(other_gamma, gy);
+                if constexpr (INTERLEAVED) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[i] = x[i ^ 1];
-                    gy[i] = gx[i ^ 1];
-                }
-            } else if constexpr (!WHOLE) { // one by one
-                if (head[r] >= 0)
                     for (int i = 0; i < 8; ++i) {
-                        if (((turned >> i) & 1) == 0) break;
-                        const int partner = d0 + i < a.half ? d0 + i + a.half : d0 + i - a.half;
-                        y[i] = load_element<T>(source[r] + partner * T::kBytes);
-                        if (from != nullptr) gy[i] = load_element<T>(from + partner * T::kBytes);
+                        y[i] = x[i ^ 1];
+                        gy[i] = gx[i ^ 1];
                     }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v.x[i] = x[i];
-                v.y[i] = y[i];
-            }
-            norm_and_turn<WHOLE>(v, from != nullptr, gx, gy, a.dim, a.eps, a.lanes_log2, turned, c, s);
-        };
-        if (cls[r] == 0) {
-            Channels<float> v;
-            norm_and_turn_row(v, a.gamma[0], gamma[0], other_gamma[0]);
-            if (head[r] >= 0) {
-                Words<BYTES> out = narrow_all<T, 8>(v.x);
-                if (where.position < 0) out = Words<BYTES>{};
-                store_words<BYTES, (R > 1)>(a.out[0] + token * a.out_token[0] + head[r] * a.out_head[0] + d0 * T::kBytes, out);
-            }
-            continue;
-        }
-        if (cls[r] == 1) {
-            if constexpr (R > 1 && !INTERLEAVED) { // as 64-bit numbers these are made anew for each row: kept, they would take the registers of more wavefronts
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float cosine = c[i], sine = s[i];
-                    asm volatile("" : "+v"(cosine), "+v"(sine));
-                    c[i] = cosine;
-                    s[i] = sine;
+                } else if constexpr (!WHOLE) { // one by one
+                    if (head[r] >= 0)
+                        for (int i = 0; i < 8; ++i) {
+                            if (((turned >> i) & 1) == 0) break;
+                            const int partner = d0 + i < a.half ? d0 + i + a.half : d0 + i - a.half;
+                            y[i] = load_element<T>(source[r] + partner * T::kBytes);
+                            if (from != nullptr) gy[i] = load_element<T>(from + partner * T::kBytes);
+                        }
                 }
-#pragma unroll
-                for (int i = 0; i < BYTES / 4; ++i) asm volatile("" : "+v"(gamma[K].w[i]), "+v"(other_gamma[K].w[i]));
+                if constexpr (decltype(exactly)::value) norm_and_turn_exactly<WHOLE>(x, y, from != nullptr, gx, gy, a.dim, a.eps, a.lanes_log2, turned, c, s);
+                else norm_and_turn<WHOLE>(x, y, from != nullptr, gx, gy, a.dim, a.eps, a.lanes_log2, turned, c, s);
+            };
+            if (cls[r] == 0) {
+                norm_and_turn_row(std::false_type{}, a.gamma[0], gamma[0], other_gamma[0]);
+                if (head[r] >= 0) {
+                    Words<BYTES> out = narrow_all<T, 8>(x);
+                    if (where.position < 0) out = Words<BYTES>{};
+                    store_words<BYTES, (R > 1)>(a.out[0] + token * a.out_token[0] + head[r] * a.out_head[0] + d0 * T::kBytes, out);
+                }
+                continue;
             }
-            Channels<double> v;
-            norm_and_turn_row(v, a.gamma[1], gamma[K], other_gamma[K]);
+            if (cls[r] == 1) norm_and_turn_row(std::true_type{}, a.gamma[1], gamma[K], other_gamma[K]);
+            uint32_t largest = 0; // magnitudes compare as whole numbers, infinities and NaN above all
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = cut(v.x[i]);
+            for (int i = 0; i < 8; ++i) largest = max(largest, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+            largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0xB1, 0xf, 0xf, false));
+            largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0x4E, 0xf, 0xf, false));
+            const bool finite = largest < 0x7f800000u;
+            const int exponent = (int)((largest + 0x00200000u) >> 23) - 2;
+            const uint32_t scale = finite ? (uint32_t)min(max(exponent, 2), a.most_exponent + 127) : 255u;
+            const float unit = __builtin_bit_cast(float, scale << 23);
+            uint32_t codes = 0;
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], unit, 0);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], unit, 1);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], unit, 2);
+            codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], unit, 3);
+            if (head[r] < 0 || where.page < 0) continue;
+            const auto &late = arguments_again<HeadRowsFp4Args>();
+            char *const to = late.out[cls[r]] + where.page * late.out_page[cls[r]] + where.slot * late.out_token[cls[r]] + head[r] * late.out_head[cls[r]];
+            store_words<4>(to + d0 / 2, Words<4>{{finite ? codes : 0u}});
+            if ((place & 3) == 0) {
+                const int i = cls[r] - 1;
+                char *const scale_to = late.scales[i] + where.page * late.scale_page[i] + where.slot * late.scale_slot[i] + head[r] * late.scale_head[i];
+                *(__attribute__((address_space(1))) uint8_t *)(scale_to + place / 4) = (uint8_t)scale;
+            }
         }
-        uint32_t largest = 0; // magnitudes compare as whole numbers, infinities and NaN above all
-#pragma unroll
-        for (int i = 0; i < 8; ++i) largest = max(largest, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
-        largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0xB1, 0xf, 0xf, false));
-        largest = max(largest, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)largest, 0x4E, 0xf, 0xf, false));
-        const bool finite = largest < 0x7f800000u;
-        const int exponent = (int)((largest + 0x00200000u) >> 23) - 2;
-        const uint32_t scale = finite ? (uint32_t)min(max(exponent, 2), a.most_exponent + 127) : 255u;
-        const float unit = __builtin_bit_cast(float, scale << 23);
-        uint32_t codes = 0;
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], unit, 0);
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], unit, 1);
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], unit, 2);
-        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], unit, 3);
-        if (head[r] < 0 || where.page < 0) continue;
-        const auto &late = arguments_again<HeadRowsFp4Args>();
-        char *const to = late.out[cls[r]] + where.page * late.out_page[cls[r]] + where.slot * late.out_token[cls[r]] + head[r] * late.out_head[cls[r]];
-        store_words<4>(to + d0 / 2, Words<4>{{finite ? codes : 0u}});
-        if ((place & 3) == 0) {
-            const int i = cls[r] - 1;
-            char *const scale_to = late.scales[i] + where.page * late.scale_page[i] + where.slot * late.scale_slot[i] + head[r] * late.scale_head[i];
-            *(__attribute__((address_space(1))) uint8_t *)(scale_to + place / 4) = (uint8_t)scale;
-        }
+        if (R == 1 || ++turn == a.turns) break;
+        round += R;
+        load();
     }
 }
 
@@ -257,10 +295,12 @@ int launch_head_rows_fp4(HeadRowsFp4Args &a, int dtype, hipStream_t s) {
     const int64_t rounds = (int64_t)a.rounds[0] + a.rounds[1] + a.rounds[2];
     const auto waves_of = [&](int rows) { return (rounds + rows - 1) / rows; };
     const bool whole = (a.interleaved ? 2 * a.half : a.half) % 8 == 0;
-    // Rows of a lane.  2048 tokens of 32 + 2 * 8 heads of 128 bf16 channels, and the caches' unpacking behind them, take 29 us with four and 32 with one,
-    // four times as many 75 and 108; fp32 rows of as many bytes take 81 with four, which cost it registers, and 75 with one; few rows are for all units.
+    // Rows of a lane, and how often it takes as many, which then share what a token has in common.  8192 tokens of 32 + 2 * 8 heads of 128 bf16 channels, and the
+    // caches' unpacking behind them, take 63 us with four rows three times, 74 with four once and 85 with one; 2048 tokens 27, 29 and 28; fp32 rows take 63 with one and 77 with four (4096 tokens), whose registers are too many.  Few rows are for all units.
     const int rows = whole && dtype != TDE_F32 && a.tokens * waves_of(4) >= 1024 ? 4 : 1;
-    const int64_t waves = waves_of(rows);
+    const int64_t all = waves_of(rows), least = rows == 1 ? all : std::min(all, std::max<int64_t>(1, 4096 / a.tokens)); // wavefronts of a token
+    a.turns = (int32_t)((all + least - 1) / least);
+    const int64_t waves = (all + a.turns - 1) / a.turns;
     if (a.tokens > (int64_t)0x7ffffff0 / waves) return TDE_ETOOBIG;
     const uint32_t blocks = (uint32_t)((a.tokens * waves + 3) / 4);
     if (!fits_launch(blocks, 256)) return TDE_ETOOBIG;
