@@ -94,6 +94,22 @@ def test_launches_that_do_not_fit():
         assert lib.tde_paged_attention_fp4_workspace(ctypes.byref(attention_fp4(**kw)), ctypes.byref(n)) == _capi.OK, kw
 
 
+def test_slots_far_apart_are_planned_another_way():
+    """Decode rows whose keys' offsets do not hold 32 bits take the tiles of 64 rows, as those over pages that 8 does not divide."""
+    lib, n = _capi.load(), ctypes.c_int64()
+
+    def workspace(page_size=16, **kw):
+        t = attention_fp4(tokens=1, batch=batch(seqs=1, page_size=page_size, table_pages=4096), **kw)
+        assert lib.tde_paged_attention_fp4_workspace(ctypes.byref(t), ctypes.byref(n)) == _capi.OK
+        return n.value
+
+    near, other = workspace(), workspace(page_size=17)
+    assert near != other
+    for name, base in (("k_cache", 64), ("v_cache", 64), ("k_scales", 4), ("v_scales", 4)):
+        assert workspace(**{name: _capi.Cache(SOMEWHERE, 4096, (1 << 27) - 64, base)}) == near
+        assert workspace(**{name: _capi.Cache(SOMEWHERE, 4096, 1 << 27, base)}) == workspace(page_size=12, **{name: _capi.Cache(SOMEWHERE, 4096, 64, base)}), name
+
+
 def test_scales_of_scores():
     """A scale whose product with log2(e) is no fp32 number would make every weight NaN."""
     lib, n = _capi.load(), ctypes.c_int64()

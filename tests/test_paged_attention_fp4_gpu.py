@@ -274,6 +274,24 @@ def test_far_pages(tde):
     assert_close(got, want, bound)
 
 
+@pytest.mark.parametrize("which", range(4), ids=["k_cache", "k_scales", "v_cache", "v_scales"])
+@pytest.mark.parametrize("new,lens", [([1, 2], [60, 75]), ([1, 150], [60, 275])], ids=["decode", "chunks"])
+def test_slots_far_apart(tde, which, new, lens):
+    """16 keys whose offsets from the first of them do not hold 32 bits."""
+    slot = (1 << 28) + (1 << 24)
+    batch = Batch(new=new, lens=lens, page_size=16, seed=14)
+    parts = held(batch, 1, 64, 7, heads_first=False)
+    here = on_gpu(parts)
+    width = here[which].size(3)
+    far = torch.zeros(15 * slot + batch.pages * width, dtype=torch.uint8, device="cuda")
+    here[which] = far.as_strided((batch.pages, 16, 1, width), (width, slot, width, 1)).copy_(here[which])
+    for dtype in (torch.bfloat16, torch.float16):
+        q = randn((batch.tokens, 2, 64), dtype, 8)
+        got = tde.paged_attention_fp4(q.cuda(), *here, *batch.on("cuda"))
+        want, bound = attention(batch, q, as_read(*parts[:2], dtype), as_read(*parts[2:], dtype), 64 ** -0.5)
+        assert_close(got, want, bound)
+
+
 def test_nothing_to_do(tde):
     batch = Batch(new=[0, 0], lens=[5, 0], page_size=4)
     parts = on_gpu(held(batch, 2, 64, 1))

@@ -124,7 +124,7 @@ int head_rows(const tde_head_rows *r, bool paged, void *hip_stream) {
 
 bool fp4_dim_ok(int dim) { return dim >= TDE_FP4_BLOCK && dim % TDE_FP4_BLOCK == 0; }
 
-int check_attention(const tde_attention *t, bool fp4, AttentionPlan *plan) {
+int check_attention(const tde_attention *t, const tde_attention_fp4 *fp4, AttentionPlan *plan) { // fp4: t in 4 bits, or null
     if (t == nullptr || t->reserved != 0) return TDE_EINVAL;
     if (t->dtype != TDE_BF16 && t->dtype != TDE_F16) return TDE_EDTYPE;
     if (t->tokens < 0 || t->tokens >= kMaxRows || t->dim < 1 || t->dim % 8 != 0) return TDE_ESHAPE;
@@ -137,13 +137,15 @@ int check_attention(const tde_attention *t, bool fp4, AttentionPlan *plan) {
     const int st = check_batch(t->batch);
     if (st != TDE_OK) return st;
     const int64_t capacity = (int64_t)t->batch.table_pages * t->batch.page_size;
-    return fp4 ? plan_attention_fp4(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch, plan)
-               : plan_attention(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch.seqs, capacity, plan);
+    if (fp4 == nullptr) return plan_attention(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch.seqs, capacity, plan);
+    bool near = true;
+    for (const tde_cache *c : {&t->k_cache, &t->v_cache, &fp4->k_scales, &fp4->v_scales}) near = near && c->slot_stride < kNearSlots;
+    return plan_attention_fp4(t->dim, t->tokens, t->q_heads, t->kv_heads, t->batch, near, plan);
 }
 
 int check_attention_fp4(const tde_attention_fp4 *t, AttentionPlan *plan) {
     if (t == nullptr || t->reserved != 0) return TDE_EINVAL;
-    const int st = check_attention(&t->attention, true, plan);
+    const int st = check_attention(&t->attention, t, plan);
     if (st != TDE_OK) return st;
     if (!fp4_dim_ok(t->attention.dim)) return TDE_ESHAPE;
     for (const tde_cache *c : {&t->k_scales, &t->v_scales})
@@ -213,7 +215,7 @@ int tde_append_kv(const tde_head_rows *rows, void *hip_stream) { return head_row
 int tde_paged_attention_workspace(const tde_attention *t, int64_t *bytes) {
     if (bytes == nullptr) return TDE_EINVAL;
     AttentionPlan plan;
-    const int st = check_attention(t, false, &plan);
+    const int st = check_attention(t, nullptr, &plan);
     if (st != TDE_OK) return st;
     *bytes = t->tokens == 0 ? 0 : plan.workspace_bytes;
     return TDE_OK;
@@ -222,7 +224,7 @@ int tde_paged_attention_workspace(const tde_attention *t, int64_t *bytes) {
 int tde_paged_attention(const tde_attention *t, void *hip_stream) {
     AttentionPlan plan;
     AttentionArgs a{};
-    int st = check_attention(t, false, &plan);
+    int st = check_attention(t, nullptr, &plan);
     if (st != TDE_OK || t->tokens == 0) return st;
     st = attention_args(t, plan, 2, a);
     return st != TDE_OK ? st : launch_attention(a, plan, t->dtype, static_cast<hipStream_t>(hip_stream));

@@ -68,7 +68,9 @@ struct AttentionPlan {
 
 int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p);
 int plan_attention_rows(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, int least_rows, AttentionPlan *p);
-int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const tde_paged_batch &b, AttentionPlan *p);
+// Bytes between slots below which a lane's offset from the first of 16 keys holds 32 bits.
+constexpr int64_t kNearSlots = 1 << 27;
+int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const tde_paged_batch &b, bool near, AttentionPlan *p); // near: all slots
 int launch_attention(AttentionArgs &a, const AttentionPlan &p, int dtype, hipStream_t s);
 int launch_attention_fp4(AttentionFp4Args &a, const AttentionPlan &p, int dtype, hipStream_t s);
 

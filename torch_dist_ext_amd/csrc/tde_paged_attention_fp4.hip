@@ -810,9 +810,9 @@ int plan_tiles(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int
 
 } // namespace
 
-int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const tde_paged_batch &b, AttentionPlan *p) {
+int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const tde_paged_batch &b, bool near, AttentionPlan *p) {
     const int64_t rows_all = tokens * (q_heads / kv_heads), capacity = (int64_t)b.table_pages * b.page_size;
-    if (b.page_size % 8 != 0 || b.table_pages == 0 || b.cache_pages == 0 || rows_all > (int64_t)b.seqs * 16)
+    if (!near || b.page_size % 8 != 0 || b.table_pages == 0 || b.cache_pages == 0 || rows_all > (int64_t)b.seqs * 16)
         return plan_tiles(dim, tokens, q_heads, kv_heads, b.seqs, capacity, p);
     *p = AttentionPlan{};
     p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);

@@ -245,6 +245,13 @@ __device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t lane_offset,
     if constexpr (STREAM) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(lane_offset), "s"(base), "s"(lds) : "memory", "m0");
     else asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(lane_offset), "s"(base), "s"(lds) : "memory", "m0");
 }
+// Whether 16 keys lie in one page and lanes' offsets from the first of them hold 32 bits.
+template <class C>
+__device__ __forceinline__ bool scalar_rows_of([[maybe_unused]] const typename C::Args &a) {
+    if constexpr (C::kFp4) return a.batch.page.d % 16 == 0 && (a.k_slot | a.v_slot | a.k_scale_slot | a.v_scale_slot) < (uint32_t)kNearSlots && a.batch.cache_pages > 0;
+    return false;
+}
+
 // The kernel's arguments, for what is done at its end: those of caches in 4 bits are too many for the scalar registers.
 template <class C>
 __device__ __forceinline__ const typename C::Args &late_arguments([[maybe_unused]] const typename C::Args &a) {
@@ -477,8 +484,8 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
         mine = held(takes_values);
         asm volatile("" : "+s"(mine.codes), "+s"(mine.scales), "+s"(mine.page), "+s"(mine.slot), "+s"(mine.scale_page), "+s"(mine.scale_slot));
     }
-    // Where 16 keys lie in one page, and lanes' offsets hold 32 bits, a wavefront's rows (8, 16 or twice 16) have scalar addresses.
-    [[maybe_unused]] const bool scalar_rows = FP4 && a.batch.page.d % 16 == 0 && (a.k_slot | a.v_slot) < 1u << 27 && a.batch.cache_pages > 0;
+    // A wavefront's rows (8, 16 or twice 16) then have scalar addresses.
+    [[maybe_unused]] const bool scalar_rows = scalar_rows_of<C>(a);
     const auto fetch = [&]([[maybe_unused]] int32_t key0, [[maybe_unused]] uint64_t &lost) { // look_up has been called for the tile
         if constexpr (FP4) {
             const uint32_t first = a.batch.page.quotient((uint32_t)key0) - (uint32_t)window;
