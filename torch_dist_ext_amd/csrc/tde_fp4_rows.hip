@@ -1,7 +1,8 @@
 // Codes and scales of a cache in 4 bits as numbers of T: T(code * 2^(e - 127)), one rounding (none in bf16 and fp32 but among subnormal numbers).
 //
 // Bound by memory, by what is written: a lane turns 4 bytes of codes into 8 numbers, so that a wavefront's stores are whole lines, and past the caches:
-// 131072 rows of 8 heads of 128 channels take 51 us, 6.7 TB/s, and 63 with stores that stay in the caches.
+// 131072 rows of 8 heads of 128 channels take 51 us, 6.7 TB/s, and 63 with stores that stay in the caches.  (Four such pieces a lane: 51 us, and 512 rows of
+// a head 2.8 and not 2.2.)
 #include "tde_fp4_rows.h"
 
 namespace tde {
@@ -31,37 +32,23 @@ __device__ __forceinline__ Words<8 * T::kBytes> numbers(uint32_t codes, float sc
 
 } // namespace
 
-template <class T, int U>
+template <class T>
 __global__ void __launch_bounds__(256) unpack_fp4_kernel(const UnpackArgs a) {
-    const uint64_t first = (uint64_t)blockIdx.x * (256 * U) + threadIdx.x;
-    Words<4> codes[U];
-    uint32_t scale[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint64_t i = first + u * 256;
-        codes[u] = {};
-        scale[u] = 0;
-        if (i >= a.total) continue;
-        const uint32_t row = a.pieces.quotient((uint32_t)i), piece = (uint32_t)i - row * a.pieces.d;
-        const uint32_t outer = a.inner.quotient(row), n2 = row - outer * a.inner.d, n0 = a.middle.quotient(outer), n1 = outer - n0 * a.middle.d;
-        codes[u] = load_words<4>(a.codes + n0 * a.code_stride[0] + n1 * a.code_stride[1] + n2 * a.code_stride[2] + piece * 4);
-        scale[u] = *(const __attribute__((address_space(1))) uint8_t *)(a.scales + n0 * a.scale_stride[0] + n1 * a.scale_stride[1] + n2 * a.scale_stride[2] +
-                                                                        piece / 4);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint64_t i = first + u * 256;
-        if (i >= a.total) continue;
-        store_words<8 * T::kBytes, true>(a.out + i * (8 * T::kBytes), numbers<T>(codes[u].w[0], __builtin_bit_cast(float, scale[u] << 23)));
-    }
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.total) return;
+    const uint32_t row = a.pieces.quotient(i), piece = i - row * a.pieces.d;
+    const uint32_t outer = a.inner.quotient(row), n2 = row - outer * a.inner.d, n0 = a.middle.quotient(outer), n1 = outer - n0 * a.middle.d;
+    const Words<4> codes = load_words<4>(a.codes + n0 * a.code_stride[0] + n1 * a.code_stride[1] + n2 * a.code_stride[2] + piece * 4);
+    const uint32_t scale = *(const __attribute__((address_space(1))) uint8_t *)(a.scales + n0 * a.scale_stride[0] + n1 * a.scale_stride[1] +
+                                                                               n2 * a.scale_stride[2] + piece / 4);
+    store_words<8 * T::kBytes, true>(a.out + (uint64_t)i * (8 * T::kBytes), numbers<T>(codes.w[0], __builtin_bit_cast(float, scale << 23)));
 }
 
 int launch_unpack_fp4(const UnpackArgs &a, int out_dtype, hipStream_t s) {
-    constexpr int U = 4;
-    const uint32_t blocks = (uint32_t)(((uint64_t)a.total + 256 * U - 1) / (256 * U));
-    if (out_dtype == TDE_BF16) unpack_fp4_kernel<Bf16, U><<<blocks, 256, 0, s>>>(a);
-    else if (out_dtype == TDE_F16) unpack_fp4_kernel<F16, U><<<blocks, 256, 0, s>>>(a);
-    else unpack_fp4_kernel<F32, U><<<blocks, 256, 0, s>>>(a);
+    const uint32_t blocks = ((uint32_t)a.total + 255) / 256;
+    if (out_dtype == TDE_BF16) unpack_fp4_kernel<Bf16><<<blocks, 256, 0, s>>>(a);
+    else if (out_dtype == TDE_F16) unpack_fp4_kernel<F16><<<blocks, 256, 0, s>>>(a);
+    else unpack_fp4_kernel<F32><<<blocks, 256, 0, s>>>(a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? TDE_OK : hip_failed(e);
 }
