@@ -24,9 +24,25 @@ namespace block {
 
 namespace {
 
+template <int CONTROL>
+__device__ __forceinline__ float from_lane(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CONTROL, 0xf, 0xf, false));
+}
+template <int CONTROL>
+__device__ __forceinline__ double from_lane(double x) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)bits, CONTROL, 0xf, 0xf, false);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(bits >> 32), CONTROL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)high << 32 | low);
+}
+// Over 4, 8, 16 or 32 neighbouring lanes, the same sum in each.
 template <class A>
 __device__ __forceinline__ A sum_over_lanes(A x, int log2) {
-    for (int m = 0; m < log2; ++m) x += __shfl_xor(x, 1 << m);
+    x += from_lane<0xb1>(x);               // the neighbour's
+    x += from_lane<0x4e>(x);               // the other two's of four
+    if (log2 > 2) x += from_lane<0x141>(x); // mirrored in eight
+    if (log2 > 3) x += from_lane<0x140>(x); // in sixteen
+    if (log2 > 4) x += __shfl_xor(x, 16);
     return x;
 }
 
