@@ -757,8 +757,23 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
                     for (int r = 0; r < 4; ++r) s[n][kb][r] -= away[n];
         }
         u32x4 p[NB][KT / 32], rest[NB][REST ? KT / 32 : 1];
+        // Over caches in 4 bits weights are made two by two, those of the second 32 keys only while the matrix units are at the first's values (4096 rows behind
+        // 4096 in heads of 128: 382 us, and 395 all ahead; heads of 64 have no registers for it: 60.1 and 58.9).
+        constexpr bool LATE = FP4 && D == 128;
+        [[maybe_unused]] const auto weigh = [&](int n, int ks, int w) {
+            const f32x4 x = s[n][2 * ks + (w >> 1)];
+            const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[(w & 1) * 2], a.scale_log2, -shift[n]));
+            const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[(w & 1) * 2 + 1], a.scale_log2, -shift[n]));
+            p[n][ks][w] = T::narrow(x0, x1);
+        };
+        if constexpr (LATE) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) weigh(n, 0, w);
+        }
+#pragma unroll
+        for (int n = 0; n < (LATE ? 0 : NB); ++n) {
 #pragma unroll
             for (int kb = 0; kb < KT / 16; ++kb)
 #pragma unroll
@@ -884,7 +899,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
         }
         const uint32_t ones = T::narrow(1.0f, 1.0f);
 #pragma unroll
-        for (int ks = 0; ks < KT / 32; ++ks)
+        for (int ks = 0; ks < (LATE ? 1 : KT / 32); ++ks)
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 l[n] = Mfma<T>::mul(u32x4{ones, ones, ones, ones}, p[n][ks], l[n]);
@@ -904,13 +919,28 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
                 const int ks = unit / (D / 16 / U), d = unit % (D / 16 / U) * U;
                 if (unit + 1 < UNITS) read(unit + 1);
                 __builtin_amdgcn_sched_barrier(0);
+                if constexpr (LATE) {
+                    if (unit == UNITS / 2) {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                        for (int n = 0; n < NB; ++n) l[n] = Mfma<T>::mul(u32x4{ones, ones, ones, ones}, p[n][1], l[n]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
                         o[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], p[n][ks], o[n][d + u]);
                         if constexpr (REST) o_rest[n][d + u] = Mfma<T>::mul(vf[unit & 1][u], rest[n][ks], o_rest[n][d + u]);
                     }
+                    if constexpr (LATE) {
+                        constexpr int SLOTS = UNITS / 2 * U, EACH = (NB * 4 + SLOTS - 1) / SLOTS;
+                        const int slot = unit * U + u;
+#pragma unroll
+                        for (int i = slot * EACH; i < (slot + 1) * EACH; ++i)
+                            if (slot < SLOTS && i < NB * 4) weigh(i / 4, 1, i % 4);
+                        if (slot < SLOTS) __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
             }
         }
 
