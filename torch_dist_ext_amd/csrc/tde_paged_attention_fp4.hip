@@ -796,9 +796,9 @@ void launch_decode_type(const AttentionFp4Args &a, const AttentionPlan &p, hipSt
 namespace {
 
 // Tiles that share keys.  Heads of 65 to 128 take 256 rows where those are two workgroups a unit at most and sequences are long (128 rows, two workgroups
-// at once, make numbers of all codes twice): 4096 rows behind 4096 396 us and 427, 3700 behind 8000 604 and 660, 2 x 2048 behind 2048 218 and 246, 3100 by
-// themselves 107 and 107.  Elsewhere a unit that gets one tile more than others costs what that saves: 5000 rows behind 2000 434 and 416, 8192 by themselves 558
-// and 572, 20 sequences of up to 700 behind 3000 131 and 121.
+// at once, make numbers of all codes twice): 4096 rows behind 4096 382 us and 415, 3700 behind 8000 582 and 644, 2 x 2048 behind 2048 206 and 236, 3100 by
+// themselves 101 and 103.  Elsewhere a unit that gets one tile more than others costs what that saves: 5000 rows behind 2000 413 and 399, 8192 by themselves 526
+// and 545, 20 sequences of up to 700 behind 3000 129 and 117.
 int plan_tiles(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
     const int status = plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 64, p);
     if (status != TDE_OK || p->rows != 128 || p->wide_dim != 128) return status;
