@@ -52,6 +52,21 @@ def test_largest_tiles(tde, new, lens, dim, page, dtype):
     run(tde, batch, 64, 8, dim, dtype, seed=4, parts=parts, reference=attention_at_once)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page,new,seqs", [
+    (8, 2, 64, 16, 6, 12), (8, 2, 64, 8, 8, 70), (16, 4, 128, 64, 8, 9), (16, 4, 96, 8, 7, 60), (12, 2, 256, 16, 14, 5), (12, 2, 192, 8, 10, 33), (24, 1, 128, 16, 1, 40)])
+def test_a_few_tiles_each(tde, heads, kv_heads, dim, page, new, seqs):
+    """More than one tile of 16 rows a sequence, on both sides of where larger tiles begin."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = [new + int(x) for x in torch.randint(0, 400, (seqs,), generator=g)]
+    lens[0] = 3000
+    for more, dtype in ((0, torch.bfloat16), (new // 2, torch.float16), (3 * new, torch.bfloat16)):
+        batch = Batch([new + more] * seqs, [n + more for n in lens], page, seed=seqs, pad=3)
+        batch.table[2, 0] = -1
+        run(tde, batch, heads, kv_heads, dim, dtype, seed=dim)
+    uneven = torch.randint(0, 2 * new + 1, (seqs,), generator=g).tolist()
+    run(tde, Batch(uneven, [n + m for n, m in zip(uneven, lens)], page, seed=seqs + 1, pad=20), heads, kv_heads, dim, torch.bfloat16, seed=dim + 1, heads_first=False)
+
+
 def test_more_heads_than_the_device_holds_workgroups(tde):
     run(tde, Batch([1, 1], [70, 9], 8, seed=1), 1100, 1100, 32, torch.bfloat16, seed=2)
     run(tde, Batch([20], [33], 8, seed=3), 1100, 1100, 32, torch.bfloat16, seed=4)

@@ -791,9 +791,15 @@ void launch_decode_type(const AttentionFp4Args &a, const AttentionPlan &p, hipSt
 
 } // namespace
 
-// Which kernel.  Calls whose sequences have no more than 16 rows on average go to the decode kernel, which takes pages of whole 8 keys, and a table and caches that
-// have any; the others to tiles of 64 or 128 rows, as plan_attention says.
 namespace {
+
+// Which kernel.  Calls whose sequences have few rows on average go to the decode kernel, tiles of 16 rows; the others to tiles of 64 and more.  How many are few:
+// 16; with heads of up to 64 channels 32 where tiles of 64 would leave units idle (48 sequences of 6 x 4 rows over 6000 keys 55 us, tiles of 64 69; but 300 over
+// 600 85 and 76), of up to 128 32 (64 sequences of 8 x 4 over 4000 115 and 120, of up to as many 69 and 94; with 48 153 and 121), of more 96, as tiles of 64
+// leave them one wavefront a SIMD (20 of 8 x 6 over 6000 97 and 155, of 24 x 4 over 6000 171 and 351; 64 of up to 30 x 4 over 500 57 and 52).
+int64_t few_rows(int wide_dim, int64_t tiles) {
+    return wide_dim == 256 ? 96 : (wide_dim == 128 || tiles < device_compute_units() ? 32 : 16);
+}
 
 // Tiles that share keys.  Heads of 65 to 128 take 256 rows where those are two workgroups a unit at most and sequences are long (128 rows, two workgroups
 // at once, make numbers of all codes twice): 4096 rows behind 4096 382 us and 415, 3700 behind 8000 582 and 644, 2 x 2048 behind 2048 206 and 236, 3100 by
@@ -813,17 +819,19 @@ int plan_tiles(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int
 
 int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const tde_paged_batch &b, bool near, AttentionPlan *p) {
     const int64_t rows_all = tokens * (q_heads / kv_heads), capacity = (int64_t)b.table_pages * b.page_size;
-    if (!near || b.page_size % 8 != 0 || b.table_pages == 0 || b.cache_pages == 0 || rows_all > (int64_t)b.seqs * 16)
+    const int wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
+    // (It takes pages of whole 8 keys, and a table and caches that have any.)
+    if (!near || b.page_size % 8 != 0 || b.table_pages == 0 || b.cache_pages == 0 || rows_all > b.seqs * few_rows(wide_dim, (int64_t)b.seqs * kv_heads))
         return plan_tiles(dim, tokens, q_heads, kv_heads, b.seqs, capacity, p);
     *p = AttentionPlan{};
-    p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
+    p->wide_dim = wide_dim;
     p->rows = 16;
     // As many runners as the device holds workgroups, by their registers; every die the same number.
     const int64_t tiles = rows_all / 16 + b.seqs + 2;
     const int64_t most = std::max<int64_t>(kDecodeWaves, (capacity + kUnit) / kUnit); // units of a tile
     if (tiles > 0x7fffff00 / most) return plan_tiles(dim, tokens, q_heads, kv_heads, b.seqs, capacity, p); // units are counted in 32 bits
     const int64_t at_once = std::max<int64_t>(1, std::min<int64_t>((int64_t)resident_workgroups(p->wide_dim, b.page_size % 16 == 0 ? 16 : 8) * device_compute_units() / kv_heads, kMostRunners));
-    const int64_t likely = std::max<int64_t>(1, std::min<int64_t>(b.seqs, tokens)); // tiles
+    const int64_t likely = std::max<int64_t>({1, std::min<int64_t>(b.seqs, tokens), rows_all / 16}); // tiles
     // Where tiles alone fill the device more than twice each is a runner's, and nothing is cut (200 rows over 1500 keys 52 us and 61, 512 over 2047 216 and 225).
     p->whole_tiles = likely >= 2 * at_once;
     p->runners = p->whole_tiles ? tiles : std::min(at_once >= 8 ? at_once & ~(int64_t)7 : at_once, (tiles * most + kDecodeWaves - 1) / kDecodeWaves);
