@@ -35,7 +35,7 @@ def test_tiles_alone_fill_the_device(tde, dim, seqs, page):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
-@pytest.mark.parametrize("dim,page", [(96, 24), (128, 16), (128, 64)])
+@pytest.mark.parametrize("dim,page", [(96, 24), (128, 16), (128, 64), (256, 16)])
 @pytest.mark.parametrize("new,lens", [([1650, 0, 130], [2000, 5, 130]), ([2300, 900, 1500], [2300, 1000, 3000]), ([1950, 100], [2200, 130])],
                          ids=["few", "many", "long"])
 def test_largest_tiles(tde, new, lens, dim, page, dtype):

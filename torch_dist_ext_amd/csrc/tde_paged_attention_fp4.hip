@@ -805,13 +805,25 @@ int64_t few_rows(int wide_dim, int64_t tiles) {
 // at once, make numbers of all codes twice): 4096 rows behind 4096 382 us and 415, 3700 behind 8000 582 and 644, 2 x 2048 behind 2048 206 and 236, 3100 by
 // themselves 101 and 103.  Elsewhere a unit that gets one tile more than others costs what that saves: 5000 rows behind 2000 413 and 399, 8192 by themselves 526
 // and 545, 20 sequences of up to 700 behind 3000 129 and 117.
+//
+// Heads of more than 128 take 128 rows, two wavefronts a SIMD, where those give three units of eight a tile, of two sequences at most two of eight; fewer are split,
+// in tiles of 64 rows, whose one wavefront a SIMD is slow: 1200 rows x 4 on 4 key heads behind 4000 243 us and 432, 600 214 and 260, 450 208 and 155; of 8 sequences of
+// up to 200 behind 8000 300 and 320, of 12 of up to 120 336 and 249.
 int plan_tiles(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
     const int status = plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 64, p);
-    if (status != TDE_OK || p->rows != 128 || p->wide_dim != 128) return status;
-    const int64_t rows_all = tokens * (q_heads / kv_heads);
-    if (rows_all < (int64_t)seqs * 8192 || rows_all / 256 * kv_heads > 2 * (int64_t)device_compute_units()) return status;
-    p->rows = 256;
-    p->tiles = p->items = rows_all / 256 + seqs + 2; // no more than of 128 rows, but their workgroups have twice the threads
+    if (status != TDE_OK) return status;
+    const int64_t rows_all = tokens * (q_heads / kv_heads), cus = device_compute_units();
+    if (p->wide_dim == 256 && p->rows == 64 && rows_all / 128 * kv_heads >= cus * (seqs <= 2 ? 2 : 3) / 8) {
+        *p = AttentionPlan{};
+        p->wide_dim = 256;
+        p->rows = 128;
+        p->join_waves = 1;
+    } else if (p->wide_dim == 128 && p->rows == 128 && rows_all >= (int64_t)seqs * 8192 && rows_all / 256 * kv_heads <= 2 * cus) {
+        p->rows = 256;
+    } else {
+        return TDE_OK;
+    }
+    p->tiles = p->items = rows_all / p->rows + seqs + 2;
     return fits_launch(p->items * kv_heads, 512) ? TDE_OK : TDE_ETOOBIG;
 }
 
