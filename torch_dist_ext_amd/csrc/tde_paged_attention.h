@@ -63,11 +63,12 @@ struct AttentionPlan {
     int join_waves; // wavefronts that join a row
     int64_t runners, most_each; // caches in 4 bits, tiles of 16 rows
     bool whole_tiles;
+    bool two_numbers; // caches in 4 bits, tiles of 64 rows: weights as two numbers of T
     int64_t workspace_bytes;
 };
 
 int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p);
-int plan_attention_rows(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, int least_rows, AttentionPlan *p);
+int plan_attention_rows(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, int least_rows, int most_rows, AttentionPlan *p);
 // Bytes between slots below which a lane's offset from the first of 16 keys holds 32 bits.
 constexpr int64_t kNearSlots = 1 << 27;
 int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const tde_paged_batch &b, bool near, AttentionPlan *p); // near: all slots

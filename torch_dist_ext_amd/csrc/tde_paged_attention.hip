@@ -19,17 +19,17 @@ namespace block {
 // sees rows, not lengths, those of no sequence included: one long sequence among many, or decode rows beside chunks that fill the
 // units, are walked by one workgroup a key head.
 int plan_attention(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
-    return plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 16, p);
+    return plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 16, 128, p);
 }
 
-// least_rows: of a tile.
-int plan_attention_rows(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, int least_rows, AttentionPlan *p) {
+// least_rows, most_rows: of a tile.
+int plan_attention_rows(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, int least_rows, int most_rows, AttentionPlan *p) {
     *p = AttentionPlan{};
     p->wide_dim = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
     const int64_t group = q_heads / kv_heads, rows_all = tokens * group, cus = device_compute_units();
     if (rows_all > 0x7fffff00) return TDE_ETOOBIG;
     if (rows_all <= (int64_t)seqs * 16 && least_rows == 16) p->rows = 16;
-    else p->rows = rows_all / 128 * kv_heads >= (p->wide_dim <= 128 ? 3 : 1) * cus ? 128 : 64;
+    else p->rows = most_rows >= 128 && rows_all / 128 * kv_heads >= (p->wide_dim <= 128 ? 3 : 1) * cus ? 128 : 64;
     const int64_t tiles = rows_all / p->rows + seqs + 2; // at most: one part tile a sequence, one in front of them and one behind
     const int64_t likely = std::max<int64_t>(1, std::max(rows_all / p->rows, std::min<int64_t>(seqs, tokens))); // rather
     p->min_chunk = 256;

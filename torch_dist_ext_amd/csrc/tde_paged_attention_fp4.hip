@@ -809,10 +809,15 @@ int64_t few_rows(int wide_dim, int64_t tiles) {
 // Heads of more than 128 take 128 rows, two wavefronts a SIMD, where those give three units of eight a tile, of two sequences at most two of eight; fewer are split,
 // in tiles of 64 rows, whose one wavefront a SIMD is slow: 1200 rows x 4 on 4 key heads behind 4000 243 us and 432, 600 214 and 260, 450 208 and 155; of 8 sequences of
 // up to 200 behind 8000 300 and 320, of 12 of up to 120 336 and 249.
+//
+// Calls of 16 rows a sequence and less that the decode kernel does not take have their weights as two numbers, as it has, in tiles of 64 rows, of which they fill few (64
+// rows over up to 8192 keys in pages of 12 tokens 201 us, one number 183; 48 x 3 over up to 6000 in heads of 64 60 and 42; 20 over up to 6000 in heads of 256 238 and 197).
 int plan_tiles(int dim, int64_t tokens, int q_heads, int kv_heads, int seqs, int64_t capacity, AttentionPlan *p) {
-    const int status = plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 64, p);
-    if (status != TDE_OK) return status;
     const int64_t rows_all = tokens * (q_heads / kv_heads), cus = device_compute_units();
+    const bool two_numbers = rows_all <= (int64_t)seqs * 16;
+    const int status = plan_attention_rows(dim, tokens, q_heads, kv_heads, seqs, capacity, 64, two_numbers ? 64 : 128, p);
+    p->two_numbers = two_numbers;
+    if (status != TDE_OK || two_numbers) return status;
     if (p->wide_dim == 256 && p->rows == 64 && rows_all / 128 * kv_heads >= cus * (seqs <= 2 ? 2 : 3) / 8) {
         *p = AttentionPlan{};
         p->wide_dim = 256;

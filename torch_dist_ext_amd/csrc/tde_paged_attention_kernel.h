@@ -10,7 +10,7 @@
 // a lane, and a lane's scores of two key blocks are, converted to T, its operand of the second product without any exchange: the
 // product's keys only need the same order on both sides, and V' is read from LDS with transposing loads in just that order.
 // The weights go into the second product, whose operands are T, rounded to T, and their sum is that of the rounded ones: one more product, with
-// a row of ones.  Where calls wait for the caches' bytes (16 rows a tile) what the rounding leaves goes in as a second operand, into sums of
+// a row of ones.  In calls of 16 rows a sequence and less, which wait for the caches' bytes, what the rounding leaves goes in as a second operand, into sums of
 // its own: the result is then off by its own rounding alone (error against doubles 0.0017 in place of 0.0022 in bf16; 64 rows over up to 8192
 // keys 195.9 us and 194.8, one over 131072 24.5 and 23.9).  Chunks wait for their instructions, and stay with one: 4096 rows behind 4096
 // take 406 us, with two operands 540.
@@ -272,12 +272,13 @@ __device__ __forceinline__ void wait_for_loads() {
 // otherwise all have the same rows and take the tiles in turn, each through LDS of its own, and are joined at the end.
 // (Heads of 64: four workgroups a unit hide the loads, with the registers of three 8 rows over 16000 keys take 24.0 us in place of 20.2, and 24 sequences
 // of up to 512 rows over a cache in 4 bits 78 in place of 61.)
-constexpr int workgroups_a_unit(bool fp4, int dim, int nb, bool shared, bool split) {
-    return dim == 256 ? 1 : (dim == 64 && (!shared || (fp4 && nb == 1 && !split)) ? 4 : 2);
+constexpr int workgroups_a_unit(bool fp4, int dim, int nb, bool shared, bool split, bool rest) {
+    return dim == 256 ? 1 : (dim == 64 && (!shared || (fp4 && nb == 1 && !split && !rest)) ? 4 : 2);
 }
 
-template <class T, class C, int D, int NB, int WAVES, bool SHARED, bool SPLIT>
-__global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, SHARED, SPLIT)) attention_kernel(const typename C::Args a) {
+// REST: weights as two numbers of T.
+template <class T, class C, int D, int NB, int WAVES, bool SHARED, bool SPLIT, bool REST = !SHARED>
+__global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, SHARED, SPLIT, REST)) attention_kernel(const typename C::Args a) {
     constexpr bool FP4 = C::kFp4;
     constexpr int KT = SHARED && D <= 128 ? 64 : 32; // keys a tile
     constexpr int CH = D / 8;                        // chunks of 16 bytes a row
@@ -286,7 +287,6 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
     constexpr int AT_ONCE = 64 / CH;                  // rows of a load
     constexpr int LOADS = KT / AT_ONCE / LOADERS;     // a wavefront, of keys and of values
     constexpr int TILE = KT * D * 2;
-    constexpr bool REST = !SHARED; // weights as two numbers of T
     constexpr int BUFFERS = SHARED ? 2 : WAVES;
     constexpr int JOIN = SHARED ? 0 : WAVES * 16 * NB * (D + 4) * 4;
     constexpr int LDS = 2 * TILE * BUFFERS > JOIN ? 2 * TILE * BUFFERS : JOIN;
@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
         u32x4 p[NB][KT / 32], rest[NB][REST ? KT / 32 : 1];
         // Over caches in 4 bits weights are made two by two, those of the second 32 keys only while the matrix units are at the first's values (4096 rows behind
         // 4096 in heads of 128: 382 us, and 395 all ahead; heads of 64 have no registers for it: 60.1 and 58.9).
-        constexpr bool LATE = FP4 && D == 128;
+        constexpr bool LATE = FP4 && D == 128 && !REST;
         [[maybe_unused]] const auto weigh = [&](int n, int ks, int w) {
             const f32x4 x = s[n][2 * ks + (w >> 1)];
             const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[(w & 1) * 2], a.scale_log2, -shift[n]));
@@ -1122,14 +1122,14 @@ __global__ void __launch_bounds__(64 * RW * WAVES) attention_join_kernel(const t
 }
 namespace {
 
-template <class T, class C, int D, int NB, int WAVES, bool SHARED>
+template <class T, class C, int D, int NB, int WAVES, bool SHARED, bool REST = !SHARED>
 void launch_one(const typename C::Args &a, const AttentionPlan &p, uint32_t blocks, hipStream_t s) {
     constexpr int ROWS = 16 * NB * (SHARED ? WAVES : 1);
     if (!p.split) {
-        attention_kernel<T, C, D, NB, WAVES, SHARED, false><<<blocks, 64 * WAVES, 0, s>>>(a);
+        attention_kernel<T, C, D, NB, WAVES, SHARED, false, REST><<<blocks, 64 * WAVES, 0, s>>>(a);
         return;
     }
-    attention_kernel<T, C, D, NB, WAVES, SHARED, true><<<blocks, 64 * WAVES, 0, s>>>(a);
+    attention_kernel<T, C, D, NB, WAVES, SHARED, true, REST><<<blocks, 64 * WAVES, 0, s>>>(a);
     const uint32_t joins = (uint32_t)a.tiles * a.kv_heads.d;
     if (p.join_waves == 16) attention_join_kernel<T, C, D, ROWS, 1, 16><<<joins * ROWS, 1024, 0, s>>>(a);
     else attention_join_kernel<T, C, D, ROWS, 4, 1><<<joins * (ROWS / 4), 256, 0, s>>>(a);
@@ -1146,6 +1146,9 @@ void launch_dim(const typename C::Args &a, const AttentionPlan &p, uint32_t bloc
             attention_kernel<T, C, D, 2, 8, true, false><<<blocks, 512, 0, s>>>(a);
             return;
         }
+    }
+    if constexpr (C::kFp4) {
+        if (p.two_numbers) return launch_one<T, C, D, 1, 4, true, true>(a, p, blocks, s);
     }
     if (p.rows == 64) launch_one<T, C, D, 1, 4, true>(a, p, blocks, s);
     else attention_kernel<T, C, D, D <= 128 ? 2 : 1, D <= 128 ? 4 : 8, true, false><<<blocks, D <= 128 ? 256 : 512, 0, s>>>(a); // 128, never split
