@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(64 * WAVES, resident_workgroups(D, SPAN)) deco
 #pragma unroll
             for (int c = 0; c < E; ++c) o[c] = f32x4{0, 0, 0, 0};
 
-            const auto work = [&](const Step<D> &s, int32_t key0, uint32_t lost) {
+            const auto work = [&](Step<D> &s, int32_t key0, uint32_t lost) {
                 // ---- scores ----
                 f32x4 score[2];
 #pragma unroll
@@ -474,29 +474,71 @@ __global__ void __launch_bounds__(64 * WAVES, resident_workgroups(D, SPAN)) deco
                         vf[1][i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i], 0x07060302u);
                     }
                 };
-                // A NaN block that not all rows see: a weight of zero would not keep it from the sums.  Its scale is replaced, and rows that see it get a NaN by way of a
-                // product of their own (a block has all channels of a lane).
-                if (partly) {
-                    uint32_t largest = 0;
+                // Values that are no finite numbers: a weight of zero would not keep them from the sums of rows that do not see them, nor a second number of the other sign
+                // leave an infinity what it is.  They are taken out, and which of them a row sees is counted by a product of its own, as attention_kernel does.
+                uint32_t largest = 0; // scale
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) largest = std::max(largest, unit[i]);
-                    if (__builtin_expect(__builtin_amdgcn_ballot_w64(largest == 0x7f800000u) != 0, 0)) {
-                        const int32_t see = std::min(last, until - 1) - key0 - quad;
-                        const uint32_t one = T::narrow1(1.0f);
-                        u32x4 seen, mark; // 1 where the row sees the key, where the key's block is NaN
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const int key = (w >> 1) * 16 + (w & 1) * 8;
-                            seen[w] = (one & ~(uint32_t)((see - key) >> 31)) | ((one & ~(uint32_t)((see - key - 4) >> 31)) << 16);
+                    for (int i = 0; i < Step<D>::kScales; ++i) largest = std::max(largest, s.v_scale[t][i]);
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(largest > 127 + Mfma<T>::kMostExponent) != 0, 0)) {
+                    constexpr uint32_t X = Mfma<T>::kExponent, M = Mfma<T>::kMantissa;
+                    const int32_t see = std::min(last, until - 1) - key0 - quad;
+                    const uint32_t one = T::narrow1(1.0f);
+                    u32x4 seen; // 1 where the row sees the key
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int key = (w >> 1) * 16 + (w & 1) * 8;
+                        seen[w] = (one & ~(uint32_t)((see - key) >> 31)) | ((one & ~(uint32_t)((see - key - 4) >> 31)) << 16);
+                    }
+                    if constexpr (__is_same(T, F16)) { // whole blocks are NaN, and a lane's channels are of one block
+                        u32x4 mark;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
                             mark[w] = one * ((unit[2 * w] + 0x00800000u) >> 31) | (one * ((unit[2 * w + 1] + 0x00800000u) >> 31)) << 16;
-                        }
                         const f32x4 found = Mfma<T>::mul(mark, seen, f32x4{0, 0, 0, 0});
 #pragma unroll
                         for (int c = 0; c < E; ++c)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) o[c][r] += found[r] != 0.0f ? __builtin_nanf("") : 0.0f;
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) unit[i] &= ((unit[i] + 0x00800000u) >> 31) - 1; // an infinity: 0
+                        for (int b = 0; b < E / 2; ++b) {
+                            u32x4 vf[2];
+                            operands(b, vf);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                __builtin_amdgcn_sched_barrier(0); // one after the other: interleaved they take too many registers
+                                u32x4 mark;
+#pragma unroll
+                                for (int w = 0; w < 4; ++w) {
+                                    uint32_t marks = 0;
+#pragma unroll
+                                    for (int half = 0; half < 32; half += 16) {
+                                        const uint32_t x = (vf[h][w] >> half) & 0xffffu;
+                                        const uint32_t code = (x & M) != 0 ? T::narrow1(16384.0f) : ((x & 0x8000u) != 0 ? T::narrow1(128.0f) : T::narrow1(1.0f));
+                                        marks |= ((x & X) == X ? code : 0u) << half;
+                                    }
+                                    mark[w] = marks;
+                                }
+                                const f32x4 found = Mfma<T>::mul(mark, seen, f32x4{0, 0, 0, 0});
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) o[b * 2 + h][r] += found_adds(found[r]);
+                                asm volatile("" : "+v"(o[b * 2 + h])); // now, not once all channels' marks have been found
+                            }
+                        }
+                    }
+                    // codes that are infinities become 0, and so do NaN blocks' scales
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if constexpr (__is_same(T, Bf16)) {
+#pragma unroll
+                            for (int j = 0; j < (E + 7) / 8; ++j) {
+                                const uint32_t two = s.v[i].w[j] >> 2 & 0x11111111u, four = two & s.v[i].w[j] >> 1; // from there on, a bit for each
+                                s.v[i].w[j] &= ~((unit[i] == 0x7f000000u ? two : (unit[i] == 0x7e800000u ? four : 0u)) * 15u);
+                            }
+                        }
+                        unit[i] &= ((unit[i] + 0x00800000u) >> 31) - 1;
                     }
                 }
 #pragma unroll

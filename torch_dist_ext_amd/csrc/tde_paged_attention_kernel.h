@@ -39,6 +39,7 @@ struct Mfma<Bf16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
     static constexpr uint32_t kExponent = 0x7f80u, kMantissa = 0x007fu;
+    static constexpr uint32_t kMostExponent = 125; // of a scale with which all codes are finite
     static constexpr float kLag = 8.0f, kRaise = 0.0f; // see where weights are computed
     // Two numbers within a step of x0 and x1, where another operand takes what is left.
     static __device__ __forceinline__ uint32_t part(float x0, float x1) { return Bf16::narrow(x0, x1); }
@@ -54,6 +55,7 @@ struct Mfma<F16> {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
     static constexpr uint32_t kExponent = 0x7c00u, kMantissa = 0x03ffu;
+    static constexpr uint32_t kMostExponent = 13;
     static constexpr float kLag = 4.0f, kRaise = 11.0f;
     static __device__ __forceinline__ uint32_t part(float x0, float x1) { // towards zero: one instruction for both, to nearest it is three
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
@@ -66,7 +68,7 @@ struct Mfma<F16> {
 // What a scale's byte counts as where codes become numbers of T: blocks whose 6 is no number of fp16 are NaN there.
 template <class T>
 __device__ __forceinline__ uint32_t read_scale(uint32_t e) {
-    return __is_same(T, F16) && e > 127 + 13 ? 255 : e;
+    return __is_same(T, F16) && e > 127 + Mfma<F16>::kMostExponent ? 255 : e;
 }
 
 __device__ __forceinline__ uint32_t load_byte(const char *p) { return *(const __attribute__((address_space(1))) uint8_t *)p; }
@@ -257,6 +259,14 @@ template <class C>
 __device__ __forceinline__ const typename C::Args &late_arguments([[maybe_unused]] const typename C::Args &a) {
     if constexpr (C::kFp4) return arguments_again<typename C::Args>();
     else return a;
+}
+
+// What values that are not finite add up to, 0 where there is none; found: 1 for each +inf, 128 for each -inf, 16384 for each NaN, of 64 keys at most.
+__device__ __forceinline__ float found_adds(float found) {
+    const uint32_t f = (uint32_t)found;
+    float add = (f & 127u) != 0 ? __builtin_inff() : 0.0f;
+    add -= (f & (16384u - 128u)) != 0 ? __builtin_inff() : 0.0f;
+    return f >= 16384u ? __builtin_nanf("") : add;
 }
 
 // Until at most N loads are outstanding.
@@ -836,7 +846,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
         };
         if (__builtin_expect(poisoned, 0)) {
             // A weight of zero does not keep an infinity or NaN from the product.  Such values are taken out of the tile, and which
-            // of them a row sees is counted by a product of its own: 1 for +inf, 128 for -inf, 16384 for NaN, 64 keys at most.
+            // of them a row sees is counted by a product of its own (found_adds).
             constexpr uint32_t E = Mfma<T>::kExponent, M = Mfma<T>::kMantissa;
 #pragma unroll 1
             for (int ks = 0; ks < KT / 32; ++ks) {
@@ -872,13 +882,7 @@ __global__ void __launch_bounds__(64 * WAVES, workgroups_a_unit(C::kFp4, D, NB, 
                     for (int n = 0; n < NB; ++n) {
                         const f32x4 found = Mfma<T>::mul(mark, seen[n], f32x4{0, 0, 0, 0});
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const uint32_t f = (uint32_t)found[r];
-                            // 0, or the infinity or NaN that the found values add up to
-                            float add = (f & 127u) != 0 ? __builtin_inff() : 0.0f;
-                            add -= (f & (16384u - 128u)) != 0 ? __builtin_inff() : 0.0f;
-                            o[n][d][r] += f >= 16384u ? __builtin_nanf("") : add;
-                        }
+                        for (int r = 0; r < 4; ++r) o[n][d][r] += found_adds(found[r]);
                         asm volatile("" : "+v"(o[n][d])); // now, not once all channels' marks have been found
                     }
                 }
