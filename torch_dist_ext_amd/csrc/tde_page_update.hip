@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(1024) page_update_kernel(const PageUpdateArgs 
         const Lengths l = seq < a.seqs ? lengths_of(a, seq) : Lengths{};
         const uint32_t more = seq < a.seqs ? (uint32_t)max(a.added[seq], 0) : 0;
         const uint32_t then = l.keep + more; // below 2^32
-        const uint32_t need_pages = then <= 0x7fffffffu ? pages_of(a, then) : kAny;
+        const uint32_t need_pages = then <= 0x7fffffffu ? pages_of(a, then) : 0x80000000u; // which no row of the table has
         const bool fits = need_pages <= (uint32_t)a.width;
         const uint32_t need = fits && more != 0 ? need_pages - l.kept_pages : 0;
         const uint32_t most_pages = there + 1, most_rows = (uint32_t)a.tokens + 1;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(THREADS) page_update_once_kernel(const PageUpd
     const uint32_t more = there_is ? (uint32_t)max(a.added[tid], 0) : 0;
     const uint32_t before = (uint32_t)min(max(*a.count, 0), a.capacity);
     const uint32_t then = l.keep + more; // below 2^32
-    const uint32_t need_pages = then <= kAny ? pages_of(a, then) : kAny;
+    const uint32_t need_pages = then <= 0x7fffffffu ? pages_of(a, then) : 0x80000000u; // which no row of the table has
     const bool fits = need_pages <= (uint32_t)a.width;
     const uint32_t need = fits && more != 0 ? need_pages - l.kept_pages : 0;
 
