@@ -19,7 +19,8 @@ namespace {
 template <int N>
 using Is = std::integral_constant<int, N>;
 
-__device__ __forceinline__ uint32_t add_up_to(uint32_t x, uint32_t y, uint32_t most) { return min(x + y, most); } // x, y <= most < 2^31 + 1
+// x + y, most at most, whatever they are: the addition ends at 2^32 - 1.
+__device__ __forceinline__ uint32_t add_up_to(uint32_t x, uint32_t y, uint32_t most) { return min(__builtin_elementwise_add_sat(x, y), most); }
 
 struct Sums {
     uint32_t upto[2], all[2]; // inclusive, and over the workgroup
