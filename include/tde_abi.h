@@ -385,6 +385,7 @@ int tde_paged_attention(const tde_attention *attention, void *hip_stream);
    significant bits (from 1.75 of a power of two on it is the next one's), less 2, and lies between -125 and the largest whose 6 is a number of
    `dtype` (125, fp16 13); a channel is the nearest code to its quotient, the even code of two as near, 6 at most.  A block with an infinity or a NaN
    becomes NaN (scale 255, codes 0).  Keys are normed and rotated in 64 bits, so that only a channel's exact value decides; queries as by tde_append_kv.
+   Two rows of one call with one slot leave codes and scales of either in it, not always of the same one.
    Codes and scales need no alignment; no byte of the four tensors twice, apart from each other and the inputs. */
 typedef struct tde_append_fp4 {
     tde_head_rows rows;
@@ -393,8 +394,8 @@ typedef struct tde_append_fp4 {
 } tde_append_fp4;
 int tde_append_kv_fp4(const tde_append_fp4 *append, void *hip_stream);
 
-/* As tde_paged_attention; keys and values enter as numbers of `dtype`: exact in bf16 (down to 2^-133); in fp16 to 2^-25 below 2^-14, and blocks
-   whose 6 it does not hold (scales from 141 on) are NaN.  Codes: data and strides multiples of 16 bytes (TDE_EALIGN); scales need no alignment; page and slot strides below 2^31 bytes (TDE_ESHAPE).
+/* As tde_paged_attention; keys and values enter as numbers of `dtype`: exact in bf16 (down to 2^-133, infinities from 2^128 on); in fp16 to 2^-25 below
+   2^-14, and blocks whose 6 it does not hold (scales from 141 on) are NaN.  Codes: data and strides multiples of 16 bytes (TDE_EALIGN); scales need no alignment; page and slot strides below 2^31 bytes (TDE_ESHAPE).
    The workspace is tde_paged_attention_fp4_workspace bytes. */
 typedef struct tde_attention_fp4 {
     tde_attention attention;
@@ -405,7 +406,7 @@ int tde_paged_attention_fp4_workspace(const tde_attention_fp4 *attention, int64_
 int tde_paged_attention_fp4(const tde_attention_fp4 *attention, void *hip_stream);
 
 /* out[i][j][k][d] = T(code * scale), rounded to nearest: rows of `dim` channels in up to three dimensions.  code_strides and scale_strides in bytes, from
-   one row to the next in each dimension; out is contiguous and takes its element's alignment.  The number of rows is below 2^31. */
+   one row to the next in each dimension; out is contiguous and takes its element's alignment.  The number of rows times dim / 8 is below 2^31 (TDE_ETOOBIG). */
 typedef struct tde_unpack_fp4_rows {
     int64_t sizes[3];
     int64_t code_strides[3], scale_strides[3];

@@ -114,7 +114,8 @@ struct Shares {
 // SPAN: keys in a row that are known to lie in one page, 16 or 8; their address is scalar.
 //
 // All units of all tiles, in order, go to as many workgroups as the device holds at once, the same number to each: whatever the lengths, none has more than
-// another, and none begins when others have ended.  (A workgroup for each tile, long ones cut at one length: 64 rows over up to 8192 keys 72 us.)  A workgroup
+// another, and none begins when others have ended.  (A workgroup for each tile, long ones cut at one length: 64 rows over up to 8192 keys 72 us.)  Only where
+// tiles alone fill the device twice is each a workgroup's, however long it is (plan_attention_fp4).  A workgroup
 // has the end of one tile, whole ones, and the beginning of another; where runners are many and tiles few, tiles begin where a runner does, which has one part then
 // (48 sequences of 3 rows over up to 6000 keys 27.9 us, and 31.2 without; one row over 262144 19.2 and 22.4; 64 over up to 8192 66, and 86 if they did).
 // What is cut is joined by a second launch.  Parts go to places of the workgroup's own: 2r for the tile that others began, 2r + 1 for the one that others end.
@@ -838,7 +839,9 @@ namespace {
 // Which kernel.  Calls whose sequences have few rows on average go to the decode kernel, tiles of 16 rows; the others to tiles of 64 and more.  How many are few:
 // 16; with heads of up to 64 channels 32 where tiles of 64 would leave units idle (48 sequences of 6 x 4 rows over 6000 keys 55 us, tiles of 64 69; but 300 over
 // 600 85 and 76), of up to 128 32 (64 sequences of 8 x 4 over 4000 115 and 120, of up to as many 69 and 94; with 48 153 and 121), of more 96, as tiles of 64
-// leave them one wavefront a SIMD (20 of 8 x 6 over 6000 97 and 155, of 24 x 4 over 6000 171 and 351; 64 of up to 30 x 4 over 500 57 and 52).
+// leave them one wavefront a SIMD (20 of 8 x 6 over 6000 97 and 155, of 24 x 4 over 6000 171 and 351; 64 of up to 30 x 4 over 500 57 and 52).  The average decides for all
+// rows: a chunk beside many single rows goes to tiles of 16 as well, single rows beside a long chunk to large ones (4 heads a key head, up to 2000 keys, the chunk behind
+// 1000: 255 rows and 1500 206 us, in two calls 82 and 98; 60 and 400 62, 36 and 41; 63 and 4000, large tiles, 268, 36 and 204; in heads of 256 60 and 1500 276, 54 and 161).
 int64_t few_rows(int wide_dim, int64_t tiles) {
     return wide_dim == 256 ? 96 : (wide_dim == 128 || tiles < device_compute_units() ? 32 : 16);
 }
@@ -892,6 +895,8 @@ int plan_attention_fp4(int dim, int64_t tokens, int q_heads, int kv_heads, const
     const int64_t at_once = std::max<int64_t>(1, std::min<int64_t>((int64_t)resident_workgroups(p->wide_dim, b.page_size % 16 == 0 ? 16 : 8) * device_compute_units() / kv_heads, kMostRunners));
     const int64_t likely = std::max<int64_t>({1, std::min<int64_t>(b.seqs, tokens), rows_all / 16}); // tiles
     // Where tiles alone fill the device more than twice each is a runner's, and nothing is cut (200 rows over 1500 keys 52 us and 61, 512 over 2047 216 and 225).
+    // Lengths, which are the device's, do not count: one that is far longer than the others is walked by a workgroup for each key head (200 rows over 500 keys 35 us,
+    // with 131072 keys in one of them 943; 191 rows, which are shared out, 34 and 75).
     p->whole_tiles = likely >= 2 * at_once;
     p->runners = p->whole_tiles ? tiles : std::min(at_once >= 8 ? at_once & ~(int64_t)7 : at_once, (tiles * most + kDecodeWaves - 1) / kDecodeWaves);
     p->split = !p->whole_tiles && most > kDecodeWaves;
